@@ -29,6 +29,8 @@ EXPORTS = (
     "xnor_b200_float_conv_map_prepare", "xnor_b200_float_conv_map", "xnor_b200_float_conv_map_yolo", "xnor_b200_float_conv_1x1_tc", "xnor_b200_yolo_activate", "xnor_b200_region_activate", "xnor_b200_conv_forward_io", "xnor_b200_conv_takes_masks", "xnor_b200_tap_major_weights",
     "xnor_b200_yolo_detections", "xnor_b200_nms_sort", "xnor_b200_detection_rows", "xnor_b200_detect", "xnor_b200_rows_to_host",
     "xnor_b200_avgpool", "xnor_b200_softmax", "xnor_b200_run_ops", "xnor_b200_float_conv3_words", "xnor_b200_float_conv_tc", "xnor_b200_float_conv_tc_launches", "xnor_b200_float_conv_tc_prepare", "xnor_b200_float_conv_tc_weights_bytes", "xnor_b200_conv_words", "xnor_b200_conv_words_plan", "xnor_b200_conv_words_weights", "xnor_b200_conv_words_weights_bytes", "xnor_b200_sign_words", "xnor_b200_grid_block_words", "xnor_b200_grid_front",
+    "xnor_b200_w4_code_bytes", "xnor_b200_w4_scale_bytes", "xnor_b200_w4_quantize", "xnor_b200_w4_forward",
+    "xnor_b200_kv4_append", "xnor_b200_kv4_read", "xnor_b200_kv4_attend_scratch_bytes", "xnor_b200_kv4_attend",
     "xnor_b200_measure_popc_peak", "xnor_b200_measure_bmma_peak", "xnor_b200_measure_umma_i8_peak", "xnor_b200_measure_umma_mxf4_peak",
 )
 
@@ -111,6 +113,31 @@ class ConvGeom(C.Structure):
     """struct xnor_b200_conv_geom"""
     _fields_ = [(n, C.c_int) for n in ("out_h", "out_w", "n_out", "k", "new_lda", "bit_align", "word_path")] + \
                [("weights_bytes", C.c_size_t), ("packed_input_bytes", C.c_size_t), ("output_floats", C.c_size_t)]
+
+
+F32, F16, BF16 = 0, 1, 2
+KV4_MAX_DIM = 256               # XNOR_B200_KV4_MAX_DIM
+
+
+class W4Desc(C.Structure):
+    """struct xnor_b200_w4_desc"""
+    _fields_ = [(n, C.c_int) for n in ("n", "k", "group", "activation")]
+
+
+class Kv4Cache(C.Structure):
+    """struct xnor_b200_kv4_cache"""
+    _fields_ = [(n, C.c_void_p) for n in ("k_codes", "k_scales", "v_codes", "v_scales")] + \
+               [(n, C.c_int) for n in ("pages", "kv_heads", "page", "dim", "group")]
+
+
+class Kv4Rows(C.Structure):
+    """struct xnor_b200_kv4_rows"""
+    _fields_ = [(n, C.c_int) for n in ("batch", "tokens", "max_pages")] + [(n, C.c_void_p) for n in ("table", "lengths", "counts")]
+
+
+class Kv4Tensor(C.Structure):
+    """struct xnor_b200_kv4_tensor"""
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int)] + [(n, C.c_longlong) for n in ("stride_sequence", "stride_token", "stride_head")]
 
 
 class XnorError(RuntimeError):
@@ -200,6 +227,18 @@ def lib() -> C.CDLL:
     L.xnor_b200_measure_bmma_peak.argtypes = [ci, C.POINTER(C.c_double), C.POINTER(C.c_double)]
     L.xnor_b200_measure_umma_i8_peak.argtypes = [ci, C.POINTER(C.c_double), C.POINTER(C.c_double)]
     L.xnor_b200_measure_umma_mxf4_peak.argtypes = [ci, C.POINTER(C.c_double), C.POINTER(C.c_double)]
+    wp, kp, rp, tp, ll = C.POINTER(W4Desc), C.POINTER(Kv4Cache), C.POINTER(Kv4Rows), C.POINTER(Kv4Tensor), C.c_longlong
+    L.xnor_b200_w4_code_bytes.restype = sz
+    L.xnor_b200_w4_code_bytes.argtypes = [wp]
+    L.xnor_b200_w4_scale_bytes.restype = sz
+    L.xnor_b200_w4_scale_bytes.argtypes = [wp]
+    L.xnor_b200_w4_quantize.argtypes = [wp, vp, ci, ll, vp, vp, vp]
+    L.xnor_b200_w4_forward.argtypes = [wp, vp, ci, ci, ll, vp, vp, vp, vp, ll, vp]
+    L.xnor_b200_kv4_append.argtypes = [kp, rp, tp, tp, vp]
+    L.xnor_b200_kv4_read.argtypes = [kp, rp, tp, tp, vp]
+    L.xnor_b200_kv4_attend_scratch_bytes.restype = sz
+    L.xnor_b200_kv4_attend_scratch_bytes.argtypes = [kp, rp, ci, ci]
+    L.xnor_b200_kv4_attend.argtypes = [kp, rp, tp, ci, C.c_float, ci, tp, vp, vp, sz, vp]
     _lib = L
     return L
 

@@ -1,0 +1,238 @@
+"""Four-bit matrices and token caches, over the C ABI: the fully connected products and the attention of a network that answers token by token.
+
+    m = quantize_weights4(weights, group)              # load time: codes and (scale, low) pairs
+    y = forward_connected4(m, x, biases, activation)   # forward_connected_layer (src-lib/connected_layer.cpp) for a few rows
+    c = new_cache4(pages, kv_heads, page, dim, group)
+    append4(c, k, v, table, lengths)                   # the newest tokens of every sequence into their pages
+    out = attend4(c, q, table, lengths)                # their attention over all that their sequences hold
+
+The format, and what a row of tokens stands for, are written down in include/xnor_b200.h.  torch is used for device memory and the
+current stream only; every computation is a call into libxnor_b200.so.  Nothing here has a CPU path.  Calls are asynchronous, run on the
+current stream of the tensors' device and may be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Optional
+
+import torch
+
+from . import capi
+
+_DTYPES = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
+_GROUPS = (32, 64, 128)
+
+
+def _dtype(t: torch.Tensor, what: str) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} must be fp32, fp16 or bf16, not {t.dtype}")
+    return code
+
+
+def _on(device: torch.device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {t.device} and {device}: all of a call's tensors are on one CUDA device")
+
+
+class _Device:
+    """Makes a tensor's device the current one, where it is another, and names its current stream."""
+
+    def __init__(self, device: torch.device) -> None:
+        if device.type != "cuda":
+            raise ValueError(f"tensors on {device}: this path runs on a CUDA device only")
+        self.index = device.index
+        self.before = None
+
+    def __enter__(self) -> int:
+        if torch._C._cuda_getDevice() != self.index:
+            self.before = torch.cuda._exchange_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *_) -> None:
+        if self.before is not None:
+            torch.cuda._exchange_device(self.before)
+
+
+class Matrix4:
+    """A packed matrix of n rows of k values (struct xnor_b200_w4_desc with its two buffers): codes uint8 [n][ceil(k/32)*16], scales fp16
+    [n][ceil(k/group)][2], both contiguous."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, k: int, group: int) -> None:
+        if group not in _GROUPS:
+            raise ValueError(f"group must be one of {_GROUPS}, not {group}")
+        if codes.dim() != 2 or codes.dtype != torch.uint8 or k <= 0 or codes.shape[0] == 0 or codes.shape[1] != (k + 31) // 32 * 16 or not codes.is_contiguous():
+            raise ValueError(f"codes must be contiguous uint8 [n][{(k + 31) // 32 * 16}] for rows of {k} values")
+        if scales.dtype != torch.float16 or scales.shape != (codes.shape[0], (k + group - 1) // group, 2) or not scales.is_contiguous():
+            raise ValueError(f"scales must be contiguous fp16 [{codes.shape[0]}][{(k + group - 1) // group}][2]")
+        _on(codes.device, scales)
+        self.codes, self.scales, self.n, self.k, self.group = codes, scales, codes.shape[0], k, group
+        self._descs = {a: capi.W4Desc(self.n, k, group, a) for a in (capi.LINEAR, capi.LEAKY)}
+
+
+def quantize_weights4(weights: torch.Tensor, group: int) -> Matrix4:
+    """Packs a matrix [n][k] (rows contiguous) to four bits: xnor_b200_w4_quantize."""
+    if weights.dim() != 2 or weights.numel() == 0 or (weights.stride(1) != 1 and weights.shape[1] != 1):
+        raise ValueError("weights must be a matrix [n][k] with contiguous rows")
+    if group not in _GROUPS:
+        raise ValueError(f"group must be one of {_GROUPS}, not {group}")
+    n, k = weights.shape
+    dtype = _dtype(weights, "weights")
+    with _Device(weights.device) as stream:
+        codes = torch.empty(n, (k + 31) // 32 * 16, dtype=torch.uint8, device=weights.device)
+        scales = torch.empty(n, (k + group - 1) // group, 2, dtype=torch.float16, device=weights.device)
+        m = Matrix4(codes, scales, k, group)
+        capi.check(capi.lib().xnor_b200_w4_quantize(C.byref(m._descs[capi.LINEAR]), weights.data_ptr(), dtype, weights.stride(0) if n > 1 else k,
+                                                   codes.data_ptr(), scales.data_ptr(), stream), "xnor_b200_w4_quantize")
+    return m
+
+
+def forward_connected4(m: Matrix4, x: torch.Tensor, biases: Optional[torch.Tensor] = None, activation: int = capi.LINEAR,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x @ W.T + biases) for x [rows][k] (rows contiguous, any distance apart), W the packed matrix: xnor_b200_w4_forward.
+    biases: fp32 [n].  out: [rows][n] of x's type, rows contiguous; made where it is not given.  One pass over the weights serves up to
+    16 rows."""
+    if x.dim() != 2 or x.shape[1] != m.k or (x.stride(1) != 1 and m.k != 1):
+        raise ValueError(f"x must be [rows][{m.k}] with contiguous rows")
+    dtype, rows = _dtype(x, "x"), x.shape[0]
+    if activation not in m._descs:
+        raise ValueError("activation must be capi.LINEAR or capi.LEAKY")
+    if biases is not None and (biases.dtype != torch.float32 or biases.shape != (m.n,) or not biases.is_contiguous()):
+        raise ValueError(f"biases must be contiguous fp32 [{m.n}]")
+    if out is not None and (out.dtype != x.dtype or out.shape != (rows, m.n) or (out.stride(1) != 1 and m.n != 1)):
+        raise ValueError(f"out must be {x.dtype} [{rows}][{m.n}] with contiguous rows")
+    _on(x.device, m.codes, biases, out)
+    with _Device(x.device) as stream:
+        if out is None:
+            out = torch.empty(rows, m.n, dtype=x.dtype, device=x.device)
+        if rows == 0:
+            return out
+        rc = capi.lib().xnor_b200_w4_forward(m._descs[activation], x.data_ptr(), dtype, rows, x.stride(0) if rows > 1 else m.k, m.codes.data_ptr(),
+                                             m.scales.data_ptr(), None if biases is None else biases.data_ptr(), out.data_ptr(),
+                                             out.stride(0) if rows > 1 else m.n, stream)
+        if rc:
+            capi.check(rc, "xnor_b200_w4_forward")
+    return out
+
+
+class Cache4:
+    """Pages of four-bit keys and values (struct xnor_b200_kv4_cache): codes uint8 [pages][kv_heads][page][dim/2], scales fp16
+    [pages][kv_heads][page][dim/group][2], contiguous."""
+
+    def __init__(self, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor, group: int) -> None:
+        if group not in _GROUPS:
+            raise ValueError(f"group must be one of {_GROUPS}, not {group}")
+        if k_codes.dim() != 4 or 0 in k_codes.shape:
+            raise ValueError("codes must be [pages][kv_heads][page][dim/2]")
+        pages, kv_heads, page, half = k_codes.shape
+        dim = 2 * half
+        if page % 16 or dim % 32 or dim % group or dim > capi.KV4_MAX_DIM:
+            raise ValueError(f"page must be a multiple of 16, dim one of 32 and of the group, at most {capi.KV4_MAX_DIM}: got page {page}, dim {dim}, group {group}")
+        for codes, scales in ((k_codes, k_scales), (v_codes, v_scales)):
+            if codes.dtype != torch.uint8 or codes.shape != k_codes.shape or not codes.is_contiguous():
+                raise ValueError(f"codes of keys and values must be contiguous uint8 {list(k_codes.shape)}")
+            if scales.dtype != torch.float16 or scales.shape != (pages, kv_heads, page, dim // group, 2) or not scales.is_contiguous():
+                raise ValueError(f"scales must be contiguous fp16 {[pages, kv_heads, page, dim // group, 2]}")
+        _on(k_codes.device, k_scales, v_codes, v_scales)
+        self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
+        self.pages, self.kv_heads, self.page, self.dim, self.group, self.device = pages, kv_heads, page, dim, group, k_codes.device
+
+    def struct(self) -> capi.Kv4Cache:
+        """Made for every call, so that it never names memory of a tensor that was replaced."""
+        return capi.Kv4Cache(self.k_codes.data_ptr(), self.k_scales.data_ptr(), self.v_codes.data_ptr(), self.v_scales.data_ptr(), self.pages,
+                             self.kv_heads, self.page, self.dim, self.group)
+
+
+def new_cache4(pages: int, kv_heads: int, page: int, dim: int, group: int, device="cuda:0") -> Cache4:
+    """An empty cache (zeros)."""
+    def buffer(*shape, dtype):
+        return torch.zeros(pages, kv_heads, page, *shape, dtype=dtype, device=device)
+    if group not in _GROUPS:
+        raise ValueError(f"group must be one of {_GROUPS}, not {group}")
+    return Cache4(buffer(dim // 2, dtype=torch.uint8), buffer(dim // group, 2, dtype=torch.float16), buffer(dim // 2, dtype=torch.uint8),
+                  buffer(dim // group, 2, dtype=torch.float16), group)
+
+
+def _rows(c: Cache4, batch: int, tokens: int, table: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor]) -> capi.Kv4Rows:
+    if table.dim() != 2 or table.shape[0] != batch or table.shape[1] == 0 or table.dtype != torch.int32 or not table.is_contiguous():
+        raise ValueError(f"table must be contiguous int32 [{batch}][pages of a sequence]")
+    for name, t in (("lengths", lengths), ("counts", counts)):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (batch,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous int32 [{batch}]")
+    _on(c.device, table, lengths, counts)
+    return capi.Kv4Rows(batch, tokens, table.shape[1], table.data_ptr(), lengths.data_ptr(), None if counts is None else counts.data_ptr())
+
+
+def _tensor(t: torch.Tensor, what: str) -> capi.Kv4Tensor:
+    if t.stride(3) != 1 and t.shape[3] != 1:
+        raise ValueError(f"the last dimension of {what} must be contiguous")
+    return capi.Kv4Tensor(t.data_ptr(), _dtype(t, what), t.stride(0), t.stride(1), t.stride(2))
+
+
+def append4(c: Cache4, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor] = None) -> None:
+    """Packs the newest tokens' keys and values [batch][tokens][kv_heads][dim] into their pages: xnor_b200_kv4_append.  lengths: what each
+    sequence holds with them; counts: how many of the rows are tokens (default: all), the first ones of each sequence.  table: int32
+    [batch][pages of a sequence].  No two rows may share a place."""
+    if k.dim() != 4 or k.shape[2:] != (c.kv_heads, c.dim) or v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError(f"k and v must be [batch][tokens][{c.kv_heads}][{c.dim}] of one type")
+    _on(c.device, k, v)
+    if k.numel() == 0:
+        return
+    rows = _rows(c, k.shape[0], k.shape[1], table, lengths, counts)
+    kt, vt = _tensor(k, "k"), _tensor(v, "v")
+    with _Device(c.device) as stream:
+        rc = capi.lib().xnor_b200_kv4_append(c.struct(), rows, kt, vt, stream)
+        if rc:
+            capi.check(rc, "xnor_b200_kv4_append")
+
+
+def read4(c: Cache4, table: torch.Tensor, lengths: torch.Tensor, tokens: int, counts: Optional[torch.Tensor] = None, dtype=torch.float32):
+    """What the cache holds for the last `tokens` positions (or counts[b] of them) of every sequence, as keys and values [batch][tokens][kv_heads][dim]:
+    xnor_b200_kv4_read.  Rows that stand for no token are 0."""
+    if dtype not in _DTYPES:
+        raise ValueError(f"dtype must be fp32, fp16 or bf16, not {dtype}")
+    if table.dim() != 2 or tokens < 0:
+        raise ValueError("table must be int32 [batch][pages of a sequence], tokens at least 0")
+    with _Device(c.device) as stream:
+        k = torch.empty(table.shape[0], tokens, c.kv_heads, c.dim, dtype=dtype, device=c.device)
+        v = torch.empty_like(k)
+        if k.numel():
+            rc = capi.lib().xnor_b200_kv4_read(c.struct(), _rows(c, table.shape[0], tokens, table, lengths, counts), _tensor(k, "k"), _tensor(v, "v"), stream)
+            if rc:
+                capi.check(rc, "xnor_b200_kv4_read")
+    return k, v
+
+
+def attend4(c: Cache4, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor] = None,
+            scale: Optional[float] = None, window: int = 0, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the newest tokens' queries [batch][tokens][heads][dim] over what their sequences hold, those tokens among it (append4
+    comes first): xnor_b200_kv4_attend.  scale: 1/sqrt(dim) where not given.  window: positions that a token sees, itself among them
+    (0: all).  Rows that see nothing are 0.  out: as q; made where it is not given.  lse: fp32 [batch][tokens][heads], contiguous, receives
+    the logarithm of each row's sum of exponentials."""
+    if q.dim() != 4 or q.shape[3] != c.dim or q.shape[2] == 0 or q.shape[2] % c.kv_heads:
+        raise ValueError(f"q must be [batch][tokens][heads][{c.dim}], heads a multiple of {c.kv_heads}")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
+        raise ValueError(f"out must be {q.dtype} {list(q.shape)}")
+    if out is not None and torch._debug_has_internal_overlap(out) == 1:
+        raise ValueError("out has rows that share memory")
+    if lse is not None and (lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous()):
+        raise ValueError(f"lse must be contiguous fp32 {list(q.shape[:3])}")
+    if window < 0:
+        raise ValueError("window must be at least 0")
+    _on(c.device, q, out, lse)
+    batch, tokens, heads = q.shape[:3]
+    with _Device(c.device) as stream:
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if q.numel() == 0:
+            return out
+        cache, rows, L = c.struct(), _rows(c, batch, tokens, table, lengths, counts), capi.lib()
+        nbytes = L.xnor_b200_kv4_attend_scratch_bytes(cache, rows, heads, window)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        rc = L.xnor_b200_kv4_attend(cache, rows, _tensor(q, "q"), heads, 1.0 / math.sqrt(c.dim) if scale is None else scale, window, _tensor(out, "out"),
+                                    None if lse is None else lse.data_ptr(), None if scratch is None else scratch.data_ptr(), nbytes, stream)
+        if rc:
+            capi.check(rc, "xnor_b200_kv4_attend")
+    return out

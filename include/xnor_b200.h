@@ -572,6 +572,101 @@ XNOR_B200_API int xnor_b200_measure_umma_i8_peak(int iters, double * gops, doubl
  * tensor-core kernel. */
 XNOR_B200_API int xnor_b200_measure_umma_mxf4_peak(int iters, double * gops, double * ms);
 
+/* ---- four bits a value ------------------------------------------------------------------------------------------------
+ * Matrices and token caches packed as the sign tensors above are, with four bits where one says too little: fully connected layers
+ * of one to some rows, and the attention of a network that answers token by token.
+ *
+ * One format for both.  A row of values lies in groups of `group` neighbours (32, 64 or 128); each group has a pair of fp16 numbers
+ * (scale, low), and value = low + scale * code with code 0..15.  Byte b of a row: code 2b in the low four bits, 2b + 1 in the high.
+ * Packing takes low = the group's minimum rounded down to fp16 and scale = (maximum - low) / 15 rounded up, code = the nearest (half
+ * to even): nothing is clipped and every value comes back within half a scale.  NaN counts as 0, magnitudes above 65504 as 65504.
+ * Codes with a zero point in the middle, scale * (code - 8), are low = -8 * scale.
+ *
+ * Types of the tensors that go in and out: */
+#define XNOR_B200_F32  0
+#define XNOR_B200_F16  1
+#define XNOR_B200_BF16 2
+
+/* A matrix of n rows (filters) of k values: codes n * ceil(k/32)*16 bytes (16-byte aligned; bits behind k are 0 when packed here and
+ * never matter), scales [n][ceil(k/group)][2] fp16.  activation: of the layer's output, XNOR_B200_LINEAR or XNOR_B200_LEAKY. */
+#define XNOR_B200_W4_MAX_K    (1 << 24)
+#define XNOR_B200_W4_MAX_N    (1 << 28)
+#define XNOR_B200_W4_MAX_ROWS (1 << 16)
+typedef struct xnor_b200_w4_desc
+{
+	int n, k;
+	int group;
+	int activation;
+} xnor_b200_w4_desc;
+
+/* Bytes of codes and of scales; 0 for a descriptor that is not valid. */
+XNOR_B200_API size_t xnor_b200_w4_code_bytes(const xnor_b200_w4_desc * desc);
+XNOR_B200_API size_t xnor_b200_w4_scale_bytes(const xnor_b200_w4_desc * desc);
+
+/* Load-time packing of weights [n][k] of type `dtype`, rows ld elements apart: what xnor_b200_binary_align_weights is to one bit. */
+XNOR_B200_API int xnor_b200_w4_quantize(const xnor_b200_w4_desc * desc, const void * weights, int dtype, long long ld,
+		uint8_t * codes, void * scales, void * stream);
+
+/* forward_connected_layer_gpu (src-lib/connected_layer.cpp) with such weights: output[r][i] = act(sum_j x[r][j] * value[i][j] + biases[i])
+ * for `rows` rows of x, ldx elements apart, to rows ldo elements apart, both of type `dtype`; biases fp32 [n] or NULL.  Sums are fp32,
+ * rounded once.  A row of x that holds an infinity or a NaN gives NaN.  Made for few rows (one pass over the weights serves 16).
+ * output overlaps no input. */
+XNOR_B200_API int xnor_b200_w4_forward(const xnor_b200_w4_desc * desc, const void * x, int dtype, int rows, long long ldx,
+		const uint8_t * codes, const void * scales, const float * biases, void * output, long long ldo, void * stream);
+
+/* Keys and values of tokens in pages of `page` tokens (a multiple of 16): codes [pages][kv_heads][page][dim/2] bytes, scales
+ * [pages][kv_heads][page][dim/group][2] fp16, all four 16-byte aligned.  dim: a multiple of 32, at most XNOR_B200_KV4_MAX_DIM, and
+ * of group. */
+#define XNOR_B200_KV4_MAX_DIM 256
+typedef struct xnor_b200_kv4_cache
+{
+	uint8_t * k_codes;
+	void * k_scales;
+	uint8_t * v_codes;
+	void * v_scales;
+	int pages, kv_heads, page, dim, group;
+} xnor_b200_kv4_cache;
+
+/* The newest tokens of `batch` sequences.  lengths[b]: tokens that sequence b holds, the new ones among them; counts[b]: how many are
+ * new (NULL: `tokens` of each).  Row i < counts[b] of sequence b is the token at position lengths[b] - counts[b] + i, kept at place
+ * position % page of page table[b][position / page].  Rows of counts[b] and above, positions below 0 or behind the table's last page,
+ * and pages that the cache does not have (a table may hold -1) stand for no token. */
+typedef struct xnor_b200_kv4_rows
+{
+	int batch, tokens, max_pages;
+	const int32_t * table;       /* [batch][max_pages] */
+	const int32_t * lengths;     /* [batch] */
+	const int32_t * counts;      /* [batch] or NULL */
+} xnor_b200_kv4_rows;
+
+/* A tensor [batch][tokens][heads][dim] with strides in elements; the last dimension is contiguous. */
+typedef struct xnor_b200_kv4_tensor
+{
+	void * data;
+	int dtype;
+	long long stride_sequence, stride_token, stride_head;
+} xnor_b200_kv4_tensor;
+
+/* Packs the rows' keys and values into their places; rows that stand for no token are left out.  No two rows may have the same place
+ * (sequences that share a page write it once, before they share it). */
+XNOR_B200_API int xnor_b200_kv4_append(const xnor_b200_kv4_cache * cache, const xnor_b200_kv4_rows * rows,
+		const xnor_b200_kv4_tensor * k, const xnor_b200_kv4_tensor * v, void * stream);
+/* The other way: what the cache holds for the rows, 0 for rows that stand for no token. */
+XNOR_B200_API int xnor_b200_kv4_read(const xnor_b200_kv4_cache * cache, const xnor_b200_kv4_rows * rows,
+		const xnor_b200_kv4_tensor * k, const xnor_b200_kv4_tensor * v, void * stream);
+
+/* Attention of the rows over their sequences: row i of sequence b, at position lengths[b] - counts[b] + i, sees the positions up to its
+ * own (with window > 0 the last `window` of them) that are kept in pages that the cache has; per head of `heads` (a multiple of
+ * kv_heads; heads / kv_heads neighbours share a head of keys), output = sum_j softmax_j(scale * q . k_j) v_j.  q and output:
+ * [batch][tokens][heads][dim] of one type, no memory in common.  A row that sees nothing, and rows of counts[b] and above, are 0.
+ * lse: fp32 [batch][tokens][heads] or NULL, receives log(sum_j exp(scale * q . k_j)), -infinity where nothing is seen.  Scores,
+ * softmax and sums are fp32, rounded once.  What lies behind a sequence's length in its last page is never counted.
+ * scratch: xnor_b200_kv4_attend_scratch_bytes() bytes on the current device (0: may be NULL), 16-byte aligned, of this call alone until
+ * it has run; needs no initialisation. */
+XNOR_B200_API size_t xnor_b200_kv4_attend_scratch_bytes(const xnor_b200_kv4_cache * cache, const xnor_b200_kv4_rows * rows, int heads, int window);
+XNOR_B200_API int xnor_b200_kv4_attend(const xnor_b200_kv4_cache * cache, const xnor_b200_kv4_rows * rows, const xnor_b200_kv4_tensor * q,
+		int heads, float scale, int window, const xnor_b200_kv4_tensor * output, float * lse, void * scratch, size_t scratch_bytes, void * stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,143 @@
+"""Four-bit operators without a GPU: the format's reference, sizes, and refusals that answer before anything is launched."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import four_reference as R
+
+torch = pytest.importorskip("torch")
+
+from darknet_b200 import build, capi, fourbit as F  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def L():
+    build.build()
+    return capi.lib()
+
+
+def test_the_format_clips_nothing():
+    rows = np.random.default_rng(1).standard_normal((50, 96)) * np.logspace(-7, 4, 50)[:, None]
+    codes, scales = R.quantize(rows, 32)
+    back, size = R.values(R.pack(codes), scales, 32, 96)
+    step = np.repeat(scales[..., 0].astype(np.float64), 32, -1)
+    assert (np.abs(back - rows) <= step * 0.5 * (1 + 1e-12)).all() and (size >= np.abs(back) * (1 - 1e-12)).all()
+    assert codes.min() == 0 and codes.max() == 15
+    np.testing.assert_array_equal(R.unpack(R.pack(codes), 96), codes)
+
+
+def test_sizes(L):
+    def sizes(n, k, group):
+        d = capi.W4Desc(n, k, group, 0)
+        return L.xnor_b200_w4_code_bytes(C.byref(d)), L.xnor_b200_w4_scale_bytes(C.byref(d))
+    assert sizes(10, 256, 64) == (10 * 128, 10 * 4 * 4)
+    assert sizes(3, 33, 32) == (3 * 32, 3 * 2 * 4)
+    assert sizes(3, 1, 128) == (3 * 16, 3 * 4)
+    assert sizes(1 << 20, 1 << 20, 32) == (1 << 39, 1 << 37)
+    for wrong in ((0, 8, 32), (8, 0, 32), (8, 8, 16), (8, -1, 64)):
+        assert sizes(*wrong) == (0, 0)
+    assert L.xnor_b200_w4_code_bytes(None) == 0 and L.xnor_b200_w4_scale_bytes(None) == 0
+
+
+def test_products_refuse(L):
+    d = capi.W4Desc(16, 64, 32, 0)
+
+    def forward(d=d, x=256, dtype=0, rows=1, ldx=64, codes=256, scales=256, biases=None, out=256, ldo=16):
+        return L.xnor_b200_w4_forward(None if d is None else C.byref(d), x, dtype, rows, ldx, codes, scales, biases, out, ldo, None)
+
+    for null in ("d", "x", "codes", "scales", "out"):
+        assert forward(**{null: None}) == 2
+    for wrong in (dict(dtype=3), dict(dtype=-1), dict(rows=0), dict(rows=-4), dict(ldx=-1), dict(ldo=15), dict(d=capi.W4Desc(0, 64, 32, 0)),
+                  dict(d=capi.W4Desc(16, 64, 48, 0)), dict(d=capi.W4Desc(16, 64, 32, 2)), dict(d=capi.W4Desc(16, -5, 32, 0))):
+        assert forward(**wrong) == 1, wrong
+    for odd in (dict(codes=264), dict(scales=258), dict(x=258), dict(out=258), dict(biases=257)):
+        assert forward(**odd) == 5, odd
+    assert forward(rows=(1 << 16) + 1) == 6
+    assert forward(d=capi.W4Desc(16, (1 << 24) + 1, 32, 0)) == 6
+    assert L.xnor_b200_w4_quantize(C.byref(d), None, 0, 64, 256, 256, None) == 2
+    assert L.xnor_b200_w4_quantize(C.byref(d), 256, 7, 64, 256, 256, None) == 1
+    assert L.xnor_b200_w4_quantize(C.byref(d), 256, 0, 64, 264, 256, None) == 5
+
+
+def cache(pages=4, kv_heads=2, page=16, dim=64, group=32, **pointers):
+    at = dict(k_codes=256, k_scales=256, v_codes=256, v_scales=256) | pointers
+    return capi.Kv4Cache(at["k_codes"], at["k_scales"], at["v_codes"], at["v_scales"], pages, kv_heads, page, dim, group)
+
+
+def rows(batch=1, tokens=1, max_pages=2, table=256, lengths=256, counts=None):
+    return capi.Kv4Rows(batch, tokens, max_pages, table, lengths, counts)
+
+
+def tensor(data=256, dtype=0):
+    return capi.Kv4Tensor(data, dtype, 64, 64, 64)
+
+
+def test_caches_refuse(L):
+    def every(c, r):
+        t = tensor()
+        return {L.xnor_b200_kv4_append(c, r, t, t, None), L.xnor_b200_kv4_read(c, r, t, t, None),
+                L.xnor_b200_kv4_attend(c, r, t, 4, 1.0, 0, t, None, None, 0, None)}
+
+    for c in (cache(pages=0), cache(page=8), cache(page=24), cache(dim=48), cache(group=16), cache(dim=96, group=64), cache(kv_heads=0), cache(dim=0)):
+        assert every(c, rows()) == {1}
+    for r in (rows(batch=0), rows(tokens=-1), rows(max_pages=0)):
+        assert every(cache(), r) == {1}
+    for name in ("k_codes", "k_scales", "v_codes", "v_scales"):
+        assert every(cache(**{name: None}), rows()) == {2}
+        assert every(cache(**{name: 264}), rows()) == {5}
+    assert every(cache(), rows(table=None)) == {2} and every(cache(), rows(lengths=None)) == {2}
+    assert every(cache(), rows(table=258)) == {5} and every(cache(), rows(counts=257)) == {5}
+    assert every(cache(dim=288), rows()) == {6} and every(cache(), rows(batch=1 << 16, tokens=1 << 16)) == {6}
+
+
+def test_attention_refuses(L):
+    def attend(c=cache(), r=rows(), q=tensor(), heads=4, scale=1.0, window=0, out=tensor(), lse=None, scratch=None, nbytes=0):
+        return L.xnor_b200_kv4_attend(c, r, q, heads, scale, window, out, lse, scratch, nbytes, None)
+
+    for wrong in (dict(heads=3), dict(heads=0), dict(window=-1), dict(scale=float("inf")), dict(scale=float("nan")), dict(q=tensor(dtype=1)), dict(q=tensor(dtype=4), out=tensor(dtype=4))):
+        assert attend(**wrong) == 1, wrong
+    assert attend(q=tensor(None)) == 2 and attend(out=None) == 2
+    assert attend(q=tensor(258)) == 5 and attend(lse=258) == 5
+    assert attend(r=rows(batch=65536)) == 6
+    # a long table of one sequence is split over CTAs that leave their sums in scratch memory
+    c, r = cache(pages=100000), rows(max_pages=4096)
+    need = L.xnor_b200_kv4_attend_scratch_bytes(c, r, 4, 0)
+    assert need > 0 and need % 4 == 0
+    assert attend(c=c, r=r) == 2
+    assert attend(c=c, r=r, scratch=256, nbytes=need - 1) == 3
+    assert attend(c=c, r=r, scratch=264, nbytes=need) == 5
+    assert L.xnor_b200_kv4_attend_scratch_bytes(c, rows(), 4, 0) == 0                   # a short one is not
+    assert L.xnor_b200_kv4_attend_scratch_bytes(c, r, 4, 100) == 0                      # nor a short window
+    assert L.xnor_b200_kv4_attend_scratch_bytes(c, r, 3, 0) == 0
+
+
+def test_tensors_off_the_gpu_are_refused():
+    codes, scales = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, 2, dtype=torch.float16)
+    m = F.Matrix4(codes, scales, 64, 32)
+    with pytest.raises(ValueError, match="CUDA device"):
+        F.forward_connected4(m, torch.zeros(1, 64))
+    with pytest.raises(ValueError, match="CUDA device"):
+        F.quantize_weights4(torch.zeros(4, 64), 32)
+    c = F.new_cache4(3, 2, 16, 64, 32, device="cpu")
+    i32 = dict(dtype=torch.int32)
+    table, lengths, x = torch.zeros(1, 2, **i32), torch.zeros(1, **i32), torch.zeros(1, 1, 2, 64)
+    for call in (lambda: F.append4(c, x, x, table, lengths), lambda: F.read4(c, table, lengths, 1), lambda: F.attend4(c, x, table, lengths)):
+        with pytest.raises(ValueError, match="CUDA device"):
+            call()
+
+
+@pytest.mark.parametrize("what", ["codes", "scales", "group", "k", "dtype"])
+def test_matrices_of_other_shapes_are_refused(what):
+    args = dict(codes=torch.zeros(4, 32, dtype=torch.uint8), scales=torch.zeros(4, 2, 2, dtype=torch.float16), k=64, group=32)
+    F.Matrix4(**args)
+    args |= dict(codes=dict(codes=torch.zeros(4, 33, dtype=torch.uint8)), scales=dict(scales=torch.zeros(4, 3, 2, dtype=torch.float16)),
+                 group=dict(group=48), k=dict(k=0), dtype=dict(scales=torch.zeros(4, 2, 2)))[what]
+    with pytest.raises(ValueError):
+        F.Matrix4(**args)
+
+
+@pytest.mark.parametrize("shape", [(3, 2, 8, 64, 32), (3, 2, 16, 48, 32), (3, 2, 16, 96, 64), (3, 2, 16, 288, 32), (0, 2, 16, 64, 32), (3, 2, 16, 64, 16)])
+def test_caches_of_other_shapes_are_refused(shape):
+    with pytest.raises(ValueError):
+        F.new_cache4(*shape, device="cpu")
