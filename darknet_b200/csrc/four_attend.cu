@@ -29,7 +29,7 @@ namespace cg = cooperative_groups;
 int validate_kv4(const xnor_b200_kv4_cache * c, const xnor_b200_kv4_rows * r);
 
 constexpr int FA_WARPS = 4, FA_THREADS = 32 * FA_WARPS;
-constexpr int FA_STAGES = 4;
+constexpr int FA_STAGES = 2;
 constexpr float FA_SLACK = 8.0f;                          // how far (log2) a score may pass the running maximum
 
 struct AttendParams
@@ -49,31 +49,32 @@ struct AttendParams
 struct Span
 {
 	int count;
-	long long at;                 // position of row 0
-	long long end;                // positions that there are
-	long long first, last;        // first 16-position step and the one behind the last, of all columns
+	int at;                       // position of row 0
+	int end;                      // positions that there are
+	int first, last;              // first step of 16 positions and the one behind the last, of all columns
 };
 
 __device__ __forceinline__ Span span_of(const AttendParams & p, int b, int i0, int i1)
 {
 	Span s;
-	s.count = p.r.counts != nullptr ? __ldg(p.r.counts + b) : p.r.tokens;
-	const int length = __ldg(p.r.lengths + b);
-	s.at = (long long)length - s.count;
-	s.end = min((long long)length, (long long)p.r.max_pages * p.c.page);
+	s.count = p.r.counts != nullptr ? min(__ldg(p.r.counts + b), p.r.tokens) : p.r.tokens;
+	const int length = max(__ldg(p.r.lengths + b), 0);
+	const long long at = (long long)length - (p.r.counts != nullptr ? __ldg(p.r.counts + b) : p.r.tokens), room = (long long)p.r.max_pages * p.c.page;
+	s.at = (int)max(at, -0x40000000LL);                   // (rows that far in front of a sequence see nothing either way)
+	s.end = (int)min((long long)length, room);
 	i1 = min(i1, s.count - 1);
-	const long long to = i1 < i0 ? 0 : min(s.end, s.at + i1 + 1);
-	const long long from = p.window > 0 ? max(0LL, s.at + i0 + 1 - p.window) : 0;
-	s.first = from / 16;
-	s.last = to > from ? (to + 15) / 16 : s.first;
+	const long long to = i1 < i0 ? 0 : min((long long)s.end, at + i1 + 1);
+	const long long from = p.window > 0 ? max(0LL, at + i0 + 1 - p.window) : 0;
+	s.first = (int)(from / 16);
+	s.last = to > from ? (int)((to + 15) / 16) : s.first;
 	return s;
 }
 
-// Steps of one split: the same for the kernel and for the one that joins.
-__device__ __forceinline__ long long steps_of_split(const Span & s, int splits)
+// Steps of one split, whole pairs for each warp: the same for the kernel and for the one that joins.
+__device__ __forceinline__ int steps_of_split(const Span & s, int splits)
 {
-	const long long n = s.last - s.first;
-	return max((n + splits - 1) / splits, (long long)FA_WARPS);
+	const int n = s.last - s.first, each = n / splits + (n % splits != 0);
+	return max((each + 1) / 2 * 2, 2 * FA_WARPS);
 }
 
 __device__ __forceinline__ float exp2_fast(float v)
@@ -86,6 +87,31 @@ __device__ __forceinline__ float exp2_fast(float v)
 // What the sums at maximum m count for next to those at maximum `top`
 __device__ __forceinline__ float weight_of(float m, float top) { return m == -INFINITY ? 0.0f : exp2_fast(m - top); }
 
+__device__ __forceinline__ void add_weighted(float4 & v, float by, const float4 & u)
+{
+	if (by == 0.0f) { return; }
+	v.x += by * u.x;
+	v.y += by * u.y;
+	v.z += by * u.z;
+	v.w += by * u.w;
+}
+
+// Four channels of a row, from its sums at maximum m and their total l.
+template <class T>
+__device__ __forceinline__ void write_out(const AttendParams & p, int b, int row, int head, int d, bool none, float m, float l, const float4 & v)
+{
+	none |= m == -INFINITY;
+	T * to = (T *)p.out.data + b * p.out.stride_sequence + row * p.out.stride_token + head * p.out.stride_head + d;
+	to[0] = from_f32<T>(none ? 0.0f : v.x / l);
+	to[1] = from_f32<T>(none ? 0.0f : v.y / l);
+	to[2] = from_f32<T>(none ? 0.0f : v.z / l);
+	to[3] = from_f32<T>(none ? 0.0f : v.w / l);
+	if (p.lse != nullptr && d == 0)
+	{
+		p.lse[((size_t)b * p.r.tokens + row) * p.heads + head] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+	}
+}
+
 __device__ __forceinline__ uint32_t transposed(uint32_t v)
 {
 	uint32_t r;
@@ -97,80 +123,121 @@ template <class T> struct Parts { static constexpr int Q = 1, P = 1; };
 template <> struct Parts<__half> { static constexpr int Q = 1, P = 2; };
 template <> struct Parts<float> { static constexpr int Q = 2, P = 2; };
 
-__host__ __device__ __forceinline__ int attend_pitch(int nb) { return (nb | 1) * 16; }           // of a row of codes: an odd number of 16 bytes
-__host__ __device__ __forceinline__ int attend_stage(int nb, int groups) { return 32 * attend_pitch(nb) + 2 * 16 * groups * 4; }
-__host__ __device__ __forceinline__ int attend_q_pitch(int nb) { return (nb | 1) * 64; }
+// A stage holds 32 positions: rows of keys' codes, rows of values' codes, scales.  A lane reads GB words of a row of a group; the pitches
+// put rows that are read at a time into different banks.
+template <int NB, int GB, int NT, int QP>
+struct AttendShape
+{
+	static constexpr int GROUPS = NB / GB, COLS = NT * 8;
+	static constexpr int K_PITCH = (GROUPS | 1) * 16 * GB, V_PITCH = (NB | 1) * 16, Q_PITCH = (NB | 1) * 64;
+	static constexpr int V_AT = 32 * K_PITCH, PAIRS_AT = V_AT + 32 * V_PITCH, STAGE = PAIRS_AT + 2 * 32 * GROUPS * 4;
+	static constexpr int U_PITCH = NB * 32 + 4, WARP = FA_STAGES * STAGE > COLS * U_PITCH * 4 ? FA_STAGES * STAGE : COLS * U_PITCH * 4;
+	static constexpr size_t SMEM = (size_t)FA_WARPS * WARP + QP * COLS * Q_PITCH + COLS * (4 + GROUPS * 4 + 8 + FA_WARPS * 12 + 8);
+};
 
-// NB: most blocks of 32 channels.  GB: blocks of a group.  NT: tiles of eight columns.
+template <int W>
+__device__ __forceinline__ void load_words(uint32_t (&w)[W], const void * p)
+{
+	if (W == 4)
+	{
+		const uint4 v = *(const uint4 *)p;
+		w[0] = v.x; w[W / 4] = v.y; w[W / 2] = v.z; w[W - 1] = v.w;
+	}
+	else if (W == 2)
+	{
+		const uint2 v = *(const uint2 *)p;
+		w[0] = v.x; w[W - 1] = v.y;
+	}
+	else { w[0] = *(const uint32_t *)p; }
+}
+
+// NB: blocks of 32 channels.  GB: blocks of a group.  NT: tiles of eight columns.
 template <class T, int NB, int GB, int NT>
 __global__ void __launch_bounds__(FA_THREADS)
 four_attend_kernel(const AttendParams p)
 {
-	constexpr int QP = Parts<T>::Q, PP = Parts<T>::P, COLS = NT * 8, GROUPS = NB / GB;
+	constexpr int QP = Parts<T>::Q, PP = Parts<T>::P;
+	using S = AttendShape<NB, GB, NT, QP>;
 	using How = Codes<T>;
+	constexpr int COLS = S::COLS, GROUPS = S::GROUPS, DIM = NB * 32;
 	constexpr bool CENTRED = How::CENTRED;
 	extern __shared__ __align__(128) unsigned char smem[];
 	const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-	const int dim = p.c.dim, nb = dim / 32, groups = dim / (32 * GB);
-	const int pitch = attend_pitch(nb), stage_bytes = attend_stage(nb, groups), q_pitch = attend_q_pitch(nb);
-	unsigned char * ring = smem + warp * FA_STAGES * stage_bytes;
-	unsigned char * s_q = smem + FA_WARPS * FA_STAGES * stage_bytes;                  // [part][column][q_pitch]
-	float * s_qf = (float *)(s_q + QP * COLS * q_pitch);                              // [column]
+	unsigned char * ring = smem + warp * S::WARP;
+	unsigned char * s_q = smem + FA_WARPS * S::WARP;                                  // [part][column]
+	float * s_qf = (float *)(s_q + QP * COLS * S::Q_PITCH);                           // [column]
 	float * s_qsum = s_qf + COLS;                                                     // [group][column]
-	long long * s_from = (long long *)(s_qsum + GROUPS * COLS);                       // [column]: positions that it sees
-	long long * s_to = s_from + COLS;
+	int * s_from = (int *)(s_qsum + GROUPS * COLS);                                   // [column]: positions that it sees
+	int * s_to = s_from + COLS;
 	float * s_m = (float *)(s_to + COLS);                                             // [warp][column]
-	float * s_l = s_m + FA_WARPS * COLS;
+	float * s_l = s_m + FA_WARPS * COLS, * s_by = s_l + FA_WARPS * COLS;
+	float * s_top = s_by + FA_WARPS * COLS, * s_all = s_top + COLS;                   // [column]
 
 	const int b = blockIdx.z, head = blockIdx.y / p.tiles, tile = blockIdx.y % p.tiles, split = blockIdx.x;
 	const int col0 = tile * COLS, cols = min(COLS, p.r.tokens * p.share - col0);
 	const Span span = span_of(p, b, col0 / p.share, (col0 + cols - 1) / p.share);
-	const long long per = steps_of_split(span, p.splits);
-	const long long begin = span.first + split * per, end = min(span.last, begin + per);
+	const int per = steps_of_split(span, p.splits);
+	const int begin = (int)min((long long)span.last, span.first + (long long)split * per), end = min(span.last, begin + per);
 
-	// ---- the ring: a step's keys and values, 16 positions of one page
+	// ---- the ring.  A step is 16 positions of one page; a warp takes two at a time.
 	const int page_steps = p.c.page / 16;
-	long long next = begin + warp;                            // the step that the next request is for
-	long long next_page = next / page_steps;
-	int next_sub = (int)(next - next_page * page_steps), next_id = -1;
-	auto look_up = [&]() { next_id = next < end ? __ldg(p.r.table + (long long)b * p.r.max_pages + next_page) : -1; };
-	uint32_t live = 0;                                        // a bit a stage: its page is one of the cache's
+	const uint32_t ring_at = four_smem(ring);
+	int next = begin + 2 * warp;                              // the step that the next request is for
+	int next_page = next / page_steps, next_sub = next - next_page * page_steps;
+	const int32_t * table = p.r.table + (size_t)b * p.r.max_pages;
+	int next_id[2];
+	auto look_up = [&]()
+	{
+		next_id[0] = next < end ? __ldg(table + next_page) : -1;
+		next_id[1] = next + 1 < end ? __ldg(table + next_page + (next_sub + 1 >= page_steps)) : -1;
+	};
+	// what a lane copies of a step: COPIES times 16 bytes of keys' and of values' codes, and of the scales
+	constexpr int COPIES = (NB + 1) / 2, STEP_CODES = 8 * DIM, STEP_SCALES = 64 * GROUPS;       // bytes of a step in memory
+	int k_to[COPIES], v_to[COPIES];
+	#pragma unroll
+	for (int j = 0; j < COPIES; ++j)
+	{
+		const int i = j * 32 + lane;
+		k_to[j] = i / NB * S::K_PITCH + i % NB * 16;
+		v_to[j] = S::V_AT + i / NB * S::V_PITCH + i % NB * 16;
+	}
+	uint32_t live = 0;                                        // a bit a step of a stage: its page is one of the cache's
 	auto request = [&](int stage)
 	{
-		const bool there = next_id >= 0 && next_id < p.c.pages;
-		live = (live & ~(1u << stage)) | ((there ? 1u : 0u) << stage);
-		if (there)
+		#pragma unroll
+		for (int h = 0; h < 2; ++h)
 		{
-			const uint32_t at = four_smem(ring) + stage * stage_bytes;
-			const size_t row = ((size_t)next_id * p.c.kv_heads + head) * p.c.page + next_sub * 16;
-			const uint8_t * kc = p.c.k_codes + row * (dim / 2), * vc = p.c.v_codes + row * (dim / 2);
+			const bool there = next_id[h] >= 0 && next_id[h] < p.c.pages;
+			const uint32_t bit = 1u << (stage * 2 + h);
+			live = there ? live | bit : live & ~bit;
+			if (!there) { continue; }
+			const int sub = h == 0 ? next_sub : next_sub + 1 >= page_steps ? 0 : next_sub + 1;
+			const size_t step = ((size_t)next_id[h] * p.c.kv_heads + head) * page_steps + sub;
+			const size_t codes = step * STEP_CODES + lane * 16, scales = step * STEP_SCALES;
+			const uint32_t at = ring_at + stage * S::STAGE;
 			#pragma unroll
-			for (int j = 0; j < NB / 2; ++j)
+			for (int j = 0; j < COPIES; ++j)
 			{
-				const int i = j * 32 + lane;
-				if (i < 16 * nb)
+				if ((j + 1) * 32 <= 16 * NB || j * 32 + lane < 16 * NB)
 				{
-					const uint32_t to = at + i / nb * pitch + i % nb * 16;
-					copy16(to, kc + i * 16, true);
-					copy16(to + 16 * pitch, vc + i * 16, true);
+					copy16(at + k_to[j] + h * 16 * S::K_PITCH, p.c.k_codes + codes + j * 512, true);
+					copy16(at + v_to[j] + h * 16 * S::V_PITCH, p.c.v_codes + codes + j * 512, true);
 				}
 			}
-			if (lane < 8 * groups)
+			#pragma unroll
+			for (int j = 0; j < (GROUPS > 4 ? 2 : 1); ++j)
 			{
-				const int i = lane % (4 * groups);
-				const char * src = (const char *)(lane < 4 * groups ? p.c.k_scales : p.c.v_scales) + row * groups * 4;
-				copy16(at + 32 * pitch + lane * 16, src + i * 16, true);
-			}
-			if (GROUPS > 4 && lane + 32 < 8 * groups)
-			{
-				const int i = (lane + 32) % (4 * groups);
-				const char * src = (const char *)(lane + 32 < 4 * groups ? p.c.k_scales : p.c.v_scales) + row * groups * 4;
-				copy16(at + 32 * pitch + (lane + 32) * 16, src + i * 16, true);
+				const int i = j * 32 + lane, own = i - 4 * GROUPS;
+				if (i < 8 * GROUPS)
+				{
+					const char * from = own < 0 ? (const char *)p.c.k_scales + scales + i * 16 : (const char *)p.c.v_scales + scales + own * 16;
+					copy16(at + S::PAIRS_AT + h * STEP_SCALES + (own < 0 ? i : own + 8 * GROUPS) * 16, from, true);
+				}
 			}
 		}
 		copies_close();
-		next += FA_WARPS;
-		next_sub += FA_WARPS;
+		next += 2 * FA_WARPS;
+		next_sub += 2 * FA_WARPS;
 		while (next_sub >= page_steps) { next_sub -= page_steps; ++next_page; }
 		look_up();
 	};
@@ -182,195 +249,241 @@ four_attend_kernel(const AttendParams p)
 	for (int c = warp; c < COLS; c += FA_WARPS)
 	{
 		const int i = (col0 + c) / p.share, h = head * p.share + (col0 + c) % p.share;
-		const bool there = c < cols && i < span.count;
-		float v[8] = {};
-		if (there && lane < dim / 8)
+		if (c >= cols || i >= span.count)                     // (sees nothing)
 		{
-			load8((const T *)p.q.data + b * p.q.stride_sequence + i * p.q.stride_token + h * p.q.stride_head + lane * 8, 8, p.wide_q != 0, v);
+			for (int j = lane; j < QP * NB * 4; j += 32) { *(uint4 *)(s_q + (j / (NB * 4) * COLS + c) * S::Q_PITCH + j % (NB * 4) * 16) = make_uint4(0, 0, 0, 0); }
+			if (lane < GROUPS) { s_qsum[lane * COLS + c] = 0.0f; }
+			if (lane == 0)
+			{
+				s_qf[c] = 0.0f;
+				s_from[c] = s_to[c] = 0;
+			}
+			continue;
 		}
+		float v[8];
+		eight_f32(load8((const T *)p.q.data + b * p.q.stride_sequence + i * p.q.stride_token + h * p.q.stride_head + lane * 8,
+				lane < NB * 4 ? 8 : 0, p.wide_q != 0), v);
 		uint32_t largest = 0;
-		float part = 0.0f;
+		#pragma unroll
+		for (int e = 0; e < 8; ++e) { largest = max(largest, __float_as_uint(fabsf(v[e]))); }
+		largest = __reduce_max_sync(0xffffffffu, largest);
+		float factor, inverse, part = 0.0f;
+		fit_f16(largest, factor, inverse);
 		#pragma unroll
 		for (int e = 0; e < 8; ++e)
 		{
-			largest = max(largest, __float_as_uint(fabsf(v[e])));
+			v[e] *= factor;
 			part += v[e];
 		}
-		largest = __reduce_max_sync(0xffffffffu, largest);
 		#pragma unroll
 		for (int m = 1; m < GB * 4; m <<= 1) { part += __shfl_xor_sync(0xffffffffu, part, m); }
-		if (lane < dim / 8 && lane % (GB * 4) == 0) { s_qsum[lane / (GB * 4) * COLS + c] = part * p.scale_log2; }
-		float factor, inverse;
-		fit_f16(largest, factor, inverse);
+		if (lane < NB * 4 && lane % (GB * 4) == 0) { s_qsum[lane / (GB * 4) * COLS + c] = part * (1.0f / How::UNIT); }
 		if (lane == 0)
 		{
 			s_qf[c] = inverse * (How::UNIT * p.scale_log2);
-			const long long at = span.at + i;
-			s_to[c] = there ? min(span.end, at + 1) : 0;
-			s_from[c] = there && p.window > 0 ? max(0LL, at + 1 - p.window) : 0;
+			s_to[c] = min(span.end, span.at + i + 1);
+			s_from[c] = p.window > 0 ? max(0, span.at + i + 1 - p.window) : 0;
 		}
-		if (lane < dim / 8)
+		if (lane < NB * 4)
 		{
 			float high[8], rest[8];
 			#pragma unroll
-			for (int e = 0; e < 8; ++e) { split_f16(factor == 0.0f ? 0.0f : v[e] * factor * (e & 1 ? How::ODD : 1.0f), high[e], rest[e]); }
-			unsigned char * at = s_q + c * q_pitch + lane * 16;
+			for (int e = 0; e < 8; ++e)
+			{
+				high[e] = v[e] * (e & 1 ? How::ODD : 1.0f);
+				if (QP == 2) { split_f16(high[e], high[e], rest[e]); }
+			}
+			// the four lanes of a row read GB words each of a group: those of a place lie side by side
+			unsigned char * at = s_q + c * S::Q_PITCH + (lane / (4 * GB) * (4 * GB) + lane % GB * 4 + lane / GB % 4) * 16;
 			*reinterpret_cast<uint4 *>(at) = make_uint4(pair_f16(high[0], high[4]), pair_f16(high[2], high[6]), pair_f16(high[1], high[5]), pair_f16(high[3], high[7]));
 			if (QP == 2)
 			{
-				*reinterpret_cast<uint4 *>(at + COLS * q_pitch) = make_uint4(pair_f16(rest[0], rest[4]), pair_f16(rest[2], rest[6]), pair_f16(rest[1], rest[5]), pair_f16(rest[3], rest[7]));
+				*reinterpret_cast<uint4 *>(at + COLS * S::Q_PITCH) = make_uint4(pair_f16(rest[0], rest[4]), pair_f16(rest[2], rest[6]), pair_f16(rest[1], rest[5]), pair_f16(rest[3], rest[7]));
 			}
 		}
 	}
 	__syncthreads();
-	// Positions that every column sees: no step inside them asks again
-	long long all_from = 0, all_to = LLONG_MAX;
-	for (int c = 0; c < cols; ++c)
-	{
-		if ((col0 + c) / p.share >= span.count) { continue; }
-		all_from = max(all_from, s_from[c]);
-		all_to = min(all_to, s_to[c]);
-	}
+	// Positions that every column of a token sees: no step inside them asks again
+	const int row_first = col0 / p.share, row_last = min((col0 + cols - 1) / p.share, span.count - 1);
+	const int all_to = min(span.end, span.at + row_first + 1), all_from = p.window > 0 ? max(0, span.at + row_last + 1 - p.window) : 0;
 
-	float o[NB][2][NT][4] = {};                               // [block][even, odd channels][tile][channel g: columns 2t, 2t+1; channel g + 8]
+	float o[GROUPS][GB][2][NT][4] = {};                       // [group][word][even, odd channels][tile][channel of g: columns 2t, 2t+1; of g + 8]
 	float lows[GROUPS][NT][2] = {};                           // sum(p * low_v) of this lane's positions
-	float top[NT][2], total[NT][2] = {};                      // running maximum (log2), sum(p) of this lane's positions
+	// running maximum (log2; base: 0 while there is none), the scores that move it, sum(p) of this lane's positions
+	float base[NT][2] = {}, limit[NT][2], total[NT][2] = {};
 	#pragma unroll
-	for (int nt = 0; nt < NT; ++nt) { top[nt][0] = top[nt][1] = -INFINITY; }
+	for (int nt = 0; nt < NT; ++nt) { limit[nt][0] = limit[nt][1] = -INFINITY; }
 	uint32_t unit_top = 0;                                    // scales of values up to these fp16 bits fit
 	float unit = 1.0f;                                        // what p * scale_v is multiplied by: a power of two
+	const uint32_t pick = g < 4 ? 0x5410u : 0x7632u;          // the half of a word that holds this lane's channels
 
 	int stage = 0;
-	for (long long step = begin + warp; step < end; step += FA_WARPS)
+	for (int step = begin + 2 * warp; step < end; step += 2 * FA_WARPS)
 	{
 		request((stage + FA_STAGES - 1) % FA_STAGES);
 		copies_wait<FA_STAGES - 1>();
 		__syncwarp();
-		const unsigned char * at = ring + stage * stage_bytes;
-		const bool there = live >> stage & 1;
+		const unsigned char * at = ring + stage * S::STAGE;
+		const uint32_t there = live >> (stage * 2) & 3;
 		stage = (stage + 1) % FA_STAGES;
-		if (!there) { continue; }
-		const uint32_t * k_pairs = (const uint32_t *)(at + 32 * pitch), * v_pairs = k_pairs + 16 * groups;
+		const uint32_t * k_pairs = (const uint32_t *)(at + S::PAIRS_AT) + g * GROUPS, * v_pairs = k_pairs + 32 * GROUPS;
 
 		// ---- scores
-		float s[NT][4] = {}, low_part[NT][4] = {};
+		float s[2][NT][4] = {};
 		#pragma unroll
 		for (int gr = 0; gr < GROUPS; ++gr)
 		{
-			if (gr >= groups) { continue; }
-			float acc[NT][4] = {};
+			float acc[2][NT][4] = {};
+			uint32_t w[2][2][GB];
+			#pragma unroll
+			for (int h = 0; h < 2; ++h)
+			{
+				#pragma unroll
+				for (int r = 0; r < 2; ++r) { load_words<GB>(w[h][r], at + (h * 16 + r * 8 + g) * S::K_PITCH + gr * 16 * GB + t * 4 * GB); }
+			}
 			#pragma unroll
 			for (int j = 0; j < GB; ++j)
 			{
-				const int blk = gr * GB + j;
-				const uint32_t w0 = *(const uint32_t *)(at + g * pitch + blk * 16 + t * 4);
-				const uint32_t w1 = *(const uint32_t *)(at + (g + 8) * pitch + blk * 16 + t * 4);
-				const uint32_t even[4] = {even_codes<CENTRED>(w0), even_codes<CENTRED>(w1), even_codes<CENTRED>(w0 >> 8), even_codes<CENTRED>(w1 >> 8)};
-				const uint32_t odd[4] = {odd_codes<CENTRED>(w0), odd_codes<CENTRED>(w1), odd_codes<CENTRED>(w0 >> 8), odd_codes<CENTRED>(w1 >> 8)};
+				uint4 qs[NT][QP];
 				#pragma unroll
 				for (int nt = 0; nt < NT; ++nt)
 				{
 					#pragma unroll
-					for (int part = 0; part < QP; ++part)
+					for (int part = 0; part < QP; ++part) { qs[nt][part] = *(const uint4 *)(s_q + (part * COLS + nt * 8 + g) * S::Q_PITCH + (gr * GB + j) * 64 + t * 16); }
+				}
+				#pragma unroll
+				for (int h = 0; h < 2; ++h)
+				{
+					const uint32_t w0 = w[h][0][j], w1 = w[h][1][j];
+					const uint32_t even[4] = {even_codes<CENTRED>(w0), even_codes<CENTRED>(w1), even_codes<CENTRED>(w0 >> 8), even_codes<CENTRED>(w1 >> 8)};
+					const uint32_t odd[4] = {odd_codes<CENTRED>(w0), odd_codes<CENTRED>(w1), odd_codes<CENTRED>(w0 >> 8), odd_codes<CENTRED>(w1 >> 8)};
+					#pragma unroll
+					for (int nt = 0; nt < NT; ++nt)
 					{
-						const uint4 qs = *(const uint4 *)(s_q + (part * COLS + nt * 8 + g) * q_pitch + blk * 64 + t * 16);
-						mma_16816(acc[nt], even, qs.x, qs.y);
-						mma_16816(acc[nt], odd, qs.z, qs.w);
+						#pragma unroll
+						for (int part = 0; part < QP; ++part)
+						{
+							mma_16816(acc[h][nt], even, qs[nt][part].x, qs[nt][part].y);
+							mma_16816(acc[h][nt], odd, qs[nt][part].z, qs[nt][part].w);
+						}
 					}
 				}
 			}
-			float2 sl0 = halves(k_pairs[g * groups + gr]), sl1 = halves(k_pairs[(g + 8) * groups + gr]);
-			sl0.y += How::SHIFT * sl0.x;
-			sl1.y += How::SHIFT * sl1.x;
 			#pragma unroll
-			for (int nt = 0; nt < NT; ++nt)
+			for (int h = 0; h < 2; ++h)
 			{
-				const float2 qsum = *(const float2 *)(s_qsum + gr * COLS + nt * 8 + t * 2);
-				s[nt][0] += sl0.x * acc[nt][0];
-				s[nt][1] += sl0.x * acc[nt][1];
-				s[nt][2] += sl1.x * acc[nt][2];
-				s[nt][3] += sl1.x * acc[nt][3];
-				low_part[nt][0] += sl0.y * qsum.x;
-				low_part[nt][1] += sl0.y * qsum.y;
-				low_part[nt][2] += sl1.y * qsum.x;
-				low_part[nt][3] += sl1.y * qsum.y;
+				float2 sl0 = halves(k_pairs[h * 16 * GROUPS + gr]), sl1 = halves(k_pairs[(h * 16 + 8) * GROUPS + gr]);
+				sl0.y += How::SHIFT * sl0.x;
+				sl1.y += How::SHIFT * sl1.x;
+				#pragma unroll
+				for (int nt = 0; nt < NT; ++nt)
+				{
+					const float2 qsum = *(const float2 *)(s_qsum + gr * COLS + nt * 8 + t * 2);
+					s[h][nt][0] += sl0.x * acc[h][nt][0] + sl0.y * qsum.x;
+					s[h][nt][1] += sl0.x * acc[h][nt][1] + sl0.y * qsum.y;
+					s[h][nt][2] += sl1.x * acc[h][nt][2] + sl1.y * qsum.x;
+					s[h][nt][3] += sl1.x * acc[h][nt][3] + sl1.y * qsum.y;
+				}
 			}
 		}
 		#pragma unroll
 		for (int nt = 0; nt < NT; ++nt)
 		{
 			const float2 qf = *(const float2 *)(s_qf + nt * 8 + t * 2);
-			s[nt][0] = s[nt][0] * qf.x + low_part[nt][0];
-			s[nt][1] = s[nt][1] * qf.y + low_part[nt][1];
-			s[nt][2] = s[nt][2] * qf.x + low_part[nt][2];
-			s[nt][3] = s[nt][3] * qf.y + low_part[nt][3];
+			#pragma unroll
+			for (int h = 0; h < 2; ++h)
+			{
+				s[h][nt][0] *= qf.x;
+				s[h][nt][1] *= qf.y;
+				s[h][nt][2] *= qf.x;
+				s[h][nt][3] *= qf.y;
+			}
 		}
 
 		// ---- what is not seen: neither its score nor its scales count, whatever they are
-		float2 sv[GROUPS][2];
+		uint32_t sv[GROUPS][2][2];
 		#pragma unroll
 		for (int gr = 0; gr < GROUPS; ++gr)
 		{
-			sv[gr][0] = gr < groups ? halves(v_pairs[g * groups + gr]) : make_float2(0.0f, 0.0f);
-			sv[gr][1] = gr < groups ? halves(v_pairs[(g + 8) * groups + gr]) : make_float2(0.0f, 0.0f);
-			sv[gr][0].y += How::SHIFT * sv[gr][0].x;
-			sv[gr][1].y += How::SHIFT * sv[gr][1].x;
+			#pragma unroll
+			for (int h = 0; h < 2; ++h)
+			{
+				#pragma unroll
+				for (int r = 0; r < 2; ++r) { sv[gr][h][r] = v_pairs[(h * 16 + r * 8) * GROUPS + gr]; }
+			}
 		}
-		const long long pos = step * 16;
-		if (pos < all_from || pos + 16 > all_to)
+		const bool edge = step * 16 < all_from || step * 16 + 32 > all_to || there != 3;
+		if (edge)
 		{
 			#pragma unroll
-			for (int r = 0; r < 2; ++r)
+			for (int h = 0; h < 2; ++h)
 			{
-				bool any = false;
 				#pragma unroll
-				for (int nt = 0; nt < NT; ++nt)
+				for (int r = 0; r < 2; ++r)
 				{
+					const int at_step = step + h, place = g + 8 * r;
+					bool any = false;
 					#pragma unroll
-					for (int e = 0; e < 2; ++e)
+					for (int nt = 0; nt < NT; ++nt)
 					{
-						const int c = nt * 8 + t * 2 + e;
-						const bool seen = pos + g + 8 * r >= s_from[c] && pos + g + 8 * r < s_to[c];
-						s[nt][2 * r + e] = seen ? s[nt][2 * r + e] : -INFINITY;
-						any |= seen;
+						#pragma unroll
+						for (int e = 0; e < 2; ++e)
+						{
+							const int c = nt * 8 + t * 2 + e;
+							const bool seen = (there >> h & 1) && at_step < end && at_step * 16 + place >= s_from[c] && at_step * 16 + place < s_to[c];
+							s[h][nt][2 * r + e] = seen ? s[h][nt][2 * r + e] : -INFINITY;
+							any |= seen;
+						}
 					}
-				}
-				#pragma unroll
-				for (int gr = 0; gr < GROUPS; ++gr)
-				{
-					if (!any) { sv[gr][r] = make_float2(0.0f, 0.0f); }
+					#pragma unroll
+					for (int gr = 0; gr < GROUPS; ++gr) { sv[gr][h][r] = any ? sv[gr][h][r] : 0; }
 				}
 			}
 		}
 
 		// ---- the maximum, and the unit of the values' scales, where they have to move
 		bool move = false;
+		__half2 widest = __habs2(as_half2(sv[0][0][0]));
 		#pragma unroll
-		for (int nt = 0; nt < NT; ++nt)
+		for (int h = 0; h < 2; ++h)
 		{
 			#pragma unroll
-			for (int e = 0; e < 4; ++e) { move |= !(s[nt][e] <= top[nt][e & 1] + FA_SLACK); }         // (a NaN moves it, too)
+			for (int nt = 0; nt < NT; ++nt)
+			{
+				#pragma unroll
+				for (int e = 0; e < 4; ++e) { move |= !(s[h][nt][e] <= limit[nt][e & 1]); }           // (a NaN moves it, too)
+			}
+			#pragma unroll
+			for (int gr = 0; gr < GROUPS; ++gr)
+			{
+				#pragma unroll
+				for (int r = 0; r < 2; ++r) { widest = __hmax2(widest, __habs2(as_half2(sv[gr][h][r]))); }
+			}
 		}
-		// (a scale that is not finite makes sums that are not, in any unit: it does not take the others' bits away)
-		uint32_t largest = 0;
-		#pragma unroll
-		for (int gr = 0; gr < GROUPS; ++gr)
-		{
-			const uint32_t a = __float_as_uint(fabsf(sv[gr][0].x)), c = __float_as_uint(fabsf(sv[gr][1].x));
-			largest = max(largest, max(a < 0x7f800000u ? a : 0, c < 0x7f800000u ? c : 0));
-		}
-		move |= largest > unit_top;
+		move |= (as_word(widest) & 0xffffu) > unit_top;
 		if (__any_sync(0xffffffffu, move))
 		{
+			// a scale that is not finite makes sums that are not, in any unit: it does not take the others' bits away
+			uint32_t largest = 0;
+			#pragma unroll
+			for (int gr = 0; gr < GROUPS; ++gr)
+			{
+				#pragma unroll
+				for (int i = 0; i < 4; ++i)
+				{
+					const uint32_t bits = sv[gr][i / 2][i % 2] & 0x7fffu;
+					largest = max(largest, bits < 0x7c00u ? bits : 0);
+				}
+			}
 			largest = __reduce_max_sync(0xffffffffu, largest);
 			float rescale = 1.0f;
 			if (largest > unit_top)
 			{
-				const uint32_t e = largest >> 23;
+				const uint32_t e = __float_as_uint(__half2float(__ushort_as_half((unsigned short)largest))) >> 23;
 				const float now = __uint_as_float((260 - e) << 23);       // 2^(6 - (e - 127)): the largest scale comes to [2^6, 2^7)
 				rescale = unit_top == 0 ? 1.0f : now / unit;
 				unit = now;
-				unit_top = e << 23 | 0x7fffffu;
+				unit_top = largest < 0x400u ? largest : largest | 0x3ffu; // all that share its exponent; subnormals: up to this one
 			}
 			#pragma unroll
 			for (int nt = 0; nt < NT; ++nt)
@@ -378,27 +491,36 @@ four_attend_kernel(const AttendParams p)
 				#pragma unroll
 				for (int e = 0; e < 2; ++e)
 				{
-					// a NaN counts as an infinity: that makes the column's sums NaN
-					s[nt][e] = s[nt][e] != s[nt][e] ? INFINITY : s[nt][e];
-					s[nt][2 + e] = s[nt][2 + e] != s[nt][2 + e] ? INFINITY : s[nt][2 + e];
-					float m = fmaxf(s[nt][e], s[nt][2 + e]);
+					float m = -INFINITY;
+					#pragma unroll
+					for (int i = 0; i < 4; ++i)
+					{
+						// a NaN counts as an infinity: that makes the column's sums NaN
+						float & v = s[i / 2][nt][i % 2 * 2 + e];
+						v = v != v ? INFINITY : v;
+						m = fmaxf(m, v);
+					}
 					m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
 					m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
 					m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-					if (m <= top[nt][e] + FA_SLACK) { m = top[nt][e]; }       // others moved theirs: a column's sums depend on its own scores alone
-					const float keep = m == top[nt][e] ? 1.0f : weight_of(top[nt][e], m);
-					top[nt][e] = m;
+					// others may have moved theirs: a column's sums depend on its own scores alone
+					float keep = 1.0f;
+					if (m > limit[nt][e])
+					{
+						keep = limit[nt][e] == -INFINITY ? 0.0f : exp2_fast(base[nt][e] - m);
+						base[nt][e] = m;
+						limit[nt][e] = m + FA_SLACK;
+					}
 					total[nt][e] *= keep;
 					#pragma unroll
-					for (int gr = 0; gr < GROUPS; ++gr) { lows[gr][nt][e] *= keep; }
-					#pragma unroll
-					for (int blk = 0; blk < NB; ++blk)
+					for (int gr = 0; gr < GROUPS; ++gr)
 					{
+						lows[gr][nt][e] *= keep;
 						#pragma unroll
-						for (int odd = 0; odd < 2; ++odd)
+						for (int i = 0; i < GB * 2; ++i)
 						{
-							o[blk][odd][nt][e] *= keep * rescale;
-							o[blk][odd][nt][2 + e] *= keep * rescale;
+							o[gr][i / 2][i % 2][nt][e] *= keep * rescale;
+							o[gr][i / 2][i % 2][nt][2 + e] *= keep * rescale;
 						}
 					}
 				}
@@ -406,61 +528,79 @@ four_attend_kernel(const AttendParams p)
 		}
 
 		// ---- weights: 0 for what is not seen
-		float w[NT][4];
 		#pragma unroll
-		for (int nt = 0; nt < NT; ++nt)
+		for (int h = 0; h < 2; ++h)
 		{
-			#pragma unroll
-			for (int e = 0; e < 4; ++e)
-			{
-				w[nt][e] = s[nt][e] == -INFINITY ? 0.0f : exp2_fast(s[nt][e] - top[nt][e & 1]);
-				total[nt][e & 1] += w[nt][e];
-			}
-		}
-
-		// ---- values
-		const uint32_t pick = g < 4 ? 0x5410u : 0x7632u;      // the half of a word that holds this lane's channels
-		#pragma unroll
-		for (int gr = 0; gr < GROUPS; ++gr)
-		{
-			if (gr >= groups) { continue; }
-			uint32_t pv[NT][PP][2];
 			#pragma unroll
 			for (int nt = 0; nt < NT; ++nt)
 			{
 				#pragma unroll
-				for (int r = 0; r < 2; ++r)
+				for (int e = 0; e < 4; ++e)
 				{
-					const float scale = sv[gr][r].x * unit, wx = w[nt][2 * r], wy = w[nt][2 * r + 1];
-					lows[gr][nt][0] += wx == 0.0f ? 0.0f : wx * sv[gr][r].y;
-					lows[gr][nt][1] += wy == 0.0f ? 0.0f : wy * sv[gr][r].y;
-					const float x = wx == 0.0f ? 0.0f : wx * scale, y = wy == 0.0f ? 0.0f : wy * scale;
-					const uint32_t high = pair_f16(x, y);
-					pv[nt][0][r] = transposed(high);
-					if (PP == 2)
-					{
-						const float2 back = halves(high);
-						pv[nt][PP - 1][r] = transposed(pair_f16(x - back.x, y - back.y));
-					}
+					s[h][nt][e] = exp2_fast(s[h][nt][e] - base[nt][e & 1]);
+					total[nt][e & 1] += s[h][nt][e];
 				}
 			}
+		}
+
+		// ---- values
+		#pragma unroll
+		for (int gr = 0; gr < GROUPS; ++gr)
+		{
 			#pragma unroll
-			for (int j = 0; j < GB; ++j)
+			for (int h = 0; h < 2; ++h)
 			{
-				const int blk = gr * GB + j;
-				const unsigned char * vw = at + 16 * pitch + 2 * t * pitch + blk * 16 + (g & 3) * 4;
-				const uint32_t x = __byte_perm(*(const uint32_t *)vw, *(const uint32_t *)(vw + pitch), pick);
-				const uint32_t y = __byte_perm(*(const uint32_t *)(vw + 8 * pitch), *(const uint32_t *)(vw + 9 * pitch), pick);
-				const uint32_t even[4] = {even_codes<CENTRED>(x), even_codes<CENTRED>(x >> 8), even_codes<CENTRED>(y), even_codes<CENTRED>(y >> 8)};
-				const uint32_t odd[4] = {odd_codes<CENTRED>(x), odd_codes<CENTRED>(x >> 8), odd_codes<CENTRED>(y), odd_codes<CENTRED>(y >> 8)};
+				uint32_t pv[NT][PP][2];
 				#pragma unroll
-				for (int nt = 0; nt < NT; ++nt)
+				for (int r = 0; r < 2; ++r)
 				{
+					float2 sl = halves(sv[gr][h][r]);
+					sl.y += 8.0f * sl.x;
+					sl.x *= unit;
 					#pragma unroll
-					for (int part = 0; part < PP; ++part)
+					for (int nt = 0; nt < NT; ++nt)
 					{
-						mma_16816(o[blk][0][nt], even, pv[nt][part][0], pv[nt][part][1]);
-						mma_16816(o[blk][1][nt], odd, pv[nt][part][0], pv[nt][part][1]);
+						const float wx = s[h][nt][2 * r], wy = s[h][nt][2 * r + 1];
+						float x = wx * sl.x, y = wy * sl.x, lx = wx * sl.y, ly = wy * sl.y;
+						if (edge)                                 // a scale that another column sees may be anything
+						{
+							x = wx == 0.0f ? 0.0f : x;
+							y = wy == 0.0f ? 0.0f : y;
+							lx = wx == 0.0f ? 0.0f : lx;
+							ly = wy == 0.0f ? 0.0f : ly;
+						}
+						lows[gr][nt][0] += lx;
+						lows[gr][nt][1] += ly;
+						const uint32_t high = pair_f16(x, y);
+						pv[nt][0][r] = transposed(high);
+						if (PP == 2)
+						{
+							const float2 back = halves(high);
+							pv[nt][PP - 1][r] = transposed(pair_f16(x - back.x, y - back.y));
+						}
+					}
+				}
+				uint32_t w[4][GB];
+				#pragma unroll
+				for (int i = 0; i < 4; ++i)
+				{
+					load_words<GB>(w[i], at + S::V_AT + (h * 16 + i / 2 * 8 + i % 2 + 2 * t) * S::V_PITCH + gr * 16 * GB + (g & 3) * 4 * GB);
+				}
+				#pragma unroll
+				for (int j = 0; j < GB; ++j)
+				{
+					const uint32_t x = __byte_perm(w[0][j], w[1][j], pick), y = __byte_perm(w[2][j], w[3][j], pick);
+					const uint32_t even[4] = {even_codes<true>(x), even_codes<true>(x >> 8), even_codes<true>(y), even_codes<true>(y >> 8)};
+					const uint32_t odd[4] = {odd_codes<true>(x), odd_codes<true>(x >> 8), odd_codes<true>(y), odd_codes<true>(y >> 8)};
+					#pragma unroll
+					for (int nt = 0; nt < NT; ++nt)
+					{
+						#pragma unroll
+						for (int part = 0; part < PP; ++part)
+						{
+							mma_16816(o[gr][j][0][nt], even, pv[nt][part][0], pv[nt][part][1]);
+							mma_16816(o[gr][j][1][nt], odd, pv[nt][part][0], pv[nt][part][1]);
+						}
 					}
 				}
 			}
@@ -471,7 +611,6 @@ four_attend_kernel(const AttendParams p)
 	// ---- the warps' sums meet
 	copies_wait<0>();
 	__syncwarp();
-	const int u_pitch = dim + 4;
 	float * u = (float *)ring;                                // [column][channel]
 	#pragma unroll
 	for (int nt = 0; nt < NT; ++nt)
@@ -485,7 +624,7 @@ four_attend_kernel(const AttendParams p)
 			const int c = nt * 8 + t * 2 + e;
 			if (g == 0)
 			{
-				s_m[warp * COLS + c] = top[nt][e];
+				s_m[warp * COLS + c] = limit[nt][e] == -INFINITY ? -INFINITY : base[nt][e];
 				s_l[warp * COLS + c] = l;
 			}
 			#pragma unroll
@@ -494,122 +633,140 @@ four_attend_kernel(const AttendParams p)
 				float low = lows[gr][nt][e];
 				#pragma unroll
 				for (int m = 4; m < 32; m <<= 1) { low += __shfl_xor_sync(0xffffffffu, low, m); }
-				if (gr >= groups) { continue; }
+					const float by = 1.0f / unit;
 				#pragma unroll
 				for (int j = 0; j < GB; ++j)
 				{
-					const int blk = gr * GB + j;
-					float * to = u + c * u_pitch + blk * 32 + (g & 3) * 8 + (g >> 2) * 4;
-					const float even = How::UNIT / unit, odd = even * How::ODD;
-					to[0] = o[blk][0][nt][e] * even + low;
-					to[2] = o[blk][0][nt][2 + e] * even + low;
-					to[1] = o[blk][1][nt][e] * odd + low;
-					to[3] = o[blk][1][nt][2 + e] * odd + low;
+					float * to = u + c * S::U_PITCH + (gr * 4 * GB + (g & 3) * GB + j) * 8 + (g >> 2) * 4;
+					to[0] = o[gr][j][0][nt][e] * by + low;
+					to[2] = o[gr][j][0][nt][2 + e] * by + low;
+					to[1] = o[gr][j][1][nt][e] * by + low;
+					to[3] = o[gr][j][1][nt][2 + e] * by + low;
 				}
 			}
 		}
 	}
 	__syncthreads();
-	float * first_u = (float *)smem;
-	const int warp_floats = FA_STAGES * stage_bytes / 4;
-	for (int i = threadIdx.x; i < cols * dim; i += FA_THREADS)
-	{
-		const int c = i / dim, d = i - c * dim;
-		float m = s_m[c];
-		#pragma unroll
-		for (int w = 1; w < FA_WARPS; ++w) { m = fmaxf(m, s_m[w * COLS + c]); }
-		float v = 0.0f;
-		#pragma unroll
-		for (int w = 0; w < FA_WARPS; ++w)
-		{
-			const float by = weight_of(s_m[w * COLS + c], m);
-			v += by == 0.0f ? 0.0f : by * first_u[w * warp_floats + c * u_pitch + d];
-		}
-		first_u[c * u_pitch + d] = v;
-	}
-	__syncthreads();
+	// per column: what each warp's sums count for, the maximum and the total of all
 	if (threadIdx.x < COLS)
 	{
 		const int c = threadIdx.x;
 		float m = s_m[c], l = 0.0f;
+		#pragma unroll
 		for (int w = 1; w < FA_WARPS; ++w) { m = fmaxf(m, s_m[w * COLS + c]); }
-		for (int w = 0; w < FA_WARPS; ++w) { l += s_l[w * COLS + c] * weight_of(s_m[w * COLS + c], m); }
-		s_m[c] = m;
-		s_l[c] = l;
+		float by[FA_WARPS];
+		#pragma unroll
+		for (int w = 0; w < FA_WARPS; ++w)
+		{
+			by[w] = weight_of(s_m[w * COLS + c], m);
+			l += by[w] == 0.0f ? 0.0f : by[w] * s_l[w * COLS + c];
+		}
+		#pragma unroll
+		for (int w = 0; w < FA_WARPS; ++w) { s_by[w * COLS + c] = by[w]; }
+		s_top[c] = m;
+		s_all[c] = l;
+	}
+	__syncthreads();
+	float * first_u = (float *)smem;
+	constexpr int WARP_FLOATS = S::WARP / 4, quads = DIM / 4;
+	const bool joined = p.partial == nullptr;
+	float * partial = joined ? nullptr : p.partial + (((size_t)(b * p.c.kv_heads + head) * p.tiles + tile) * p.splits + split) * COLS * (DIM + 4);
+	for (int c = threadIdx.x / quads, q = threadIdx.x % quads; c < cols; c += FA_THREADS / quads)
+	{
+		if (threadIdx.x >= FA_THREADS / quads * quads) { break; }
+		float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+		#pragma unroll
+		for (int w = 0; w < FA_WARPS; ++w) { add_weighted(v, s_by[w * COLS + c], *(const float4 *)(first_u + w * WARP_FLOATS + c * S::U_PITCH + q * 4)); }
+		if (joined) { *(float4 *)(first_u + c * S::U_PITCH + q * 4) = v; }
+		else if (begin < end) { *(float4 *)(partial + c * DIM + q * 4) = v; }
 	}
 
 	// ---- the splits' sums meet
-	if (p.partial != nullptr)
+	if (!joined)
 	{
-		__syncthreads();
-		if (begin >= end) { return; }
-		float * to = p.partial + (((size_t)(b * p.c.kv_heads + head) * p.tiles + tile) * p.splits + split) * COLS * (dim + 2);
-		for (int i = threadIdx.x; i < cols * dim; i += FA_THREADS) { to[i] = first_u[i / dim * u_pitch + i % dim]; }
-		if (threadIdx.x < cols)
+		if (threadIdx.x < cols && begin < end)
 		{
-			to[COLS * dim + threadIdx.x] = s_m[threadIdx.x];
-			to[COLS * (dim + 1) + threadIdx.x] = s_l[threadIdx.x];
+			partial[COLS * DIM + threadIdx.x] = s_top[threadIdx.x];
+			partial[COLS * (DIM + 1) + threadIdx.x] = s_all[threadIdx.x];
 		}
 		return;
 	}
 	const cg::cluster_group cluster = cg::this_cluster();
 	const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
 	cluster.sync();
-	for (int i = rank * FA_THREADS + threadIdx.x; i < cols * dim; i += ranks * FA_THREADS)
+	for (int i = rank * FA_THREADS + threadIdx.x; i < cols * quads; i += ranks * FA_THREADS)
 	{
-		const int c = i / dim, d = i - c * dim, row = (col0 + c) / p.share, h = head * p.share + (col0 + c) % p.share;
-		float m = -INFINITY, l = 0.0f, v = 0.0f;
-		for (int r = 0; r < ranks; ++r) { m = fmaxf(m, cluster.map_shared_rank(s_m, r)[c]); }
+		const int c = i / quads, q = i - c * quads, row = (col0 + c) / p.share, h = head * p.share + (col0 + c) % p.share;
+		float m = -INFINITY, l = 0.0f;
+		float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+		for (int r = 0; r < ranks; ++r) { m = fmaxf(m, cluster.map_shared_rank(s_top, r)[c]); }
 		for (int r = 0; r < ranks; ++r)
 		{
-			const float by = weight_of(cluster.map_shared_rank(s_m, r)[c], m);
-			l += by == 0.0f ? 0.0f : by * cluster.map_shared_rank(s_l, r)[c];
-			v += by == 0.0f ? 0.0f : by * cluster.map_shared_rank(first_u, r)[c * u_pitch + d];
+			const float by = weight_of(cluster.map_shared_rank(s_top, r)[c], m);
+			if (by == 0.0f) { continue; }
+			l += by * cluster.map_shared_rank(s_all, r)[c];
+			add_weighted(v, by, *(const float4 *)(cluster.map_shared_rank(first_u, r) + c * S::U_PITCH + q * 4));
 		}
-		const bool none = row >= span.count || m == -INFINITY;
-		((T *)p.out.data)[b * p.out.stride_sequence + row * p.out.stride_token + h * p.out.stride_head + d] = from_f32<T>(none ? 0.0f : v / l);
-		if (p.lse != nullptr && d == 0)
-		{
-			p.lse[((size_t)b * p.r.tokens + row) * p.heads + h] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-		}
+		write_out<T>(p, b, row, h, q * 4, row >= span.count, m, l, v);
 	}
 	cluster.sync();                                           // nobody leaves while its sums are read
 }
 
-// One block a column: joins what the splits left.
+// A warp takes a column's 128 channels: joins what the splits left.
 template <class T>
 __global__ void __launch_bounds__(FA_THREADS)
 four_attend_join_kernel(const AttendParams p, int cols_of_tile)
 {
+	const int dim = p.c.dim, quads = dim / 4;
 	const int b = blockIdx.z, head = blockIdx.y, col = blockIdx.x, tile = col / cols_of_tile, c = col - tile * cols_of_tile;
-	const int row = col / p.share, h = head * p.share + col % p.share, dim = p.c.dim;
+	const int row = col / p.share, h = head * p.share + col % p.share;
 	const int col0 = tile * cols_of_tile, cols = min(cols_of_tile, p.r.tokens * p.share - col0);
 	const Span span = span_of(p, b, col0 / p.share, (col0 + cols - 1) / p.share);
-	const long long per = steps_of_split(span, p.splits);
-	const int used = (int)((span.last - span.first + per - 1) / per);
-	const float * from = p.partial + ((size_t)(b * p.c.kv_heads + head) * p.tiles + tile) * p.splits * cols_of_tile * (dim + 2);
-	const size_t pitch = (size_t)cols_of_tile * (dim + 2);
+	const int per = steps_of_split(span, p.splits), used = (span.last - span.first + per - 1) / per;
+	const size_t pitch = (size_t)cols_of_tile * (dim + 4);
+	const float * from = p.partial + ((size_t)(b * p.c.kv_heads + head) * p.tiles + tile) * p.splits * pitch;
+	const float * tops = from + cols_of_tile * dim + c, * totals = tops + cols_of_tile;
+	// every warp joins every fourth split, then the four of them meet
+	__shared__ float s_m[FA_WARPS], s_l[FA_WARPS];
+	__shared__ float4 s_v[FA_WARPS][64];
+	const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 	float m = -INFINITY, l = 0.0f;
-	for (int s = 0; s < used; ++s) { m = fmaxf(m, from[s * pitch + cols_of_tile * dim + c]); }
-	for (int s = 0; s < used; ++s)
+	for (int s = warp + lane * FA_WARPS; s < used; s += 32 * FA_WARPS) { m = fmaxf(m, tops[s * pitch]); }
+	#pragma unroll
+	for (int i = 1; i < 32; i <<= 1) { m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i)); }
+	float4 v[2] = {};
+	for (int s = warp; s < used; s += FA_WARPS)
 	{
-		const float by = weight_of(from[s * pitch + cols_of_tile * dim + c], m);
-		l += by == 0.0f ? 0.0f : by * from[s * pitch + cols_of_tile * (dim + 1) + c];
-	}
-	const bool none = row >= span.count || m == -INFINITY;
-	for (int d = threadIdx.x; d < dim; d += FA_THREADS)
-	{
-		float v = 0.0f;
-		for (int s = 0; s < used; ++s)
+		const float by = weight_of(tops[s * pitch], m);
+		if (by == 0.0f) { continue; }
+		l += by * totals[s * pitch];
+		#pragma unroll
+		for (int j = 0; j < 2; ++j)
 		{
-			const float by = weight_of(from[s * pitch + cols_of_tile * dim + c], m);
-			v += by == 0.0f ? 0.0f : by * from[s * pitch + c * dim + d];
+			if (lane + j * 32 < quads) { add_weighted(v[j], by, *(const float4 *)(from + s * pitch + c * dim + (lane + j * 32) * 4)); }
 		}
-		((T *)p.out.data)[b * p.out.stride_sequence + row * p.out.stride_token + h * p.out.stride_head + d] = from_f32<T>(none ? 0.0f : v / l);
 	}
-	if (p.lse != nullptr && threadIdx.x == 0)
+	if (lane == 0)
 	{
-		p.lse[((size_t)b * p.r.tokens + row) * p.heads + h] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+		s_m[warp] = m;
+		s_l[warp] = l;
+	}
+	s_v[warp][lane] = v[0];
+	s_v[warp][lane + 32] = v[1];
+	__syncthreads();
+	for (int q = threadIdx.x; q < quads; q += FA_THREADS)
+	{
+		m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+		l = 0.0f;
+		float4 all = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+		#pragma unroll
+		for (int w = 0; w < FA_WARPS; ++w)
+		{
+			const float by = weight_of(s_m[w], m);
+			l += by == 0.0f ? 0.0f : by * s_l[w];
+			add_weighted(all, by, s_v[w][q]);
+		}
+		write_out<T>(p, b, row, h, q * 4, row >= span.count, m, l, all);
 	}
 }
 
@@ -620,6 +777,10 @@ struct AttendPlan
 	bool cluster;
 };
 
+#ifdef FOUR_SWEEP
+static int g_splits = 0, g_cluster = 0;
+#endif
+
 static AttendPlan plan_attend(const xnor_b200_kv4_cache & c, const xnor_b200_kv4_rows & r, int heads, int window)
 {
 	AttendPlan a;
@@ -629,26 +790,23 @@ static AttendPlan plan_attend(const xnor_b200_kv4_cache & c, const xnor_b200_kv4
 	a.tiles = (int)(tiles < INT_MAX ? tiles : INT_MAX);
 	long long most = (long long)r.max_pages * c.page;                          // positions that a tile may see
 	if (window > 0 && most > (long long)window + r.tokens) { most = (long long)window + r.tokens; }
-	const long long steps = (most + 15) / 16, want = 4LL * sm_count();
-	long long splits = (want + base - 1) / base, room = steps / (2 * FA_WARPS);
+	const int nb = c.dim / 32, on_sm = a.nt == 2 ? (nb <= 2 ? 3 : 2) : nb <= 2 ? 5 : nb <= 5 ? 4 : nb <= 7 ? 3 : 2;       // CTAs (registers, shared memory)
+	const long long steps = (most + 15) / 16, resident = (long long)sm_count() * on_sm;
+	long long splits = resident / base, room = steps / (4 * FA_WARPS);
 	if (splits > room) { splits = room; }
 	if (splits < 1) { splits = 1; }
 	a.cluster = splits <= 8;
-	if (a.cluster)
-	{
-		a.splits = 1;
-		while (a.splits < splits) { a.splits *= 2; }
-	}
-	else { a.splits = (int)splits; }
+#ifdef FOUR_SWEEP
+	if (g_splits) { splits = g_splits; a.cluster = g_cluster != 0; }
+#endif
+	a.splits = (int)splits;
 	return a;
 }
 
 template <class T, int NB, int GB, int NT>
 static int launch_attend(const AttendParams & p, const AttendPlan & plan, cudaStream_t stream)
 {
-	const int nb = p.c.dim / 32, groups = p.c.dim / p.c.group;
-	const size_t smem = (size_t)FA_WARPS * FA_STAGES * attend_stage(nb, groups) + (size_t)Parts<T>::Q * NT * 8 * attend_q_pitch(nb)
-			+ (size_t)NT * 8 * (4 + (NB / GB) * 4 + 16 + FA_WARPS * 8);
+	constexpr size_t smem = AttendShape<NB, GB, NT, Parts<T>::Q>::SMEM;
 	const auto kernel = four_attend_kernel<T, NB, GB, NT>;
 	const int rc = ensure_dynamic_smem((const void *)kernel, smem);
 	if (rc != XNOR_B200_OK) { return rc; }
@@ -686,15 +844,23 @@ static int launch_attend_columns(const AttendParams & p, const AttendPlan & plan
 template <class T>
 static int launch_attend_shape(const AttendParams & p, const AttendPlan & plan, cudaStream_t stream)
 {
-	const int d = p.c.dim, g = p.c.group;
-	if (d <= 64) { return g == 32 ? launch_attend_columns<T, 2, 1>(p, plan, stream) : launch_attend_columns<T, 2, 2>(p, plan, stream); }
-	if (d <= 128)
+	switch (p.c.dim / 32 * 8 + p.c.group / 32)                // (a group divides the dimension)
 	{
-		return g == 32 ? launch_attend_columns<T, 4, 1>(p, plan, stream) : g == 64 ? launch_attend_columns<T, 4, 2>(p, plan, stream)
-				: launch_attend_columns<T, 4, 4>(p, plan, stream);
+		case 1 * 8 + 1: return launch_attend_columns<T, 1, 1>(p, plan, stream);
+		case 2 * 8 + 1: return launch_attend_columns<T, 2, 1>(p, plan, stream);
+		case 2 * 8 + 2: return launch_attend_columns<T, 2, 2>(p, plan, stream);
+		case 3 * 8 + 1: return launch_attend_columns<T, 3, 1>(p, plan, stream);
+		case 4 * 8 + 1: return launch_attend_columns<T, 4, 1>(p, plan, stream);
+		case 4 * 8 + 2: return launch_attend_columns<T, 4, 2>(p, plan, stream);
+		case 4 * 8 + 4: return launch_attend_columns<T, 4, 4>(p, plan, stream);
+		case 5 * 8 + 1: return launch_attend_columns<T, 5, 1>(p, plan, stream);
+		case 6 * 8 + 1: return launch_attend_columns<T, 6, 1>(p, plan, stream);
+		case 6 * 8 + 2: return launch_attend_columns<T, 6, 2>(p, plan, stream);
+		case 7 * 8 + 1: return launch_attend_columns<T, 7, 1>(p, plan, stream);
+		case 8 * 8 + 1: return launch_attend_columns<T, 8, 1>(p, plan, stream);
+		case 8 * 8 + 2: return launch_attend_columns<T, 8, 2>(p, plan, stream);
+		default: return launch_attend_columns<T, 8, 4>(p, plan, stream);
 	}
-	return g == 32 ? launch_attend_columns<T, 8, 1>(p, plan, stream) : g == 64 ? launch_attend_columns<T, 8, 2>(p, plan, stream)
-			: launch_attend_columns<T, 8, 4>(p, plan, stream);
 }
 
 static int check_attend(const xnor_b200_kv4_cache * cache, const xnor_b200_kv4_rows * rows, int heads, int window)
@@ -715,7 +881,7 @@ extern "C" size_t xnor_b200_kv4_attend_scratch_bytes(const xnor_b200_kv4_cache *
 {
 	if (check_attend(cache, rows, heads, window) != XNOR_B200_OK) { return 0; }
 	const AttendPlan a = plan_attend(*cache, *rows, heads, window);
-	return a.cluster ? 0 : (size_t)rows->batch * cache->kv_heads * a.tiles * a.splits * a.nt * 8 * (cache->dim + 2) * sizeof(float);
+	return a.cluster ? 0 : (size_t)rows->batch * cache->kv_heads * a.tiles * a.splits * a.nt * 8 * (cache->dim + 4) * sizeof(float);
 }
 
 extern "C" int xnor_b200_kv4_attend(const xnor_b200_kv4_cache * cache, const xnor_b200_kv4_rows * rows, const xnor_b200_kv4_tensor * q, int heads,
@@ -757,3 +923,7 @@ extern "C" int xnor_b200_kv4_attend(const xnor_b200_kv4_cache * cache, const xno
 		default: return launch_attend_shape<__nv_bfloat16>(p, plan, s);
 	}
 }
+
+#ifdef FOUR_SWEEP
+extern "C" __attribute__((visibility("default"))) void four_sweep(int splits, int cluster, int) { g_splits = splits; g_cluster = cluster; }
+#endif

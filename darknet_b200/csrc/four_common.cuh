@@ -46,22 +46,38 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight neighbours from p, of which the first `there` exist (the others read as 0); wide: p is aligned to its 16 (fp32: 32) bytes and all exist.
+// Eight neighbours as they lie in memory.
+template <class T> struct Eight { uint4 raw[sizeof(T) / 2]; };
+
+// Eight neighbours from p, of which the first `there` exist (the others read as 0); wide: p is aligned to 16 bytes.
 template <class T>
-__device__ __forceinline__ void load8(const T * p, int there, bool wide, float (&v)[8])
+__device__ __forceinline__ Eight<T> load8(const T * p, int there, bool wide)
 {
+	Eight<T> v;
 	if (wide && there >= 8)
 	{
-		uint4 raw[sizeof(T) / 2];
-		raw[0] = __ldg(reinterpret_cast<const uint4 *>(p));
-		if (sizeof(T) == 4) { raw[sizeof(T) / 2 - 1] = __ldg(reinterpret_cast<const uint4 *>(p) + 1); }
-		const T * e = reinterpret_cast<const T *>(raw);
-		#pragma unroll
-		for (int i = 0; i < 8; ++i) { v[i] = to_f32(e[i]); }
-		return;
+		v.raw[0] = __ldg(reinterpret_cast<const uint4 *>(p));
+		if (sizeof(T) == 4) { v.raw[sizeof(T) / 2 - 1] = __ldg(reinterpret_cast<const uint4 *>(p) + 1); }
+		return v;
 	}
+	uint32_t * w = reinterpret_cast<uint32_t *>(v.raw);
 	#pragma unroll
-	for (int i = 0; i < 8; ++i) { v[i] = i < there ? to_f32(p[i]) : 0.0f; }
+	for (int i = 0; i < 8; ++i)
+	{
+		if (sizeof(T) == 4) { w[i] = i < there ? __ldg(reinterpret_cast<const uint32_t *>(p) + i) : 0; continue; }
+		const uint32_t h = i < there ? __ldg(reinterpret_cast<const uint16_t *>(p) + i) : 0;
+		if (i % 2 == 0) { w[i / 2] = h; }
+		else { w[i / 2] |= h << 16; }
+	}
+	return v;
+}
+
+template <class T>
+__device__ __forceinline__ void eight_f32(const Eight<T> & e, float (&v)[8])
+{
+	const T * p = reinterpret_cast<const T *>(e.raw);
+	#pragma unroll
+	for (int i = 0; i < 8; ++i) { v[i] = to_f32(p[i]); }
 }
 
 template <class T>

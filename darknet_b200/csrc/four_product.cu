@@ -17,13 +17,9 @@ namespace xnor
 
 namespace cg = cooperative_groups;
 
-constexpr int FP_WARPS = 4, FP_THREADS = 32 * FP_WARPS, FP_ROWS = 16 * FP_WARPS;
 constexpr int FP_K = 256;                                 // neighbours of a block: one power of two for x, one step of the ring
-constexpr int FP_STEPS = 6;                               // steps of a warp's ring
-constexpr int FP_CODE_BYTES = 16 * FP_K / 2;              // a step's codes of a warp
-constexpr int FP_SCALE_PITCH = FP_K / 32 + 1;             // words; odd, so that eight filters lie in eight banks
-constexpr int FP_STEP_BYTES = FP_CODE_BYTES + 16 * FP_SCALE_PITCH * 4;
 constexpr int FP_X_BYTES = FP_K * 2 + 64;                 // a row's block of x: the pitch puts neighbouring rows 16 banks apart
+constexpr int FP_CODE_PITCH = FP_K / 2;                   // a filter's block of codes
 
 struct ProductParams
 {
@@ -36,71 +32,125 @@ struct ProductParams
 	int n, k, rows, leaky, wide;
 	int row_bytes, groups;        // of one filter
 	int slice;                    // blocks of 256 of one CTA of a cluster
+	int steps;                    // of a warp's ring
 };
 
-// NT: tiles of eight rows.  XB: blocks of x in shared memory at a time.
-template <class T, int NT, int GROUP, int XB>
-__global__ void __launch_bounds__(FP_THREADS)
+// NT: tiles of eight rows.  MT: tiles of 16 filters of a warp.  XB: blocks of x converted at a time.
+template <class T, int NT, int MT, int WARPS, int GROUP, int XB>
+struct ProductShape
+{
+	static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, ROWS = NT * 8, THREADS = 32 * WARPS, FILTERS = 16 * MT * WARPS;
+	static constexpr int GROUPS = FP_K / GROUP, SCALE_PITCH = GROUPS + 1;             // words; odd, so that eight filters lie in eight banks
+	static constexpr int CODE_BYTES = 16 * MT * FP_CODE_PITCH, STEP_BYTES = CODE_BYTES + 16 * MT * SCALE_PITCH * 4;
+	static constexpr int TASKS = (XB * ROWS + WARPS - 1) / WARPS;                     // rows' blocks that a warp converts
+	// a buffer of x: [XB][part][row] blocks, [XB][row] powers of two, [XB][group][row] sums; behind the two of them a block of zeros,
+	// which the columns of rows that are not there read
+	__host__ __device__ static constexpr int x_bytes(int rows) { return XB * PARTS * rows * FP_X_BYTES; }
+	__host__ __device__ static constexpr int buffer_bytes(int rows) { return x_bytes(rows) + XB * ROWS * 4 * (1 + GROUPS); }
+	static size_t smem(int rows, int steps)
+	{
+		const size_t all = (size_t)WARPS * steps * STEP_BYTES + 2 * buffer_bytes(rows) + FP_X_BYTES, sums = (size_t)ROWS * (FILTERS + 1) * 4;
+		return all > sums ? all : sums;
+	}
+};
+
+template <int W>
+__device__ __forceinline__ void load_words(uint32_t (&w)[W], const void * p)
+{
+	if (W == 4)
+	{
+		const uint4 v = *(const uint4 *)p;
+		w[0] = v.x; w[W / 4] = v.y; w[W / 2] = v.z; w[W - 1] = v.w;
+	}
+	else if (W == 2)
+	{
+		const uint2 v = *(const uint2 *)p;
+		w[0] = v.x; w[W - 1] = v.y;
+	}
+	else { w[0] = *(const uint32_t *)p; }
+}
+
+template <class T, int NT, int MT, int WARPS, int GROUP, int XB>
+__global__ void __launch_bounds__(32 * WARPS)
 four_product_kernel(const ProductParams p)
 {
-	constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, ROWS = NT * 8, GROUPS = FP_K / GROUP, GROUP_BLOCKS = GROUP / 32;
+	using S = ProductShape<T, NT, MT, WARPS, GROUP, XB>;
 	using How = Codes<T>;
 	constexpr bool CENTRED = How::CENTRED;
+	constexpr int PARTS = S::PARTS, ROWS = S::ROWS, GROUPS = S::GROUPS, W = GROUP / 32, WARP_FILTERS = 16 * MT;
 	extern __shared__ __align__(128) unsigned char smem[];
-	unsigned char * s_x = smem + FP_WARPS * FP_STEPS * FP_STEP_BYTES;                 // [XB][part][row][FP_X_BYTES]
-	float * s_inverse = (float *)(s_x + XB * PARTS * ROWS * FP_X_BYTES);              // [XB][row]
-	float * s_sum = s_inverse + XB * ROWS;                                            // [XB][group][row]
 	const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
 	const cg::cluster_group cluster = cg::this_cluster();
 	const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
-	const int filter0 = (blockIdx.x / ranks) * FP_ROWS + warp * 16;
-	const int row0 = blockIdx.y * ROWS, rows = min(ROWS, p.rows - row0);
+	const int cta_filter = (blockIdx.x / ranks) * S::FILTERS, filter0 = cta_filter + warp * WARP_FILTERS;
+	const int row0 = blockIdx.y * ROWS, rows = min(ROWS, p.rows - row0), x_rows = min(ROWS, p.rows);
 	const int first = rank * p.slice, last = min(first + p.slice, (p.k + FP_K - 1) / FP_K);      // blocks of 256
-	unsigned char * ring = smem + warp * FP_STEPS * FP_STEP_BYTES;
+	unsigned char * ring = smem + warp * p.steps * S::STEP_BYTES;
+	unsigned char * buffers = smem + WARPS * p.steps * S::STEP_BYTES;
 	const uint32_t ring_at = four_smem(ring);
 
-	auto request = [&](int block)
+	// Codes: a lane copies 16 bytes of every fourth filter.  Filters that are not there read the last one's, and are never stored.  In
+	// shared memory the four lanes of a filter read W words each of a group: places are exchanged by the filter's number, so that the
+	// filters that are read at a time lie in different banks.
+	int ask = first, ask_stage = 0;
+	const int my_byte = lane % 8 * 16, my_place = my_byte ^ (W == 4 ? lane / 8 % 2 * 64 : W == 2 ? lane / 8 * 32 : lane / 8 * 16);
+	const uint8_t * code_from[4 * MT];
+	#pragma unroll
+	for (int j = 0; j < 4 * MT; ++j)
 	{
-		if (block < last)
+		code_from[j] = p.codes + (size_t)min(filter0 + j * 4 + lane / 8, p.n - 1) * p.row_bytes + min(first * (FP_K / 2) + my_byte, p.row_bytes - 16);
+	}
+	constexpr int SCALE_COPIES = WARP_FILTERS * GROUPS / 32;
+	const uint32_t * scale_from = p.scales + (size_t)min(filter0 + lane / GROUPS, p.n - 1) * p.groups + lane % GROUPS;
+	auto request = [&]()
+	{
+		if (ask < last)
 		{
-			const uint32_t at = ring_at + (block - first) % FP_STEPS * FP_STEP_BYTES;
+			const uint32_t at = ring_at + ask_stage * S::STEP_BYTES, to = at + lane / 8 * FP_CODE_PITCH;
+			const bool there = ask * (FP_K / 2) + my_byte < p.row_bytes;
+			const int on = ask * (FP_K / 2) + my_byte + FP_K / 2 < p.row_bytes ? FP_K / 2 : 0;       // stays inside the filter
 			#pragma unroll
-			for (int j = 0; j < 4; ++j)
+			for (int j = 0; j < 4 * MT; ++j)
 			{
-				const int r = j * 4 + lane / 8, c = lane % 8, byte = block * (FP_K / 2) + c * 16;
-				const bool there = filter0 + r < p.n && byte < p.row_bytes;
-				copy16(at + r * 128 + ((c ^ (r & 7)) * 16), p.codes + (there ? (size_t)(filter0 + r) * p.row_bytes + byte : 0), there);
+				copy16(to + j * 4 * FP_CODE_PITCH + (W == 1 && j % 2 ? my_place ^ 64 : my_place), code_from[j], there);
+				code_from[j] += on;
 			}
+			const bool there_group = ask * GROUPS + lane % GROUPS < p.groups;
 			#pragma unroll
-			for (int i = lane; i < 16 * GROUPS; i += 32)
+			for (int j = 0; j < SCALE_COPIES; ++j)
 			{
-				const int r = i / GROUPS, q = i % GROUPS, group = block * GROUPS + q;
-				const bool there = filter0 + r < p.n && group < p.groups;
-				copy4(at + FP_CODE_BYTES + (r * FP_SCALE_PITCH + q) * 4, p.scales + (there ? (size_t)(filter0 + r) * p.groups + group : 0), there);
+				constexpr int EACH = 32 / GROUPS;             // filters that the lanes take at a time
+				const uint32_t * from = scale_from + ask * GROUPS + (size_t)max(0, min(j * EACH, p.n - 1 - filter0 - lane / GROUPS)) * p.groups;
+				copy4(at + S::CODE_BYTES + ((j * EACH + lane / GROUPS) * S::SCALE_PITCH + lane % GROUPS) * 4, there_group ? from : p.scales, there_group);
 			}
+			++ask;
+			ask_stage = ask_stage + 1 == p.steps ? 0 : ask_stage + 1;
 		}
 		copies_close();
 	};
-	#pragma unroll
-	for (int i = 0; i < FP_STEPS - 1; ++i) { request(first + i); }
 
-	float sum[NT][4] = {};
-	for (int chunk = first; chunk < last; chunk += XB)
+	// x: a warp takes a row's block of 256, a lane eight neighbours; loaded a chunk ahead, converted when the chunk before is through
+	Eight<T> raw[S::TASKS];
+	auto load_x = [&](int chunk)
 	{
-		if (chunk != first) { __syncthreads(); }
-		// x: a warp takes a row's block of 256, a lane eight neighbours
-		const int blocks = min(XB, last - chunk);
-		for (int i = warp; i < blocks * rows; i += FP_WARPS)
+		#pragma unroll
+		for (int i = 0; i < S::TASKS; ++i)
 		{
-			const int xb = i / rows, row = i - xb * rows, k0 = (chunk + xb) * FP_K + lane * 8;
+			const int task = i * WARPS + warp, xb = task / rows, row = task - xb * rows, k0 = (chunk + xb) * FP_K + lane * 8;
+			const bool there = xb < XB && chunk + xb < last;
+			raw[i] = load8((const T *)p.x + (there ? (row0 + row) * p.ldx + k0 : 0), there ? p.k - k0 : 0, p.wide != 0);
+		}
+	};
+	auto convert_x = [&](int chunk, unsigned char * buffer)
+	{
+		float * inverses = (float *)(buffer + S::x_bytes(x_rows)), * sums = inverses + XB * ROWS;
+		#pragma unroll
+		for (int i = 0; i < S::TASKS; ++i)
+		{
+			const int task = i * WARPS + warp, xb = task / rows, row = task - xb * rows;
+			if (xb >= XB || chunk + xb >= last) { continue; }
 			float v[8];
-			const int there = min(8, p.k - k0);
-			if (there > 0) { load8((const T *)p.x + (row0 + row) * p.ldx + k0, there, p.wide != 0, v); }
-			else
-			{
-				#pragma unroll
-				for (int e = 0; e < 8; ++e) { v[e] = 0.0f; }
-			}
+			eight_f32(raw[i], v);
 			uint32_t largest = 0;
 			float part = 0.0f;
 			#pragma unroll
@@ -112,108 +162,168 @@ four_product_kernel(const ProductParams p)
 			largest = __reduce_max_sync(0xffffffffu, largest);
 			#pragma unroll
 			for (int m = 1; m < GROUP / 8; m <<= 1) { part += __shfl_xor_sync(0xffffffffu, part, m); }
-			if (lane % (GROUP / 8) == 0) { s_sum[(xb * GROUPS + lane / (GROUP / 8)) * ROWS + row] = part; }
+			if (lane % (GROUP / 8) == 0) { sums[(xb * GROUPS + lane / (GROUP / 8)) * ROWS + row] = part; }
 			float factor, inverse;
 			fit_f16(largest, factor, inverse);
-			if (lane == 0) { s_inverse[xb * ROWS + row] = inverse * How::UNIT; }
+			if (lane == 0) { inverses[xb * ROWS + row] = inverse * How::UNIT; }
 			float high[8], rest[8];
+			const float odd_factor = factor * How::ODD;
 			#pragma unroll
 			for (int e = 0; e < 8; ++e)
 			{
-				const float f = factor == 0.0f ? 0.0f : v[e] * factor * (e & 1 ? How::ODD : 1.0f);
-				split_f16(f, high[e], rest[e]);
+				high[e] = factor == 0.0f ? 0.0f : v[e] * (e & 1 ? odd_factor : factor);
+				if (PARTS == 2) { split_f16(high[e], high[e], rest[e]); }
 			}
-			unsigned char * at = s_x + ((xb * PARTS) * ROWS + row) * FP_X_BYTES + lane * 16;
+			unsigned char * at = buffer + (xb * PARTS * x_rows + row) * FP_X_BYTES + (lane / (4 * W) * (4 * W) + lane % W * 4 + lane / W % 4) * 16;
 			*reinterpret_cast<uint4 *>(at) = make_uint4(pair_f16(high[0], high[4]), pair_f16(high[2], high[6]), pair_f16(high[1], high[5]), pair_f16(high[3], high[7]));
 			if (PARTS == 2)
 			{
-				*reinterpret_cast<uint4 *>(at + ROWS * FP_X_BYTES) = make_uint4(pair_f16(rest[0], rest[4]), pair_f16(rest[2], rest[6]), pair_f16(rest[1], rest[5]), pair_f16(rest[3], rest[7]));
+				*reinterpret_cast<uint4 *>(at + x_rows * FP_X_BYTES) = make_uint4(pair_f16(rest[0], rest[4]), pair_f16(rest[2], rest[6]), pair_f16(rest[1], rest[5]), pair_f16(rest[3], rest[7]));
 			}
 		}
-		__syncthreads();
-		for (int xb = 0; xb < blocks; ++xb)
+	};
+
+	load_x(first);
+	for (int i = 0; i < p.steps - 1; ++i) { request(); }
+	uint32_t * zeros = (uint32_t *)(buffers + 2 * S::buffer_bytes(x_rows));
+	for (int i = threadIdx.x; i < FP_X_BYTES / 4; i += S::THREADS) { zeros[i] = 0; }
+	convert_x(first, buffers);
+
+	float sum[MT][NT][4] = {};
+	int stage = 0, which = 0;
+	for (int chunk = first; chunk < last; chunk += XB)
+	{
+		__syncthreads();                                      // this chunk's x is there, and nobody reads the buffer of the one before
+		const unsigned char * buffer = buffers + which * S::buffer_bytes(x_rows);
+		which ^= 1;
+		if (chunk + XB < last) { load_x(chunk + XB); }
+		const float * inverses = (const float *)(buffer + S::x_bytes(x_rows)), * sums = inverses + XB * ROWS;
+		#pragma unroll 1
+		for (int xb = 0; xb < XB && chunk + xb < last; ++xb)
 		{
-			request(chunk + xb + FP_STEPS - 1);
-			copies_wait<FP_STEPS - 1>();
+			request();
+			// of the copies asked for so far (a step each), all but the last steps - 1 have to be there
+			if (p.steps == 6) { copies_wait<5>(); }
+			else if (p.steps == 4) { copies_wait<3>(); }
+			else if (p.steps == 3) { copies_wait<2>(); }
+			else { copies_wait<1>(); }
 			__syncwarp();
-			const unsigned char * step = ring + (chunk + xb - first) % FP_STEPS * FP_STEP_BYTES;
-			const uint32_t * pairs = (const uint32_t *)(step + FP_CODE_BYTES);
-			float of_block[NT][4] = {};
+			const unsigned char * step = ring + stage * S::STEP_BYTES;
+			stage = stage + 1 == p.steps ? 0 : stage + 1;
+			const unsigned char * mine = step + g * FP_CODE_PITCH;
+			const int place = t * W * 4 ^ (W == 4 ? g % 2 * 64 : W == 2 ? g % 4 * 32 : g * 16);
+			const uint32_t * pairs = (const uint32_t *)(step + S::CODE_BYTES) + g * S::SCALE_PITCH;
+			const unsigned char * x_from[NT][PARTS];
+			#pragma unroll
+			for (int nt = 0; nt < NT; ++nt)
+			{
+				#pragma unroll
+				for (int part = 0; part < PARTS; ++part)
+				{
+					const bool there = nt * 8 + g < rows;
+					x_from[nt][part] = (there ? buffer + ((xb * PARTS + part) * x_rows + nt * 8 + g) * FP_X_BYTES : (const unsigned char *)zeros) + t * 16;
+				}
+			}
+			float of_block[MT][NT][4] = {};
 			#pragma unroll
 			for (int q = 0; q < GROUPS; ++q)
 			{
-				float acc[NT][4] = {};
+				float acc[MT][NT][4] = {};
+				uint32_t w[MT][2][W];
 				#pragma unroll
-				for (int j = 0; j < GROUP_BLOCKS; ++j)
+				for (int mt = 0; mt < MT; ++mt)
 				{
-					const int b = q * GROUP_BLOCKS + j;
-					const uint32_t w0 = *(const uint32_t *)(step + g * 128 + ((b ^ g) * 16) + t * 4);
-					const uint32_t w1 = *(const uint32_t *)(step + (g + 8) * 128 + ((b ^ g) * 16) + t * 4);
-					const uint32_t even[4] = {even_codes<CENTRED>(w0), even_codes<CENTRED>(w1), even_codes<CENTRED>(w0 >> 8), even_codes<CENTRED>(w1 >> 8)};
-					const uint32_t odd[4] = {odd_codes<CENTRED>(w0), odd_codes<CENTRED>(w1), odd_codes<CENTRED>(w0 >> 8), odd_codes<CENTRED>(w1 >> 8)};
+					#pragma unroll
+					for (int r = 0; r < 2; ++r) { load_words<W>(w[mt][r], mine + (mt * 16 + r * 8) * FP_CODE_PITCH + (place ^ q * (GROUP / 2))); }
+				}
+				#pragma unroll
+				for (int j = 0; j < W; ++j)
+				{
+					uint4 xs[NT][PARTS];
 					#pragma unroll
 					for (int nt = 0; nt < NT; ++nt)
 					{
 						#pragma unroll
-						for (int part = 0; part < PARTS; ++part)
+						for (int part = 0; part < PARTS; ++part) { xs[nt][part] = *(const uint4 *)(x_from[nt][part] + (q * W + j) * 64); }
+					}
+					#pragma unroll
+					for (int mt = 0; mt < MT; ++mt)
+					{
+						const uint32_t w0 = w[mt][0][j], w1 = w[mt][1][j];
+						const uint32_t even[4] = {even_codes<CENTRED>(w0), even_codes<CENTRED>(w1), even_codes<CENTRED>(w0 >> 8), even_codes<CENTRED>(w1 >> 8)};
+						const uint32_t odd[4] = {odd_codes<CENTRED>(w0), odd_codes<CENTRED>(w1), odd_codes<CENTRED>(w0 >> 8), odd_codes<CENTRED>(w1 >> 8)};
+						#pragma unroll
+						for (int nt = 0; nt < NT; ++nt)
 						{
-							uint4 xs = make_uint4(0, 0, 0, 0);
-							if (nt * 8 + g < rows)
+							#pragma unroll
+							for (int part = 0; part < PARTS; ++part)
 							{
-								xs = *(const uint4 *)(s_x + ((xb * PARTS + part) * ROWS + nt * 8 + g) * FP_X_BYTES + (b * 4 + t) * 16);
+								mma_16816(acc[mt][nt], even, xs[nt][part].x, xs[nt][part].y);
+								mma_16816(acc[mt][nt], odd, xs[nt][part].z, xs[nt][part].w);
 							}
-							mma_16816(acc[nt], even, xs.x, xs.y);
-							mma_16816(acc[nt], odd, xs.z, xs.w);
 						}
 					}
 				}
-				float2 sl0 = halves(pairs[g * FP_SCALE_PITCH + q]), sl1 = halves(pairs[(g + 8) * FP_SCALE_PITCH + q]);
-				sl0.y += How::SHIFT * sl0.x;
-				sl1.y += How::SHIFT * sl1.x;
 				#pragma unroll
-				for (int nt = 0; nt < NT; ++nt)
+				for (int mt = 0; mt < MT; ++mt)
 				{
-					const float2 xsum = *(const float2 *)(s_sum + (xb * GROUPS + q) * ROWS + nt * 8 + t * 2);
-					of_block[nt][0] += sl0.x * acc[nt][0];
-					of_block[nt][1] += sl0.x * acc[nt][1];
-					of_block[nt][2] += sl1.x * acc[nt][2];
-					of_block[nt][3] += sl1.x * acc[nt][3];
-					sum[nt][0] += sl0.y * xsum.x;
-					sum[nt][1] += sl0.y * xsum.y;
-					sum[nt][2] += sl1.y * xsum.x;
-					sum[nt][3] += sl1.y * xsum.y;
+					float2 sl0 = halves(pairs[mt * 16 * S::SCALE_PITCH + q]), sl1 = halves(pairs[(mt * 16 + 8) * S::SCALE_PITCH + q]);
+					sl0.y += How::SHIFT * sl0.x;
+					sl1.y += How::SHIFT * sl1.x;
+					#pragma unroll
+					for (int nt = 0; nt < NT; ++nt)
+					{
+						const float2 xsum = *(const float2 *)(sums + (xb * GROUPS + q) * ROWS + nt * 8 + t * 2);
+						of_block[mt][nt][0] += sl0.x * acc[mt][nt][0];
+						of_block[mt][nt][1] += sl0.x * acc[mt][nt][1];
+						of_block[mt][nt][2] += sl1.x * acc[mt][nt][2];
+						of_block[mt][nt][3] += sl1.x * acc[mt][nt][3];
+						sum[mt][nt][0] += sl0.y * xsum.x;
+						sum[mt][nt][1] += sl0.y * xsum.y;
+						sum[mt][nt][2] += sl1.y * xsum.x;
+						sum[mt][nt][3] += sl1.y * xsum.y;
+					}
 				}
 			}
 			#pragma unroll
 			for (int nt = 0; nt < NT; ++nt)
 			{
-				const float2 inverse = *(const float2 *)(s_inverse + xb * ROWS + nt * 8 + t * 2);
-				sum[nt][0] += inverse.x * of_block[nt][0];
-				sum[nt][1] += inverse.y * of_block[nt][1];
-				sum[nt][2] += inverse.x * of_block[nt][2];
-				sum[nt][3] += inverse.y * of_block[nt][3];
+				const float2 inverse = *(const float2 *)(inverses + xb * ROWS + nt * 8 + t * 2);
+				#pragma unroll
+				for (int mt = 0; mt < MT; ++mt)
+				{
+					sum[mt][nt][0] += inverse.x * of_block[mt][nt][0];
+					sum[mt][nt][1] += inverse.y * of_block[mt][nt][1];
+					sum[mt][nt][2] += inverse.x * of_block[mt][nt][2];
+					sum[mt][nt][3] += inverse.y * of_block[mt][nt][3];
+				}
 			}
 			__syncwarp();
 		}
+		if (chunk + XB < last) { convert_x(chunk + XB, buffers + which * S::buffer_bytes(x_rows)); }
 	}
 
 	// Columns of rows that are not there hold what shared memory held: never stored.
 	copies_wait<0>();
 	__syncthreads();
-	float * s_out = (float *)smem;                                                    // [row][64 filters + 1]
-	constexpr int PITCH = FP_ROWS + 1;
+	float * s_out = (float *)smem;                                                    // [row][filters of the CTA + 1]
+	constexpr int PITCH = S::FILTERS + 1;
 	#pragma unroll
-	for (int nt = 0; nt < NT; ++nt)
+	for (int mt = 0; mt < MT; ++mt)
 	{
 		#pragma unroll
-		for (int e = 0; e < 4; ++e) { s_out[(nt * 8 + t * 2 + (e & 1)) * PITCH + warp * 16 + g + (e >> 1) * 8] = sum[nt][e]; }
+		for (int nt = 0; nt < NT; ++nt)
+		{
+			#pragma unroll
+			for (int e = 0; e < 4; ++e) { s_out[(nt * 8 + t * 2 + (e & 1)) * PITCH + warp * WARP_FILTERS + mt * 16 + g + (e >> 1) * 8] = sum[mt][nt][e]; }
+		}
 	}
 	cluster.sync();
-	const int share = FP_ROWS / ranks;                                                // this CTA finishes some of the 64 filters
-	for (int i = threadIdx.x; i < rows * share; i += FP_THREADS)
+	const int share = (S::FILTERS + ranks - 1) / ranks;                               // this CTA finishes some of the filters
+	for (int i = threadIdx.x; i < rows * share; i += S::THREADS)
 	{
-		const int row = i / share, f = rank * share + i % share, filter = (blockIdx.x / ranks) * FP_ROWS + f;
-		if (filter >= p.n) { continue; }
+		const int row = i / share, f = rank * share + i % share, filter = cta_filter + f;
+		if (f >= S::FILTERS || filter >= p.n) { continue; }
 		float v = 0.0f;
 		for (int r = 0; r < ranks; ++r) { v += cluster.map_shared_rank(s_out, r)[row * PITCH + f]; }
 		if (p.biases != nullptr) { v += __ldg(p.biases + filter); }
@@ -223,22 +333,32 @@ four_product_kernel(const ProductParams p)
 	cluster.sync();                                                                   // nobody leaves while its sums are read
 }
 
-template <class T, int NT, int GROUP>
+#ifdef FOUR_SWEEP
+static int g_ranks = 0, g_steps = 0, g_shape = 0;
+#endif
+
+template <class T, int NT, int MT, int WARPS, int GROUP>
 static int launch_product(ProductParams & p, cudaStream_t stream)
 {
-	constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, XB = 4 / NT / PARTS < 1 ? 1 : 4 / NT / PARTS;
-	const int tiles = (p.n + FP_ROWS - 1) / FP_ROWS, blocks = (p.k + FP_K - 1) / FP_K;
+	constexpr int XB = NT == 1 ? 2 : 1;
+	using S = ProductShape<T, NT, MT, WARPS, GROUP, XB>;
+	const int tiles = (p.n + S::FILTERS - 1) / S::FILTERS, blocks = (p.k + FP_K - 1) / FP_K;
+	const auto kernel = four_product_kernel<T, NT, MT, WARPS, GROUP, XB>;
 	int ranks = 1;
-	while (ranks < 8 && tiles * ranks < 4 * sm_count() && blocks >= 2 * ranks) { ranks *= 2; }
+	while (ranks < 8 && tiles * ranks < 2 * sm_count() && blocks >= 2 * ranks) { ranks *= 2; }
+	p.steps = 4;
+#ifdef FOUR_SWEEP
+	if (g_ranks) { ranks = g_ranks; }
+	if (g_steps) { p.steps = g_steps; }
+#endif
 	p.slice = (blocks + ranks - 1) / ranks;
-	const size_t smem = (size_t)FP_WARPS * FP_STEPS * FP_STEP_BYTES + (size_t)XB * PARTS * NT * 8 * FP_X_BYTES
-			+ (size_t)XB * NT * 8 * 4 * (1 + FP_K / GROUP);
-	const auto kernel = four_product_kernel<T, NT, GROUP, XB>;
+	if (p.slice < p.steps) { p.steps = p.slice < 3 ? 2 : 3; }
+	const size_t smem = S::smem(p.rows < S::ROWS ? p.rows : S::ROWS, p.steps);
 	const int rc = ensure_dynamic_smem((const void *)kernel, smem);
 	if (rc != XNOR_B200_OK) { return rc; }
 	cudaLaunchConfig_t cfg = {};
 	cfg.gridDim = dim3((unsigned)(tiles * ranks), (unsigned)((p.rows + NT * 8 - 1) / (NT * 8)), 1);
-	cfg.blockDim = dim3(FP_THREADS, 1, 1);
+	cfg.blockDim = dim3(S::THREADS, 1, 1);
 	cfg.dynamicSmemBytes = smem;
 	cfg.stream = stream;
 	cudaLaunchAttribute attr[1];
@@ -252,14 +372,26 @@ static int launch_product(ProductParams & p, cudaStream_t stream)
 	return e == cudaSuccess ? check_launch() : cuda_fail(e);
 }
 
+template <class T, int NT, int GROUP>
+static int launch_product_shape(ProductParams & p, cudaStream_t stream)
+{
+#ifdef FOUR_SWEEP
+	if (g_shape == 1) { return launch_product<T, NT, 1, 4, GROUP>(p, stream); }
+	if (g_shape == 2) { return launch_product<T, NT, 2, 4, GROUP>(p, stream); }
+	if (g_shape == 3) { return launch_product<T, NT, 2, 8, GROUP>(p, stream); }
+	if (g_shape == 4) { return launch_product<T, NT, 1, 8, GROUP>(p, stream); }
+#endif
+	return launch_product<T, NT, 1, 4, GROUP>(p, stream);
+}
+
 template <class T, int NT>
 static int launch_product_group(ProductParams & p, int group, cudaStream_t stream)
 {
 	switch (group)
 	{
-		case 32: return launch_product<T, NT, 32>(p, stream);
-		case 64: return launch_product<T, NT, 64>(p, stream);
-		default: return launch_product<T, NT, 128>(p, stream);
+		case 32: return launch_product_shape<T, NT, 32>(p, stream);
+		case 64: return launch_product_shape<T, NT, 64>(p, stream);
+		default: return launch_product_shape<T, NT, 128>(p, stream);
 	}
 }
 
@@ -307,3 +439,7 @@ extern "C" int xnor_b200_w4_forward(const xnor_b200_w4_desc * d, const void * x,
 		default: return launch_product_rows<__nv_bfloat16>(p, d->group, s);
 	}
 }
+
+#ifdef FOUR_SWEEP
+extern "C" __attribute__((visibility("default"))) void four_sweep(int ranks, int steps, int shape) { g_ranks = ranks; g_steps = steps; g_shape = shape; }
+#endif

@@ -55,12 +55,7 @@ four_weights_kernel(const T * __restrict__ weights, long long ld, int k, int gro
 	{
 		const int w = w0 + threadIdx.x, there = min(8, k - 8 * w);
 		float v[8];
-		if (there > 0) { load8(row + 8 * (long long)w, there, wide != 0, v); }
-		else
-		{
-			#pragma unroll
-			for (int i = 0; i < 8; ++i) { v[i] = 0.0f; }
-		}
+		eight_f32(load8(row + 8 * (long long)w, there, wide != 0), v);
 		__half2 pair;
 		const uint32_t word = quantize8(v, there, lanes, pair);
 		if (w < words) { codes[(size_t)blockIdx.x * words + w] = word; }
@@ -106,8 +101,8 @@ kv4_append_kernel(const RowsParams p)
 	for (int w0 = 0; w0 < total; w0 += FR_THREADS)
 	{
 		const int w = w0 + threadIdx.x, head = w / words, word = w - head * words;
-		float v[8] = {};
-		if (w < total) { load8(src + head * t.stride_head + 8 * word, 8, p.wide[half] != 0, v); }
+		float v[8];
+		eight_f32(load8(src + head * t.stride_head + 8 * word, w < total ? 8 : 0, p.wide[half] != 0), v);
 		__half2 pair;
 		const uint32_t c = quantize8(v, 8, lanes, pair);
 		if (w >= total) { continue; }

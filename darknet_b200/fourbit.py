@@ -13,7 +13,7 @@ current stream of the tensors' device and may be captured into a CUDA graph.
 from __future__ import annotations
 
 import ctypes as C
-import math
+import struct
 from typing import Optional
 
 import torch
@@ -22,6 +22,30 @@ from . import capi
 
 _DTYPES = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
 _GROUPS = (32, 64, 128)
+
+# A decoding step is a few small kernels, so what a call costs on the host counts: its structs are packed as bytes, in the layout of
+# capi's (which takes a third of the time that filling those takes), and its checks are one expression each; only when that fails
+# _refuse_* look for the fault.
+_CACHE, _ROWS, _TENSOR = struct.Struct("=QQQQiiiii4x").pack, struct.Struct("=iii4xQQQ").pack, struct.Struct("=Qi4xqqq").pack
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+class _Calls:
+    """The library's entry points, as functions that take packed structs."""
+
+    def __getattr__(self, name: str):
+        vp, ci, ll = C.c_void_p, C.c_int, C.c_longlong
+        for entry, args in (("w4_forward", [vp, vp, ci, ci, ll, vp, vp, vp, vp, ll, vp]), ("kv4_append", [vp] * 5), ("kv4_read", [vp] * 5),
+                            ("kv4_attend", [vp, vp, vp, ci, C.c_float, ci, vp, vp, vp, C.c_size_t, vp]),
+                            ("kv4_attend_scratch_bytes", [vp, vp, ci, ci])):
+            f = capi.lib()["xnor_b200_" + entry]
+            f.argtypes = args
+            f.restype = C.c_size_t if entry.endswith("bytes") else ci
+            setattr(self, entry, f)
+        return object.__getattribute__(self, name)
+
+
+_calls = _Calls()
 
 
 def _dtype(t: torch.Tensor, what: str) -> int:
@@ -35,25 +59,8 @@ def _on(device: torch.device, *tensors) -> None:
     for t in tensors:
         if t is not None and t.device != device:
             raise ValueError(f"tensors on {t.device} and {device}: all of a call's tensors are on one CUDA device")
-
-
-class _Device:
-    """Makes a tensor's device the current one, where it is another, and names its current stream."""
-
-    def __init__(self, device: torch.device) -> None:
-        if device.type != "cuda":
-            raise ValueError(f"tensors on {device}: this path runs on a CUDA device only")
-        self.index = device.index
-        self.before = None
-
-    def __enter__(self) -> int:
-        if torch._C._cuda_getDevice() != self.index:
-            self.before = torch.cuda._exchange_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *_) -> None:
-        if self.before is not None:
-            torch.cuda._exchange_device(self.before)
+    if device.type != "cuda":
+        raise ValueError(f"tensors on {device}: this path runs on a CUDA device only")
 
 
 class Matrix4:
@@ -67,9 +74,11 @@ class Matrix4:
             raise ValueError(f"codes must be contiguous uint8 [n][{(k + 31) // 32 * 16}] for rows of {k} values")
         if scales.dtype != torch.float16 or scales.shape != (codes.shape[0], (k + group - 1) // group, 2) or not scales.is_contiguous():
             raise ValueError(f"scales must be contiguous fp16 [{codes.shape[0]}][{(k + group - 1) // group}][2]")
-        _on(codes.device, scales)
-        self.codes, self.scales, self.n, self.k, self.group = codes, scales, codes.shape[0], k, group
-        self._descs = {a: capi.W4Desc(self.n, k, group, a) for a in (capi.LINEAR, capi.LEAKY)}
+        if scales.device != codes.device:
+            raise ValueError(f"codes on {codes.device}, scales on {scales.device}")
+        self.codes, self.scales, self.n, self.k, self.group, self.device = codes, scales, codes.shape[0], k, group, codes.device
+        self._index = codes.get_device()
+        self._descs = {a: bytes(capi.W4Desc(self.n, k, group, a)) for a in (capi.LINEAR, capi.LEAKY)}
 
 
 def quantize_weights4(weights: torch.Tensor, group: int) -> Matrix4:
@@ -80,13 +89,27 @@ def quantize_weights4(weights: torch.Tensor, group: int) -> Matrix4:
         raise ValueError(f"group must be one of {_GROUPS}, not {group}")
     n, k = weights.shape
     dtype = _dtype(weights, "weights")
-    with _Device(weights.device) as stream:
+    _on(weights.device)
+    with torch.cuda.device(weights.device):
         codes = torch.empty(n, (k + 31) // 32 * 16, dtype=torch.uint8, device=weights.device)
         scales = torch.empty(n, (k + group - 1) // group, 2, dtype=torch.float16, device=weights.device)
-        m = Matrix4(codes, scales, k, group)
-        capi.check(capi.lib().xnor_b200_w4_quantize(C.byref(m._descs[capi.LINEAR]), weights.data_ptr(), dtype, weights.stride(0) if n > 1 else k,
-                                                   codes.data_ptr(), scales.data_ptr(), stream), "xnor_b200_w4_quantize")
-    return m
+        capi.check(capi.lib().xnor_b200_w4_quantize(C.byref(capi.W4Desc(n, k, group, capi.LINEAR)), weights.data_ptr(), dtype,
+                                                   weights.stride(0) if n > 1 else k, codes.data_ptr(), scales.data_ptr(),
+                                                   torch.cuda.current_stream().cuda_stream), "xnor_b200_w4_quantize")
+    return Matrix4(codes, scales, k, group)
+
+
+def _refuse_product(m: Matrix4, x, biases, activation, out) -> None:
+    if x.dim() != 2 or x.shape[1] != m.k or (x.stride(1) != 1 and m.k != 1):
+        raise ValueError(f"x must be [rows][{m.k}] with contiguous rows")
+    _dtype(x, "x")
+    if activation not in m._descs:
+        raise ValueError("activation must be capi.LINEAR or capi.LEAKY")
+    if biases is not None and (biases.dtype != torch.float32 or biases.shape != (m.n,) or not biases.is_contiguous()):
+        raise ValueError(f"biases must be contiguous fp32 [{m.n}]")
+    if out is not None and (out.dtype != x.dtype or out.shape != (x.shape[0], m.n) or (out.stride(1) != 1 and m.n != 1)):
+        raise ValueError(f"out must be {x.dtype} [{x.shape[0]}][{m.n}] with contiguous rows")
+    _on(m.device, x, m.codes, m.scales, biases, out)
 
 
 def forward_connected4(m: Matrix4, x: torch.Tensor, biases: Optional[torch.Tensor] = None, activation: int = capi.LINEAR,
@@ -94,26 +117,22 @@ def forward_connected4(m: Matrix4, x: torch.Tensor, biases: Optional[torch.Tenso
     """act(x @ W.T + biases) for x [rows][k] (rows contiguous, any distance apart), W the packed matrix: xnor_b200_w4_forward.
     biases: fp32 [n].  out: [rows][n] of x's type, rows contiguous; made where it is not given.  One pass over the weights serves up to
     16 rows."""
-    if x.dim() != 2 or x.shape[1] != m.k or (x.stride(1) != 1 and m.k != 1):
-        raise ValueError(f"x must be [rows][{m.k}] with contiguous rows")
-    dtype, rows = _dtype(x, "x"), x.shape[0]
-    if activation not in m._descs:
-        raise ValueError("activation must be capi.LINEAR or capi.LEAKY")
-    if biases is not None and (biases.dtype != torch.float32 or biases.shape != (m.n,) or not biases.is_contiguous()):
-        raise ValueError(f"biases must be contiguous fp32 [{m.n}]")
-    if out is not None and (out.dtype != x.dtype or out.shape != (rows, m.n) or (out.stride(1) != 1 and m.n != 1)):
-        raise ValueError(f"out must be {x.dtype} [{rows}][{m.n}] with contiguous rows")
-    _on(x.device, m.codes, biases, out)
-    with _Device(x.device) as stream:
-        if out is None:
-            out = torch.empty(rows, m.n, dtype=x.dtype, device=x.device)
-        if rows == 0:
-            return out
-        rc = capi.lib().xnor_b200_w4_forward(m._descs[activation], x.data_ptr(), dtype, rows, x.stride(0) if rows > 1 else m.k, m.codes.data_ptr(),
-                                             m.scales.data_ptr(), None if biases is None else biases.data_ptr(), out.data_ptr(),
-                                             out.stride(0) if rows > 1 else m.n, stream)
-        if rc:
-            capi.check(rc, "xnor_b200_w4_forward")
+    index, shape, dtype, desc = m._index, x.shape, _DTYPES.get(x.dtype), m._descs.get(activation)
+    if (index < 0 or dtype is None or desc is None or biases is not None or out is not None or len(shape) != 2 or shape[1] != m.k
+            or x.get_device() != index or m.codes.get_device() != index or m.scales.get_device() != index or not x.is_contiguous()):
+        _refuse_product(m, x, biases, activation, out)
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return forward_connected4(m, x, biases, activation, out)
+    rows = shape[0]
+    if out is None:
+        out = x.new_empty((rows, m.n))
+    if rows == 0:
+        return out
+    rc = _calls.w4_forward(desc, x.data_ptr(), dtype, rows, x.stride(0) if rows > 1 else m.k, m.codes.data_ptr(), m.scales.data_ptr(),
+                           None if biases is None else biases.data_ptr(), out.data_ptr(), out.stride(0) if rows > 1 else m.n, _raw_stream(index))
+    if rc:
+        capi.check(rc, "xnor_b200_w4_forward")
     return out
 
 
@@ -135,14 +154,17 @@ class Cache4:
                 raise ValueError(f"codes of keys and values must be contiguous uint8 {list(k_codes.shape)}")
             if scales.dtype != torch.float16 or scales.shape != (pages, kv_heads, page, dim // group, 2) or not scales.is_contiguous():
                 raise ValueError(f"scales must be contiguous fp16 {[pages, kv_heads, page, dim // group, 2]}")
-        _on(k_codes.device, k_scales, v_codes, v_scales)
+            if codes.device != k_codes.device or scales.device != k_codes.device:
+                raise ValueError("all four buffers must be on one device")
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
         self.pages, self.kv_heads, self.page, self.dim, self.group, self.device = pages, kv_heads, page, dim, group, k_codes.device
+        self._index = k_codes.get_device()
+        self._scratch: dict = {}                              # bytes of scratch memory by the sizes of a call
 
-    def struct(self) -> capi.Kv4Cache:
-        """Made for every call, so that it never names memory of a tensor that was replaced."""
-        return capi.Kv4Cache(self.k_codes.data_ptr(), self.k_scales.data_ptr(), self.v_codes.data_ptr(), self.v_scales.data_ptr(), self.pages,
-                             self.kv_heads, self.page, self.dim, self.group)
+    def _struct(self) -> bytes:
+        """Packed for every call, so that it never names memory of a tensor that was replaced."""
+        return _CACHE(self.k_codes.data_ptr(), self.k_scales.data_ptr(), self.v_codes.data_ptr(), self.v_scales.data_ptr(), self.pages,
+                      self.kv_heads, self.page, self.dim, self.group)
 
 
 def new_cache4(pages: int, kv_heads: int, page: int, dim: int, group: int, device="cuda:0") -> Cache4:
@@ -155,37 +177,50 @@ def new_cache4(pages: int, kv_heads: int, page: int, dim: int, group: int, devic
                   buffer(dim // group, 2, dtype=torch.float16), group)
 
 
-def _rows(c: Cache4, batch: int, tokens: int, table: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor]) -> capi.Kv4Rows:
-    if table.dim() != 2 or table.shape[0] != batch or table.shape[1] == 0 or table.dtype != torch.int32 or not table.is_contiguous():
-        raise ValueError(f"table must be contiguous int32 [{batch}][pages of a sequence]")
-    for name, t in (("lengths", lengths), ("counts", counts)):
-        if t is not None and (t.dtype != torch.int32 or t.shape != (batch,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous int32 [{batch}]")
-    _on(c.device, table, lengths, counts)
-    return capi.Kv4Rows(batch, tokens, table.shape[1], table.data_ptr(), lengths.data_ptr(), None if counts is None else counts.data_ptr())
+def _rows(c: Cache4, batch: int, tokens: int, table: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor]) -> bytes:
+    """struct xnor_b200_kv4_rows of a call, checked."""
+    index, shape = c._index, table.shape
+    if (index < 0 or len(shape) != 2 or shape[0] != batch or shape[1] == 0 or table.dtype is not torch.int32 or not table.is_contiguous()
+            or lengths.dtype is not torch.int32 or lengths.shape != (batch,) or not lengths.is_contiguous() or table.get_device() != index
+            or lengths.get_device() != index
+            or (counts is not None and (counts.dtype is not torch.int32 or counts.shape != (batch,) or not counts.is_contiguous() or counts.get_device() != index))):
+        if len(shape) != 2 or shape[0] != batch or shape[1] == 0 or table.dtype != torch.int32 or not table.is_contiguous():
+            raise ValueError(f"table must be contiguous int32 [{batch}][pages of a sequence]")
+        for name, t in (("lengths", lengths), ("counts", counts)):
+            if t is not None and (t.dtype != torch.int32 or t.shape != (batch,) or not t.is_contiguous()):
+                raise ValueError(f"{name} must be contiguous int32 [{batch}]")
+        _on(c.device, table, lengths, counts)
+    return _ROWS(batch, tokens, shape[1], table.data_ptr(), lengths.data_ptr(), 0 if counts is None else counts.data_ptr())
 
 
-def _tensor(t: torch.Tensor, what: str) -> capi.Kv4Tensor:
-    if t.stride(3) != 1 and t.shape[3] != 1:
+def _tensor(t: torch.Tensor, dtype: int, index: int, what: str) -> bytes:
+    """struct xnor_b200_kv4_tensor of a tensor of four dimensions on device `index`."""
+    a, b, c, d = t.stride()
+    if d != 1 and t.shape[3] != 1:
         raise ValueError(f"the last dimension of {what} must be contiguous")
-    return capi.Kv4Tensor(t.data_ptr(), _dtype(t, what), t.stride(0), t.stride(1), t.stride(2))
+    if t.get_device() != index or index < 0:
+        raise ValueError(f"{what} on {t.device}: all of a call's tensors are on one CUDA device, the cache's")
+    return _TENSOR(t.data_ptr(), dtype, a, b, c)
 
 
 def append4(c: Cache4, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor] = None) -> None:
     """Packs the newest tokens' keys and values [batch][tokens][kv_heads][dim] into their pages: xnor_b200_kv4_append.  lengths: what each
     sequence holds with them; counts: how many of the rows are tokens (default: all), the first ones of each sequence.  table: int32
     [batch][pages of a sequence].  No two rows may share a place."""
-    if k.dim() != 4 or k.shape[2:] != (c.kv_heads, c.dim) or v.shape != k.shape or v.dtype != k.dtype:
+    shape, dtype = k.shape, _DTYPES.get(k.dtype)
+    if dtype is None or len(shape) != 4 or shape[2] != c.kv_heads or shape[3] != c.dim or v.shape != shape or v.dtype is not k.dtype:
+        _dtype(k, "k")
         raise ValueError(f"k and v must be [batch][tokens][{c.kv_heads}][{c.dim}] of one type")
-    _on(c.device, k, v)
+    index = c._index
+    kt, vt, rows = _tensor(k, dtype, index, "k"), _tensor(v, dtype, index, "v"), _rows(c, shape[0], shape[1], table, lengths, counts)
     if k.numel() == 0:
         return
-    rows = _rows(c, k.shape[0], k.shape[1], table, lengths, counts)
-    kt, vt = _tensor(k, "k"), _tensor(v, "v")
-    with _Device(c.device) as stream:
-        rc = capi.lib().xnor_b200_kv4_append(c.struct(), rows, kt, vt, stream)
-        if rc:
-            capi.check(rc, "xnor_b200_kv4_append")
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return append4(c, k, v, table, lengths, counts)
+    rc = _calls.kv4_append(c._struct(), rows, kt, vt, _raw_stream(index))
+    if rc:
+        capi.check(rc, "xnor_b200_kv4_append")
 
 
 def read4(c: Cache4, table: torch.Tensor, lengths: torch.Tensor, tokens: int, counts: Optional[torch.Tensor] = None, dtype=torch.float32):
@@ -195,13 +230,19 @@ def read4(c: Cache4, table: torch.Tensor, lengths: torch.Tensor, tokens: int, co
         raise ValueError(f"dtype must be fp32, fp16 or bf16, not {dtype}")
     if table.dim() != 2 or tokens < 0:
         raise ValueError("table must be int32 [batch][pages of a sequence], tokens at least 0")
-    with _Device(c.device) as stream:
-        k = torch.empty(table.shape[0], tokens, c.kv_heads, c.dim, dtype=dtype, device=c.device)
-        v = torch.empty_like(k)
-        if k.numel():
-            rc = capi.lib().xnor_b200_kv4_read(c.struct(), _rows(c, table.shape[0], tokens, table, lengths, counts), _tensor(k, "k"), _tensor(v, "v"), stream)
-            if rc:
-                capi.check(rc, "xnor_b200_kv4_read")
+    index, batch = c._index, table.shape[0]
+    rows = _rows(c, batch, tokens, table, lengths, counts)
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return read4(c, table, lengths, tokens, counts, dtype)
+    k = torch.empty((batch, tokens, c.kv_heads, c.dim), dtype=dtype, device=c.device)
+    v = torch.empty_like(k)
+    if batch and tokens:
+        head = c.dim
+        strides = (_DTYPES[dtype], tokens * c.kv_heads * head, c.kv_heads * head, head)
+        rc = _calls.kv4_read(c._struct(), rows, _TENSOR(k.data_ptr(), *strides), _TENSOR(v.data_ptr(), *strides), _raw_stream(index))
+        if rc:
+            capi.check(rc, "xnor_b200_kv4_read")
     return k, v
 
 
@@ -211,28 +252,35 @@ def attend4(c: Cache4, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tens
     comes first): xnor_b200_kv4_attend.  scale: 1/sqrt(dim) where not given.  window: positions that a token sees, itself among them
     (0: all).  Rows that see nothing are 0.  out: as q; made where it is not given.  lse: fp32 [batch][tokens][heads], contiguous, receives
     the logarithm of each row's sum of exponentials."""
-    if q.dim() != 4 or q.shape[3] != c.dim or q.shape[2] == 0 or q.shape[2] % c.kv_heads:
-        raise ValueError(f"q must be [batch][tokens][heads][{c.dim}], heads a multiple of {c.kv_heads}")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
-        raise ValueError(f"out must be {q.dtype} {list(q.shape)}")
+    index, shape, dtype = c._index, q.shape, _DTYPES.get(q.dtype)
+    if dtype is None or len(shape) != 4 or shape[3] != c.dim or shape[2] == 0 or shape[2] % c.kv_heads or window < 0:
+        _dtype(q, "q")
+        raise ValueError(f"q must be [batch][tokens][heads][{c.dim}], heads a multiple of {c.kv_heads}; window at least 0")
+    if out is not None and (out.shape != shape or out.dtype != q.dtype):
+        raise ValueError(f"out must be {q.dtype} {list(shape)}")
     if out is not None and torch._debug_has_internal_overlap(out) == 1:
         raise ValueError("out has rows that share memory")
-    if lse is not None and (lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous()):
-        raise ValueError(f"lse must be contiguous fp32 {list(q.shape[:3])}")
-    if window < 0:
-        raise ValueError("window must be at least 0")
-    _on(c.device, q, out, lse)
-    batch, tokens, heads = q.shape[:3]
-    with _Device(c.device) as stream:
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if q.numel() == 0:
-            return out
-        cache, rows, L = c.struct(), _rows(c, batch, tokens, table, lengths, counts), capi.lib()
-        nbytes = L.xnor_b200_kv4_attend_scratch_bytes(cache, rows, heads, window)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        rc = L.xnor_b200_kv4_attend(cache, rows, _tensor(q, "q"), heads, 1.0 / math.sqrt(c.dim) if scale is None else scale, window, _tensor(out, "out"),
-                                    None if lse is None else lse.data_ptr(), None if scratch is None else scratch.data_ptr(), nbytes, stream)
-        if rc:
-            capi.check(rc, "xnor_b200_kv4_attend")
+    if lse is not None and (lse.shape != shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.get_device() != index):
+        raise ValueError(f"lse must be contiguous fp32 {list(shape[:3])} on the cache's device")
+    batch, tokens, heads = shape[0], shape[1], shape[2]
+    rows, qt = _rows(c, batch, tokens, table, lengths, counts), _tensor(q, dtype, index, "q")
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return attend4(c, q, table, lengths, counts, scale, window, out, lse)
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=c.device)
+    if q.numel() == 0:
+        return out
+    ot = _tensor(out, dtype, index, "out")
+    cache, sizes = c._struct(), (batch, tokens, table.shape[1], heads, window)
+    nbytes = c._scratch.get(sizes)
+    if nbytes is None:
+        if len(c._scratch) >= 1024:
+            c._scratch.clear()
+        nbytes = c._scratch[sizes] = _calls.kv4_attend_scratch_bytes(cache, rows, heads, window)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=c.device) if nbytes else None
+    rc = _calls.kv4_attend(cache, rows, qt, heads, c.dim ** -0.5 if scale is None else scale, window, ot, None if lse is None else lse.data_ptr(),
+                           None if scratch is None else scratch.data_ptr(), nbytes, _raw_stream(index))
+    if rc:
+        capi.check(rc, "xnor_b200_kv4_attend")
     return out

@@ -45,7 +45,7 @@ def unpack(packed, k):
 
 def values(packed, scales, group, k, centre=0):
     """(value, |low + centre * scale| + scale * |code - centre|) of packed rows, fp64 [..][k]: the second is what rounding errors are
-    relative to (calls of 16-bit types sum low and scale * code, fp32 ones around the middle, centre 8)."""
+    relative to (values of attention, and all of fp32 calls, are summed around the middle, centre 8)."""
     codes = unpack(np.asarray(packed), k).astype(np.float64)
     s, low = (np.repeat(np.asarray(scales)[..., i].astype(np.float64), group, -1)[..., :k] for i in (0, 1))
     return low + s * codes, np.abs(low + centre * s) + np.abs(s) * np.abs(codes - centre)
@@ -78,7 +78,7 @@ def attend(q, k_packed, k_scales, v_packed, v_scales, table, lengths, counts, gr
         where = np.array(there, int)
         for h in range(kv_heads):
             k, k_size = values(k_packed[at[0], h, at[1]], k_scales[at[0], h, at[1]], group, dim, centre)
-            v, v_size = values(v_packed[at[0], h, at[1]], v_scales[at[0], h, at[1]], group, dim, centre)
+            v, v_size = values(v_packed[at[0], h, at[1]], v_scales[at[0], h, at[1]], group, dim, 8)
             for i in range(min(tokens, count)):
                 own = lengths[b] - count + i
                 seen = (where <= own) & ((where > own - window) if window else True)

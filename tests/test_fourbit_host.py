@@ -112,6 +112,15 @@ def test_attention_refuses(L):
     assert L.xnor_b200_kv4_attend_scratch_bytes(c, r, 3, 0) == 0
 
 
+def test_packed_structs_are_the_librarys():
+    c = capi.Kv4Cache(1, 2, 3, 4, 5, 6, 7, 8, 9)
+    assert F._CACHE(1, 2, 3, 4, 5, 6, 7, 8, 9) == bytes(c)
+    r = capi.Kv4Rows(1, 2, 3, 4, 5, 6)
+    assert F._ROWS(1, 2, 3, 4, 5, 6) == bytes(r)
+    t = capi.Kv4Tensor(1, 2, 3, -4, 5)
+    assert F._TENSOR(1, 2, 3, -4, 5) == bytes(t)
+
+
 def test_tensors_off_the_gpu_are_refused():
     codes, scales = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, 2, dtype=torch.float16)
     m = F.Matrix4(codes, scales, 64, 32)

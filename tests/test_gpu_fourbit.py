@@ -321,6 +321,26 @@ def test_attention_over_long_sequences(dtype, length, batch, kv_heads, page, roo
     check_attend(s, q, counts=[3, 2, 1][:batch])
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_long_sums_lose_nothing(dtype):
+    """Equal weights over 20000 positions by one CTA: sums whose result is a hundredth of what goes into them.  Sequences enough that
+    none is split, all of them one and the same."""
+    batch, kv_heads = 60, 16
+    s = Sequences([20000], kv_heads, 32, 32, 256, seed=1)
+    s.cache.v_scales[..., 1] = -7.5 * s.cache.v_scales[..., 0]
+    q = 0.01 * torch.randn(1, 1, kv_heads, 32, generator=rng(1)).to(dtype).cuda()
+    want, _, size, score = R.attend(double(q), *s.buffers(), s.table, s.lengths, None, 32, 0.1, 0, centre(dtype))
+    table, lengths = s.device()
+    got = double(F.attend4(s.cache, q.expand(batch, -1, -1, -1), table.expand(batch, -1).contiguous(), lengths.expand(batch).contiguous(), scale=0.1))
+    assert (got == got[:1]).all()
+    # as check_attend has it, but for the sums: a link of a sum adds a rounding of what the sum has come to, which stays within a few times
+    # the square root of the links' own sizes
+    links = 20000 / 16 / 4
+    weight = 2 * score * (2.0 ** -22 + 24 * 2.0 ** -23) + 2.0 ** -22 + (2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -21)
+    tolerance = size * (weight[..., None] / 8 + 4 * links ** 0.5 * 2.0 ** -23) + np.abs(want) * R.HALF_STEP[dtype] * 1.001 + 2.0 ** -25 * (dtype == torch.float16)
+    assert (np.abs(got - want) <= tolerance).all(), (np.abs(got - want) / tolerance).max()
+
+
 @pytest.mark.parametrize("dim, group", [(64, 64), (128, 128), (256, 64)])
 def test_pages_that_are_not_there_are_not_seen(dim, group):
     s = Sequences([100, 64, 40], 2, dim, group, 16, seed=3)
@@ -511,7 +531,8 @@ def test_two_graphs_of_long_sequences_side_by_side():
         q = torch.randn(1, 1, 4, 64, generator=rng(seed)).half().cuda()
         table, lengths = s.device()
         want = F.attend4(s.cache, q, table, lengths)
-        assert capi.lib().xnor_b200_kv4_attend_scratch_bytes(s.cache.struct(), F._rows(s.cache, 1, 1, table, lengths, None), 4, 0) > 0
+        assert capi.lib().xnor_b200_kv4_attend_scratch_bytes(capi.Kv4Cache.from_buffer_copy(s.cache._struct()),
+                                                              capi.Kv4Rows.from_buffer_copy(F._rows(s.cache, 1, 1, table, lengths, None)), 4, 0) > 0
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             out = F.attend4(s.cache, q, table, lengths)
