@@ -151,6 +151,35 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[W], const void * p)
 	else { w[0] = *(const uint32_t *)p; }
 }
 
+// Weights of 16 positions with the scales of a group: operands of the product with the codes, and the sums of weight * low.  WILD: a
+// weight of 0 counts as nothing, whatever the scale (a branch that is hardly ever taken costs less than selecting every time).
+template <bool WILD, int NT, int PP>
+__device__ __forceinline__ void weigh(uint32_t (&pv)[NT][PP][2], float (&lows)[NT][2], const float (&w)[NT][4], const uint32_t (&pairs)[2], float unit)
+{
+	#pragma unroll
+	for (int r = 0; r < 2; ++r)
+	{
+		float2 sl = halves(pairs[r]);
+		sl.y += 8.0f * sl.x;
+		sl.x *= unit;
+		#pragma unroll
+		for (int nt = 0; nt < NT; ++nt)
+		{
+			const float wx = w[nt][2 * r], wy = w[nt][2 * r + 1];
+			const float x = WILD && wx == 0.0f ? 0.0f : wx * sl.x, y = WILD && wy == 0.0f ? 0.0f : wy * sl.x;
+			lows[nt][0] = WILD && wx == 0.0f ? lows[nt][0] : lows[nt][0] + wx * sl.y;
+			lows[nt][1] = WILD && wy == 0.0f ? lows[nt][1] : lows[nt][1] + wy * sl.y;
+			const uint32_t high = pair_f16(x, y);
+			pv[nt][0][r] = transposed(high);
+			if (PP == 2)
+			{
+				const float2 back = halves(high);
+				pv[nt][PP - 1][r] = transposed(pair_f16(x - back.x, y - back.y));
+			}
+		}
+	}
+}
+
 // NB: blocks of 32 channels.  GB: blocks of a group.  NT: tiles of eight columns.
 template <class T, int NB, int GB, int NT>
 __global__ void __launch_bounds__(FA_THREADS)
@@ -191,48 +220,53 @@ four_attend_kernel(const AttendParams p)
 		next_id[0] = next < end ? __ldg(table + next_page) : -1;
 		next_id[1] = next + 1 < end ? __ldg(table + next_page + (next_sub + 1 >= page_steps)) : -1;
 	};
-	// what a lane copies of a step: COPIES times 16 bytes of keys' and of values' codes, and of the scales
+	// what a lane copies of a step: COPIES times 16 bytes of keys' and of values' codes, and of the scales (keys' first, then values')
 	constexpr int COPIES = (NB + 1) / 2, STEP_CODES = 8 * DIM, STEP_SCALES = 64 * GROUPS;       // bytes of a step in memory
-	int k_to[COPIES], v_to[COPIES];
+	const uint8_t * const k_from = p.c.k_codes + lane * 16, * const v_from = p.c.v_codes + lane * 16;
+	const char * pairs_from[GROUPS > 4 ? 2 : 1];
+	uint32_t pairs_to[GROUPS > 4 ? 2 : 1], k_to[32 % NB == 0 ? 1 : COPIES], v_to[32 % NB == 0 ? 1 : COPIES];
 	#pragma unroll
-	for (int j = 0; j < COPIES; ++j)
+	for (int j = 0; j < (32 % NB == 0 ? 1 : COPIES); ++j)
 	{
 		const int i = j * 32 + lane;
-		k_to[j] = i / NB * S::K_PITCH + i % NB * 16;
-		v_to[j] = S::V_AT + i / NB * S::V_PITCH + i % NB * 16;
+		k_to[j] = ring_at + i / NB * S::K_PITCH + i % NB * 16;
+		v_to[j] = ring_at + S::V_AT + i / NB * S::V_PITCH + i % NB * 16;
+	}
+	#pragma unroll
+	for (int j = 0; j < (GROUPS > 4 ? 2 : 1); ++j)
+	{
+		const int i = j * 32 + lane, own = i - 4 * GROUPS;
+		pairs_from[j] = own < 0 ? (const char *)p.c.k_scales + i * 16 : (const char *)p.c.v_scales + own * 16;
+		pairs_to[j] = ring_at + S::PAIRS_AT + (own < 0 ? i : own + 8 * GROUPS) * 16;
 	}
 	uint32_t live = 0;                                        // a bit a step of a stage: its page is one of the cache's
 	auto request = [&](int stage)
 	{
+		live &= ~(3u << (stage * 2));
 		#pragma unroll
 		for (int h = 0; h < 2; ++h)
 		{
-			const bool there = next_id[h] >= 0 && next_id[h] < p.c.pages;
-			const uint32_t bit = 1u << (stage * 2 + h);
-			live = there ? live | bit : live & ~bit;
-			if (!there) { continue; }
+			if ((uint32_t)next_id[h] >= (uint32_t)p.c.pages) { continue; }
+			live |= 1u << (stage * 2 + h);
 			const int sub = h == 0 ? next_sub : next_sub + 1 >= page_steps ? 0 : next_sub + 1;
-			const size_t step = ((size_t)next_id[h] * p.c.kv_heads + head) * page_steps + sub;
-			const size_t codes = step * STEP_CODES + lane * 16, scales = step * STEP_SCALES;
-			const uint32_t at = ring_at + stage * S::STAGE;
+			const uint32_t step = ((uint32_t)next_id[h] * p.c.kv_heads + head) * page_steps + sub;      // (fits: a step has 128 bytes and more)
+			const uint8_t * k = k_from + (size_t)step * STEP_CODES, * v = v_from + (size_t)step * STEP_CODES;
+			const uint32_t at = stage * S::STAGE;
 			#pragma unroll
 			for (int j = 0; j < COPIES; ++j)
 			{
 				if ((j + 1) * 32 <= 16 * NB || j * 32 + lane < 16 * NB)
 				{
-					copy16(at + k_to[j] + h * 16 * S::K_PITCH, p.c.k_codes + codes + j * 512, true);
-					copy16(at + v_to[j] + h * 16 * S::V_PITCH, p.c.v_codes + codes + j * 512, true);
+					const uint32_t kt = 32 % NB == 0 ? k_to[0] + j * (32 / NB) * S::K_PITCH : k_to[32 % NB == 0 ? 0 : j];
+					const uint32_t vt = 32 % NB == 0 ? v_to[0] + j * (32 / NB) * S::V_PITCH : v_to[32 % NB == 0 ? 0 : j];
+					copy16(kt + at + h * 16 * S::K_PITCH, k + j * 512, true);
+					copy16(vt + at + h * 16 * S::V_PITCH, v + j * 512, true);
 				}
 			}
 			#pragma unroll
 			for (int j = 0; j < (GROUPS > 4 ? 2 : 1); ++j)
 			{
-				const int i = j * 32 + lane, own = i - 4 * GROUPS;
-				if (i < 8 * GROUPS)
-				{
-					const char * from = own < 0 ? (const char *)p.c.k_scales + scales + i * 16 : (const char *)p.c.v_scales + scales + own * 16;
-					copy16(at + S::PAIRS_AT + h * STEP_SCALES + (own < 0 ? i : own + 8 * GROUPS) * 16, from, true);
-				}
+				if (j * 32 + lane < 8 * GROUPS) { copy16(pairs_to[j] + at + h * STEP_SCALES, pairs_from[j] + (size_t)step * STEP_SCALES, true); }
 			}
 		}
 		copies_close();
@@ -354,9 +388,9 @@ four_attend_kernel(const AttendParams p)
 				#pragma unroll
 				for (int h = 0; h < 2; ++h)
 				{
-					const uint32_t w0 = w[h][0][j], w1 = w[h][1][j];
-					const uint32_t even[4] = {even_codes<CENTRED>(w0), even_codes<CENTRED>(w1), even_codes<CENTRED>(w0 >> 8), even_codes<CENTRED>(w1 >> 8)};
-					const uint32_t odd[4] = {odd_codes<CENTRED>(w0), odd_codes<CENTRED>(w1), odd_codes<CENTRED>(w0 >> 8), odd_codes<CENTRED>(w1 >> 8)};
+					const uint32_t w0 = w[h][0][j], w1 = w[h][1][j], w0_up = upper(w0), w1_up = upper(w1);
+					const uint32_t even[4] = {even_codes<CENTRED>(w0), even_codes<CENTRED>(w1), even_codes<CENTRED>(w0_up), even_codes<CENTRED>(w1_up)};
+					const uint32_t odd[4] = {odd_codes<CENTRED>(w0), odd_codes<CENTRED>(w1), odd_codes<CENTRED>(w0_up), odd_codes<CENTRED>(w1_up)};
 					#pragma unroll
 					for (int nt = 0; nt < NT; ++nt)
 					{
@@ -412,6 +446,7 @@ four_attend_kernel(const AttendParams p)
 				for (int r = 0; r < 2; ++r) { sv[gr][h][r] = v_pairs[(h * 16 + r * 8) * GROUPS + gr]; }
 			}
 		}
+		bool wild = false;                                    // a scale that one column sees and another does not is not finite
 		const bool edge = step * 16 < all_from || step * 16 + 32 > all_to || there != 3;
 		if (edge)
 		{
@@ -436,9 +471,14 @@ four_attend_kernel(const AttendParams p)
 						}
 					}
 					#pragma unroll
-					for (int gr = 0; gr < GROUPS; ++gr) { sv[gr][h][r] = any ? sv[gr][h][r] : 0; }
+					for (int gr = 0; gr < GROUPS; ++gr)
+					{
+						sv[gr][h][r] = any ? sv[gr][h][r] : 0;
+						wild |= (sv[gr][h][r] & 0x7c00u) == 0x7c00u || (sv[gr][h][r] & 0x7c000000u) == 0x7c000000u;
+					}
 				}
 			}
+			wild = __any_sync(0xffffffffu, wild);
 		}
 
 		// ---- the maximum, and the unit of the values' scales, where they have to move
@@ -551,35 +591,8 @@ four_attend_kernel(const AttendParams p)
 			for (int h = 0; h < 2; ++h)
 			{
 				uint32_t pv[NT][PP][2];
-				#pragma unroll
-				for (int r = 0; r < 2; ++r)
-				{
-					float2 sl = halves(sv[gr][h][r]);
-					sl.y += 8.0f * sl.x;
-					sl.x *= unit;
-					#pragma unroll
-					for (int nt = 0; nt < NT; ++nt)
-					{
-						const float wx = s[h][nt][2 * r], wy = s[h][nt][2 * r + 1];
-						float x = wx * sl.x, y = wy * sl.x, lx = wx * sl.y, ly = wy * sl.y;
-						if (edge)                                 // a scale that another column sees may be anything
-						{
-							x = wx == 0.0f ? 0.0f : x;
-							y = wy == 0.0f ? 0.0f : y;
-							lx = wx == 0.0f ? 0.0f : lx;
-							ly = wy == 0.0f ? 0.0f : ly;
-						}
-						lows[gr][nt][0] += lx;
-						lows[gr][nt][1] += ly;
-						const uint32_t high = pair_f16(x, y);
-						pv[nt][0][r] = transposed(high);
-						if (PP == 2)
-						{
-							const float2 back = halves(high);
-							pv[nt][PP - 1][r] = transposed(pair_f16(x - back.x, y - back.y));
-						}
-					}
-				}
+				if (wild) { weigh<true, NT, PP>(pv, lows[gr], s[h], sv[gr][h], unit); }
+				else { weigh<false, NT, PP>(pv, lows[gr], s[h], sv[gr][h], unit); }
 				uint32_t w[4][GB];
 				#pragma unroll
 				for (int i = 0; i < 4; ++i)
@@ -589,9 +602,9 @@ four_attend_kernel(const AttendParams p)
 				#pragma unroll
 				for (int j = 0; j < GB; ++j)
 				{
-					const uint32_t x = __byte_perm(w[0][j], w[1][j], pick), y = __byte_perm(w[2][j], w[3][j], pick);
-					const uint32_t even[4] = {even_codes<true>(x), even_codes<true>(x >> 8), even_codes<true>(y), even_codes<true>(y >> 8)};
-					const uint32_t odd[4] = {odd_codes<true>(x), odd_codes<true>(x >> 8), odd_codes<true>(y), odd_codes<true>(y >> 8)};
+					const uint32_t x = __byte_perm(w[0][j], w[1][j], pick), y = __byte_perm(w[2][j], w[3][j], pick), x_up = upper(x), y_up = upper(y);
+					const uint32_t even[4] = {even_codes<true>(x), even_codes<true>(x_up), even_codes<true>(y), even_codes<true>(y_up)};
+					const uint32_t odd[4] = {odd_codes<true>(x), odd_codes<true>(x_up), odd_codes<true>(y), odd_codes<true>(y_up)};
 					#pragma unroll
 					for (int nt = 0; nt < NT; ++nt)
 					{
@@ -868,6 +881,7 @@ static int check_attend(const xnor_b200_kv4_cache * cache, const xnor_b200_kv4_r
 	const int rc = validate_kv4(cache, rows);
 	if (rc != XNOR_B200_OK) { return rc; }
 	if (heads <= 0 || heads % cache->kv_heads != 0 || window < 0) { return XNOR_B200_ERR_INVALID; }
+	if ((long long)cache->pages * cache->kv_heads * (cache->page / 16) > 0x7fffffffLL) { return XNOR_B200_ERR_TOO_LARGE; }
 	const AttendPlan a = plan_attend(*cache, *rows, heads, window);
 	if (rows->batch > 65535 || (long long)a.tiles * cache->kv_heads > 65535 || (long long)rows->tokens * (heads / cache->kv_heads) > INT_MAX) { return XNOR_B200_ERR_TOO_LARGE; }
 	return XNOR_B200_OK;

@@ -115,18 +115,34 @@ __device__ __forceinline__ uint32_t pair_f16(float a, float b)
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2 *>(&w); }
 __device__ __forceinline__ uint32_t as_word(__half2 h) { return *reinterpret_cast<const uint32_t *>(&h); }
 
-// The low four bits of each half (even), or the next four (odd), as a pair of an operand.
+// The low four bits of each half (even), or the next four (odd), as a pair of an operand; upper: the codes of the high byte of each half, for
+// either.  Written as the instructions they are: left to itself the compiler shifts once for every mask, and the integer pipe is what
+// these kernels wait for.
+__device__ __forceinline__ uint32_t upper(uint32_t w)
+{
+	uint32_t r;
+	asm("shr.u32 %0, %1, 8;" : "=r"(r) : "r"(w));
+	return r;
+}
+template <uint32_t MASK, bool CENTRED>
+__device__ __forceinline__ uint32_t masked(uint32_t w)
+{
+	uint32_t r;
+	if (CENTRED) { asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "n"(MASK), "r"(0x64006400u)); }
+	else { asm("and.b32 %0, %1, %2;" : "=r"(r) : "r"(w), "n"(MASK)); }
+	return r;
+}
 template <bool CENTRED>
 __device__ __forceinline__ uint32_t even_codes(uint32_t w)
 {
-	if (!CENTRED) { return w & 0x000F000Fu; }
-	return as_word(__hadd2(as_half2((w & 0x000F000Fu) | 0x64006400u), as_half2(0xE408E408u)));
+	const uint32_t r = masked<0x000F000Fu, CENTRED>(w);
+	return CENTRED ? as_word(__hadd2(as_half2(r), as_half2(0xE408E408u))) : r;
 }
 template <bool CENTRED>
 __device__ __forceinline__ uint32_t odd_codes(uint32_t w)
 {
-	if (!CENTRED) { return w & 0x00F000F0u; }
-	return as_word(__hfma2(as_half2((w & 0x00F000F0u) | 0x64006400u), as_half2(0x2C002C00u), as_half2(0xD480D480u)));
+	const uint32_t r = masked<0x00F000F0u, CENTRED>(w);
+	return CENTRED ? as_word(__hfma2(as_half2(r), as_half2(0x2C002C00u), as_half2(0xD480D480u))) : r;
 }
 
 __device__ __forceinline__ float2 halves(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }

@@ -249,9 +249,9 @@ four_product_kernel(const ProductParams p)
 					#pragma unroll
 					for (int mt = 0; mt < MT; ++mt)
 					{
-						const uint32_t w0 = w[mt][0][j], w1 = w[mt][1][j];
-						const uint32_t even[4] = {even_codes<CENTRED>(w0), even_codes<CENTRED>(w1), even_codes<CENTRED>(w0 >> 8), even_codes<CENTRED>(w1 >> 8)};
-						const uint32_t odd[4] = {odd_codes<CENTRED>(w0), odd_codes<CENTRED>(w1), odd_codes<CENTRED>(w0 >> 8), odd_codes<CENTRED>(w1 >> 8)};
+						const uint32_t w0 = w[mt][0][j], w1 = w[mt][1][j], w0_up = upper(w0), w1_up = upper(w1);
+						const uint32_t even[4] = {even_codes<CENTRED>(w0), even_codes<CENTRED>(w1), even_codes<CENTRED>(w0_up), even_codes<CENTRED>(w1_up)};
+						const uint32_t odd[4] = {odd_codes<CENTRED>(w0), odd_codes<CENTRED>(w1), odd_codes<CENTRED>(w0_up), odd_codes<CENTRED>(w1_up)};
 						#pragma unroll
 						for (int nt = 0; nt < NT; ++nt)
 						{
