@@ -883,7 +883,7 @@ static int check_attend(const xnor_b200_kv4_cache * cache, const xnor_b200_kv4_r
 	if (heads <= 0 || heads % cache->kv_heads != 0 || window < 0) { return XNOR_B200_ERR_INVALID; }
 	if ((long long)cache->pages * cache->kv_heads * (cache->page / 16) > 0x7fffffffLL) { return XNOR_B200_ERR_TOO_LARGE; }
 	const AttendPlan a = plan_attend(*cache, *rows, heads, window);
-	if (rows->batch > 65535 || (long long)a.tiles * cache->kv_heads > 65535 || (long long)rows->tokens * (heads / cache->kv_heads) > INT_MAX) { return XNOR_B200_ERR_TOO_LARGE; }
+	if ((long long)a.tiles * cache->kv_heads > 65535 || (long long)rows->tokens * (heads / cache->kv_heads) > INT_MAX) { return XNOR_B200_ERR_TOO_LARGE; }
 	return XNOR_B200_OK;
 }
 

@@ -6,13 +6,36 @@
 // quotient up in fp32 on the way gives the same scale as one rounding of the exact quotient: each step's result is the smallest fp32 value
 // not below, and an fp16 value (times 15) is one of those.  NaN counts as 0, and what fp16 cannot hold as its largest value.
 //
-// A thread owns eight neighbours, one word of codes; the 4, 8 or 16 threads of a group find its minimum and maximum by shuffles.
+// A thread owns eight neighbours, one word of codes; the 4, 8 or 16 threads of a group find its minimum and maximum by shuffles.  Bound by
+// what a thread has to do (some 120 instructions for 16 bytes in) rather than by memory, so: the quotient is a product with 1/scale, whose
+// nearest integer is the bits of its sum with 1.5 * 2^23, and the remainder tells whether it is close to a half, where the division is done
+// after all; what fp16 cannot hold and NaN show in the minimum and the maximum.
 #include "four_common.cuh"
 
 namespace xnor
 {
 
 constexpr int FR_THREADS = 128;
+
+__device__ __forceinline__ float min_nan(float a, float b)
+{
+	float r;
+	asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+	return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+	float r;
+	asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+	return r;
+}
+
+__device__ __forceinline__ float reciprocal(float v)
+{
+	float r;
+	asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+	return r;
+}
 
 // Eight neighbours of a group, `there` of them real, to a word of codes; every lane of the group returns (scale, low).
 __device__ __forceinline__ uint32_t quantize8(float (&v)[8], int there, int group_lanes, __half2 & pair)
@@ -21,8 +44,18 @@ __device__ __forceinline__ uint32_t quantize8(float (&v)[8], int there, int grou
 	#pragma unroll
 	for (int i = 0; i < 8; ++i)
 	{
-		v[i] = v[i] != v[i] ? 0.0f : fminf(fmaxf(v[i], -65504.0f), 65504.0f);
-		if (i < there) { low = fminf(low, v[i]); top = fmaxf(top, v[i]); }
+		low = there == 8 || i < there ? min_nan(low, v[i]) : low;
+		top = there == 8 || i < there ? max_nan(top, v[i]) : top;
+	}
+	if (there > 0 && !(low >= -65504.0f && top <= 65504.0f))
+	{
+		low = INFINITY;
+		top = -INFINITY;
+		for (int i = 0; i < 8; ++i)
+		{
+			v[i] = v[i] != v[i] ? 0.0f : fminf(fmaxf(v[i], -65504.0f), 65504.0f);
+			if (i < there) { low = fminf(low, v[i]); top = fmaxf(top, v[i]); }
+		}
 	}
 	for (int m = 1; m < group_lanes; m <<= 1)
 	{
@@ -30,16 +63,33 @@ __device__ __forceinline__ uint32_t quantize8(float (&v)[8], int there, int grou
 		top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
 	}
 	const __half l = __float2half_rd(low);
-	const float base = __half2float(l);
-	const __half s = __float2half_ru(__fdiv_ru(__fsub_ru(top, base), 15.0f));
-	const float step = __half2float(s);
+	const float base = __half2float(l), range = __fsub_ru(top, base);
+	// the smallest fp16 value whose 15-fold is not below the range (a product of 15 bits, exact): next to the rounded quotient
+	uint32_t bits = __half_as_ushort(__float2half_rn(range * (1.0f / 15.0f)));
+	if (15.0f * __half2float(__ushort_as_half((unsigned short)bits)) < range) { ++bits; }
+	else if (bits > 0 && 15.0f * __half2float(__ushort_as_half((unsigned short)(bits - 1))) >= range) { --bits; }
+	const __half s = __ushort_as_half((unsigned short)bits);
+	const float step = __half2float(s), by = step > 0.0f ? reciprocal(step) : 0.0f;
 	pair = __halves2half2(s, l);
-	uint32_t word = 0;
+	// the bits of 1.5 * 2^23 + code are 0x4b400000 + code: times 16^i they add up to the word and a constant
+	uint32_t word = 0u - 0x4b400000u * 0x11111111u;
+	float furthest = 0.0f;
 	#pragma unroll
 	for (int i = 0; i < 8; ++i)
 	{
-		const float q = step > 0.0f && i < there ? rintf(__fdiv_rn(v[i] - base, step)) : 0.0f;
-		word |= (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f) << (4 * i);
+		const float d = v[i] - base, t = fmaf(d, by, 12582912.0f), c = t - 12582912.0f;
+		furthest = fmaxf(furthest, fabsf(fmaf(-c, step, d)));
+		word += __float_as_uint(t) * (1u << (4 * i));
+	}
+	// (1/scale and the product are off by less than 2^-22 of a quotient below 16; a scale of 0 has nothing further than 0)
+	if (there < 8 || furthest > step * (0.5f - 0x1p-17f))
+	{
+		word = 0;
+		for (int i = 0; i < 8; ++i)
+		{
+			const float q = step > 0.0f && i < there ? rintf(__fdiv_rn(v[i] - base, step)) : 0.0f;
+			word |= (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f) << (4 * i);
+		}
 	}
 	return word;
 }
@@ -53,7 +103,7 @@ four_weights_kernel(const T * __restrict__ weights, long long ld, int k, int gro
 	const T * row = weights + (long long)blockIdx.x * ld;
 	for (int w0 = 0; w0 < groups * lanes; w0 += FR_THREADS)
 	{
-		const int w = w0 + threadIdx.x, there = min(8, k - 8 * w);
+		const int w = w0 + threadIdx.x, there = max(0, min(8, k - 8 * w));
 		float v[8];
 		eight_f32(load8(row + 8 * (long long)w, there, wide != 0), v);
 		__half2 pair;
@@ -64,15 +114,17 @@ four_weights_kernel(const T * __restrict__ weights, long long ld, int k, int gro
 }
 
 // The page and the place of row i of sequence b; page < 0: there is none.
-__device__ __forceinline__ void find_row(const xnor_b200_kv4_cache & c, const xnor_b200_kv4_rows & r, int b, int i, long long & page, int & place)
+__device__ __forceinline__ void find_row(const xnor_b200_kv4_cache & c, const xnor_b200_kv4_rows & r, int b, int i, int & page, int & place)
 {
 	const int count = r.counts != nullptr ? __ldg(r.counts + b) : r.tokens;
 	const long long at = (long long)__ldg(r.lengths + b) - count + i;
 	page = -1;
 	place = 0;
-	if (i >= count || at < 0 || at >= (long long)r.max_pages * c.page) { return; }
-	const int p = __ldg(r.table + (long long)b * r.max_pages + at / c.page);
-	if (p >= 0 && p < c.pages) { page = p; place = (int)(at % c.page); }
+	if (i >= count || at < 0 || at > 0x7fffffffLL) { return; }               // (a length is below 2^31)
+	const uint32_t of = (uint32_t)at / (uint32_t)c.page;
+	if (of >= (uint32_t)r.max_pages) { return; }
+	const int p = __ldg(r.table + (size_t)b * r.max_pages + of);
+	if (p >= 0 && p < c.pages) { page = p; place = (int)((uint32_t)at - of * (uint32_t)c.page); }
 }
 
 struct RowsParams
@@ -81,61 +133,101 @@ struct RowsParams
 	xnor_b200_kv4_rows r;
 	xnor_b200_kv4_tensor t[2];       // keys, values
 	int wide[2];                     // rows of it start on 16 bytes
+	int words;                       // of a row of tokens, all heads
+	int warps;                       // that share a row
+	uint32_t by_words;               // ceil(2^32 / words of a head): the high half of a product with it divides what is below 2^27
 };
 
-// One block a row of tokens and half (keys or values).
+// What a thread does: the words of one row from `first` on.  Every thread of a warp goes through the same number of turns (the groups'
+// shuffles need all of them).
+struct RowsTask
+{
+	int i, first, step;
+};
+
+__device__ __forceinline__ RowsTask task_of(const RowsParams & p)
+{
+	RowsTask k;
+	k.step = 32 * p.warps;
+	k.first = p.warps == 1 ? (int)threadIdx.x % 32 : (int)threadIdx.x;
+	k.i = p.warps == 1 ? (int)(blockIdx.x * (FR_THREADS / 32) + threadIdx.x / 32) : (int)blockIdx.x;
+	return k;
+}
+
+// A block takes one row, or each of its warps one: of keys or of values.
 template <class T>
 __global__ void __launch_bounds__(FR_THREADS)
 kv4_append_kernel(const RowsParams p)
 {
-	const int half = blockIdx.y, b = blockIdx.x / p.r.tokens, i = blockIdx.x - b * p.r.tokens;
-	long long page;
-	int place;
-	find_row(p.c, p.r, b, i, page, place);
+	const int half = blockIdx.z, b = blockIdx.y;
+	const RowsTask k = task_of(p);
+	if (k.i >= p.r.tokens) { return; }
+	int page, place;
+	find_row(p.c, p.r, b, k.i, page, place);
 	if (page < 0) { return; }
 	const xnor_b200_kv4_tensor & t = p.t[half];
-	const int words = p.c.dim / 8, lanes = p.c.group / 8, groups = p.c.dim / p.c.group, total = words * p.c.kv_heads;
-	const T * src = (const T *)t.data + b * t.stride_sequence + i * t.stride_token;
+	const int words = p.c.dim / 8, lanes = p.c.group / 8, groups = p.c.dim / p.c.group;
+	const T * src = (const T *)t.data + b * t.stride_sequence + k.i * t.stride_token;
+	const size_t row0 = (size_t)page * p.c.kv_heads * p.c.page + place;
 	uint32_t * codes = (uint32_t *)(half ? p.c.v_codes : p.c.k_codes);
 	__half2 * scales = (__half2 *)(half ? p.c.v_scales : p.c.k_scales);
-	for (int w0 = 0; w0 < total; w0 += FR_THREADS)
+	#pragma unroll 2
+	for (int w0 = 0; w0 < p.words; w0 += k.step)
 	{
-		const int w = w0 + threadIdx.x, head = w / words, word = w - head * words;
+		const int w = w0 + k.first, head = (int)__umulhi((uint32_t)w, p.by_words), word = w - head * words;
 		float v[8];
-		eight_f32(load8(src + head * t.stride_head + 8 * word, w < total ? 8 : 0, p.wide[half] != 0), v);
+		eight_f32(load8(src + head * t.stride_head + 8 * word, w < p.words ? 8 : 0, p.wide[half] != 0), v);
 		__half2 pair;
 		const uint32_t c = quantize8(v, 8, lanes, pair);
-		if (w >= total) { continue; }
-		const long long row = (page * p.c.kv_heads + head) * p.c.page + place;
+		if (w >= p.words) { continue; }
+		const size_t row = row0 + (size_t)head * p.c.page;
 		codes[row * words + word] = c;
-		if (word % lanes == 0) { scales[row * groups + word / lanes] = pair; }
+		if ((word & (lanes - 1)) == 0) { scales[row * groups + word * 8 / p.c.group] = pair; }
 	}
+}
+
+// Codes as pairs of fp16 numbers, the low four bits of each half (even) or the next four (odd).
+__device__ __forceinline__ float2 even_values(uint32_t w)
+{
+	return __half22float2(__hadd2(as_half2(masked<0x000F000Fu, true>(w)), as_half2(0xE400E400u)));
+}
+__device__ __forceinline__ float2 odd_values(uint32_t w)
+{
+	return __half22float2(__hfma2(as_half2(masked<0x00F000F0u, true>(w)), as_half2(0x2C002C00u), as_half2(0xD400D400u)));
 }
 
 template <class T>
 __global__ void __launch_bounds__(FR_THREADS)
 kv4_read_kernel(const RowsParams p)
 {
-	const int half = blockIdx.y, b = blockIdx.x / p.r.tokens, i = blockIdx.x - b * p.r.tokens;
-	long long page;
-	int place;
-	find_row(p.c, p.r, b, i, page, place);
+	const int half = blockIdx.z, b = blockIdx.y;
+	const RowsTask k = task_of(p);
+	if (k.i >= p.r.tokens) { return; }
+	int page, place;
+	find_row(p.c, p.r, b, k.i, page, place);
 	const xnor_b200_kv4_tensor & t = p.t[half];
-	const int words = p.c.dim / 8, lanes = p.c.group / 8, groups = p.c.dim / p.c.group, total = words * p.c.kv_heads;
-	T * dst = (T *)t.data + b * t.stride_sequence + i * t.stride_token;
+	const int words = p.c.dim / 8, groups = p.c.dim / p.c.group, shift = p.c.group == 32 ? 2 : p.c.group == 64 ? 3 : 4;
+	T * dst = (T *)t.data + b * t.stride_sequence + k.i * t.stride_token;
+	const size_t row0 = (size_t)max(page, 0) * p.c.kv_heads * p.c.page + place;
 	const uint32_t * codes = (const uint32_t *)(half ? p.c.v_codes : p.c.k_codes);
-	const __half2 * scales = (const __half2 *)(half ? p.c.v_scales : p.c.k_scales);
-	for (int w = threadIdx.x; w < total; w += FR_THREADS)
+	const uint32_t * scales = (const uint32_t *)(half ? p.c.v_scales : p.c.k_scales);
+	#pragma unroll 4
+	for (int w = k.first; w < p.words; w += k.step)
 	{
-		const int head = w / words, word = w - head * words;
+		const int head = (int)__umulhi((uint32_t)w, p.by_words), word = w - head * words;
 		float v[8] = {};
 		if (page >= 0)
 		{
-			const long long row = (page * p.c.kv_heads + head) * p.c.page + place;
-			const uint32_t c = codes[row * words + word];
-			const float2 sl = __half22float2(scales[row * groups + word / lanes]);
+			const size_t row = row0 + (size_t)head * p.c.page;
+			const uint32_t c = __ldg(codes + row * words + word), up = upper(c);
+			const float2 sl = halves(__ldg(scales + row * groups + (word >> shift)));
+			const float2 pairs[4] = {even_values(c), odd_values(c), even_values(up), odd_values(up)};       // 0 and 4, 1 and 5, 2 and 6, 3 and 7
 			#pragma unroll
-			for (int e = 0; e < 8; ++e) { v[e] = __fmaf_rn(sl.x, (float)((c >> (4 * e)) & 15), sl.y); }
+			for (int e = 0; e < 4; ++e)
+			{
+				v[e] = __fmaf_rn(sl.x, pairs[e].x, sl.y);
+				v[e + 4] = __fmaf_rn(sl.x, pairs[e].y, sl.y);
+			}
 		}
 		store8(dst + head * t.stride_head + 8 * word, p.wide[half] != 0, v);
 	}
@@ -148,7 +240,7 @@ int validate_kv4(const xnor_b200_kv4_cache * c, const xnor_b200_kv4_rows * r)
 	if (c == nullptr || r == nullptr) { return XNOR_B200_ERR_NULL; }
 	if (c->pages <= 0 || c->kv_heads <= 0 || c->page <= 0 || c->page % 16 != 0 || c->dim <= 0 || c->dim % 32 != 0 || !four_group_ok(c->group)
 			|| c->dim % c->group != 0 || r->batch <= 0 || r->tokens <= 0 || r->max_pages <= 0) { return XNOR_B200_ERR_INVALID; }
-	if (c->dim > XNOR_B200_KV4_MAX_DIM || c->kv_heads > 65535 || c->page > (1 << 20) || (long long)r->batch * r->tokens > 0x7fffffffLL) { return XNOR_B200_ERR_TOO_LARGE; }
+	if (c->dim > XNOR_B200_KV4_MAX_DIM || c->kv_heads > 65535 || c->page > (1 << 20) || r->batch > 65535) { return XNOR_B200_ERR_TOO_LARGE; }
 	if (c->k_codes == nullptr || c->k_scales == nullptr || c->v_codes == nullptr || c->v_scales == nullptr || r->table == nullptr || r->lengths == nullptr)
 	{
 		return XNOR_B200_ERR_NULL;
@@ -166,6 +258,10 @@ static int fill_rows(RowsParams & p, const xnor_b200_kv4_cache * c, const xnor_b
 	if (!four_dtype_ok(k->dtype) || k->dtype != v->dtype) { return XNOR_B200_ERR_INVALID; }
 	p.c = *c;
 	p.r = *r;
+	p.words = c->kv_heads * (c->dim / 8);
+	// a warp a row where there are rows enough to fill a block with them; fewer are the sooner done the more threads they have
+	p.warps = r->tokens >= FR_THREADS / 32 ? 1 : FR_THREADS / 32;
+	p.by_words = (uint32_t)((0xffffffffu / (uint32_t)(c->dim / 8)) + 1);
 	const xnor_b200_kv4_tensor * both[2] = {k, v};
 	for (int i = 0; i < 2; ++i)
 	{
@@ -222,7 +318,7 @@ extern "C" int xnor_b200_kv4_append(const xnor_b200_kv4_cache * cache, const xno
 	RowsParams p;
 	const int rc = fill_rows(p, cache, rows, k, v);
 	if (rc != XNOR_B200_OK) { return rc; }
-	const dim3 grid((unsigned)(rows->batch * rows->tokens), 2);
+	const dim3 grid((unsigned)(p.warps == 1 ? (rows->tokens - 1) / (FR_THREADS / 32) + 1 : rows->tokens), (unsigned)rows->batch, 2);
 	const cudaStream_t s = (cudaStream_t)stream;
 	if (k->dtype == XNOR_B200_F32) { kv4_append_kernel<float><<<grid, FR_THREADS, 0, s>>>(p); }
 	else if (k->dtype == XNOR_B200_F16) { kv4_append_kernel<__half><<<grid, FR_THREADS, 0, s>>>(p); }
@@ -236,7 +332,7 @@ extern "C" int xnor_b200_kv4_read(const xnor_b200_kv4_cache * cache, const xnor_
 	RowsParams p;
 	const int rc = fill_rows(p, cache, rows, k, v);
 	if (rc != XNOR_B200_OK) { return rc; }
-	const dim3 grid((unsigned)(rows->batch * rows->tokens), 2);
+	const dim3 grid((unsigned)(p.warps == 1 ? (rows->tokens - 1) / (FR_THREADS / 32) + 1 : rows->tokens), (unsigned)rows->batch, 2);
 	const cudaStream_t s = (cudaStream_t)stream;
 	if (k->dtype == XNOR_B200_F32) { kv4_read_kernel<float><<<grid, FR_THREADS, 0, s>>>(p); }
 	else if (k->dtype == XNOR_B200_F16) { kv4_read_kernel<__half><<<grid, FR_THREADS, 0, s>>>(p); }

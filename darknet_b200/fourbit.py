@@ -63,7 +63,14 @@ def _on(device: torch.device, *tensors) -> None:
         raise ValueError(f"tensors on {device}: this path runs on a CUDA device only")
 
 
-class Matrix4:
+class _Fixed:
+    """What a handle was made of and checked for stays what it is."""
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{type(self).__name__} keeps the buffers and sizes that it was made with: make another")
+
+
+class Matrix4(_Fixed):
     """A packed matrix of n rows of k values (struct xnor_b200_w4_desc with its two buffers): codes uint8 [n][ceil(k/32)*16], scales fp16
     [n][ceil(k/group)][2], both contiguous."""
 
@@ -76,9 +83,8 @@ class Matrix4:
             raise ValueError(f"scales must be contiguous fp16 [{codes.shape[0]}][{(k + group - 1) // group}][2]")
         if scales.device != codes.device:
             raise ValueError(f"codes on {codes.device}, scales on {scales.device}")
-        self.codes, self.scales, self.n, self.k, self.group, self.device = codes, scales, codes.shape[0], k, group, codes.device
-        self._index = codes.get_device()
-        self._descs = {a: bytes(capi.W4Desc(self.n, k, group, a)) for a in (capi.LINEAR, capi.LEAKY)}
+        self.__dict__.update(codes=codes, scales=scales, n=codes.shape[0], k=k, group=group, device=codes.device, _index=codes.get_device(),
+                             _descs={a: bytes(capi.W4Desc(codes.shape[0], k, group, a)) for a in (capi.LINEAR, capi.LEAKY)})
 
 
 def quantize_weights4(weights: torch.Tensor, group: int) -> Matrix4:
@@ -117,26 +123,27 @@ def forward_connected4(m: Matrix4, x: torch.Tensor, biases: Optional[torch.Tenso
     """act(x @ W.T + biases) for x [rows][k] (rows contiguous, any distance apart), W the packed matrix: xnor_b200_w4_forward.
     biases: fp32 [n].  out: [rows][n] of x's type, rows contiguous; made where it is not given.  One pass over the weights serves up to
     16 rows."""
-    index, shape, dtype, desc = m._index, x.shape, _DTYPES.get(x.dtype), m._descs.get(activation)
-    if (index < 0 or dtype is None or desc is None or biases is not None or out is not None or len(shape) != 2 or shape[1] != m.k
-            or x.get_device() != index or m.codes.get_device() != index or m.scales.get_device() != index or not x.is_contiguous()):
+    index, shape, dtype, desc, n = m._index, x.shape, _DTYPES.get(x.dtype), m._descs.get(activation), m.n
+    if (index < 0 or dtype is None or desc is None or out is not None or len(shape) != 2 or shape[1] != m.k or x.get_device() != index
+            or not x.is_contiguous()
+            or (biases is not None and (biases.dtype is not torch.float32 or biases.shape != (n,) or not biases.is_contiguous() or biases.get_device() != index))):
         _refuse_product(m, x, biases, activation, out)
     if _current_device() != index:
         with torch.cuda.device(index):
             return forward_connected4(m, x, biases, activation, out)
     rows = shape[0]
     if out is None:
-        out = x.new_empty((rows, m.n))
+        out = x.new_empty((rows, n))
     if rows == 0:
         return out
     rc = _calls.w4_forward(desc, x.data_ptr(), dtype, rows, x.stride(0) if rows > 1 else m.k, m.codes.data_ptr(), m.scales.data_ptr(),
-                           None if biases is None else biases.data_ptr(), out.data_ptr(), out.stride(0) if rows > 1 else m.n, _raw_stream(index))
+                           None if biases is None else biases.data_ptr(), out.data_ptr(), out.stride(0) if rows > 1 else n, _raw_stream(index))
     if rc:
         capi.check(rc, "xnor_b200_w4_forward")
     return out
 
 
-class Cache4:
+class Cache4(_Fixed):
     """Pages of four-bit keys and values (struct xnor_b200_kv4_cache): codes uint8 [pages][kv_heads][page][dim/2], scales fp16
     [pages][kv_heads][page][dim/group][2], contiguous."""
 
@@ -156,13 +163,12 @@ class Cache4:
                 raise ValueError(f"scales must be contiguous fp16 {[pages, kv_heads, page, dim // group, 2]}")
             if codes.device != k_codes.device or scales.device != k_codes.device:
                 raise ValueError("all four buffers must be on one device")
-        self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
-        self.pages, self.kv_heads, self.page, self.dim, self.group, self.device = pages, kv_heads, page, dim, group, k_codes.device
-        self._index = k_codes.get_device()
-        self._scratch: dict = {}                              # bytes of scratch memory by the sizes of a call
+        # _scratch: bytes of scratch memory by the sizes of a call
+        self.__dict__.update(k_codes=k_codes, k_scales=k_scales, v_codes=v_codes, v_scales=v_scales, pages=pages, kv_heads=kv_heads, page=page,
+                             dim=dim, group=group, device=k_codes.device, _index=k_codes.get_device(), _scale=dim ** -0.5, _scratch={})
 
     def _struct(self) -> bytes:
-        """Packed for every call, so that it never names memory of a tensor that was replaced."""
+        """Packed for every call, so that it never names memory that a tensor has given up."""
         return _CACHE(self.k_codes.data_ptr(), self.k_scales.data_ptr(), self.v_codes.data_ptr(), self.v_scales.data_ptr(), self.pages,
                       self.kv_heads, self.page, self.dim, self.group)
 
@@ -268,8 +274,8 @@ def attend4(c: Cache4, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tens
         with torch.cuda.device(index):
             return attend4(c, q, table, lengths, counts, scale, window, out, lse)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=c.device)
-    if q.numel() == 0:
+        out = torch.empty_like(q)
+    if batch == 0 or tokens == 0:
         return out
     ot = _tensor(out, dtype, index, "out")
     cache, sizes = c._struct(), (batch, tokens, table.shape[1], heads, window)
@@ -279,7 +285,7 @@ def attend4(c: Cache4, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tens
             c._scratch.clear()
         nbytes = c._scratch[sizes] = _calls.kv4_attend_scratch_bytes(cache, rows, heads, window)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=c.device) if nbytes else None
-    rc = _calls.kv4_attend(cache, rows, qt, heads, c.dim ** -0.5 if scale is None else scale, window, ot, None if lse is None else lse.data_ptr(),
+    rc = _calls.kv4_attend(cache, rows, qt, heads, c._scale if scale is None else scale, window, ot, None if lse is None else lse.data_ptr(),
                            None if scratch is None else scratch.data_ptr(), nbytes, _raw_stream(index))
     if rc:
         capi.check(rc, "xnor_b200_kv4_attend")
