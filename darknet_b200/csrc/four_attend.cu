@@ -54,12 +54,16 @@ struct Span
 	int first, last;              // first step of 16 positions and the one behind the last, of all columns
 };
 
+// The token that a column asks for (one token: no division; this and its like are a good part of a short call).
+__device__ __forceinline__ int row_of(const AttendParams & p, int col) { return p.r.tokens == 1 ? 0 : col / p.share; }
+
 __device__ __forceinline__ Span span_of(const AttendParams & p, int b, int i0, int i1)
 {
 	Span s;
-	s.count = p.r.counts != nullptr ? min(__ldg(p.r.counts + b), p.r.tokens) : p.r.tokens;
+	const int count = p.r.counts != nullptr ? __ldg(p.r.counts + b) : p.r.tokens;
+	s.count = min(count, p.r.tokens);
 	const int length = max(__ldg(p.r.lengths + b), 0);
-	const long long at = (long long)length - (p.r.counts != nullptr ? __ldg(p.r.counts + b) : p.r.tokens), room = (long long)p.r.max_pages * p.c.page;
+	const long long at = (long long)length - count, room = (long long)p.r.max_pages * p.c.page;
 	s.at = (int)max(at, -0x40000000LL);                   // (rows that far in front of a sequence see nothing either way)
 	s.end = (int)min((long long)length, room);
 	i1 = min(i1, s.count - 1);
@@ -73,7 +77,7 @@ __device__ __forceinline__ Span span_of(const AttendParams & p, int b, int i0, i
 // Steps of one split, whole pairs for each warp: the same for the kernel and for the one that joins.
 __device__ __forceinline__ int steps_of_split(const Span & s, int splits)
 {
-	const int n = s.last - s.first, each = n / splits + (n % splits != 0);
+	const int n = s.last - s.first, each = splits == 1 ? n : (int)((uint32_t)(n + splits - 1) / (uint32_t)splits);
 	return max((each + 1) / 2 * 2, 2 * FA_WARPS);
 }
 
@@ -89,11 +93,11 @@ __device__ __forceinline__ float weight_of(float m, float top) { return m == -IN
 
 __device__ __forceinline__ void add_weighted(float4 & v, float by, const float4 & u)
 {
-	if (by == 0.0f) { return; }
-	v.x += by * u.x;
-	v.y += by * u.y;
-	v.z += by * u.z;
-	v.w += by * u.w;
+	// (what counts for nothing may be anything)
+	v.x += by == 0.0f ? 0.0f : by * u.x;
+	v.y += by == 0.0f ? 0.0f : by * u.y;
+	v.z += by == 0.0f ? 0.0f : by * u.z;
+	v.w += by == 0.0f ? 0.0f : by * u.w;
 }
 
 // Four channels of a row, from its sums at maximum m and their total l.
@@ -125,6 +129,9 @@ template <> struct Parts<float> { static constexpr int Q = 2, P = 2; };
 
 // A stage holds 32 positions: rows of keys' codes, rows of values' codes, scales.  A lane reads GB words of a row of a group; the pitches
 // put rows that are read at a time into different banks.
+// CTAs that an SM holds: 128 registers a thread for most shapes, shared memory for the widest.
+__host__ __device__ constexpr int attend_on_sm(int nb, int nt) { return nt == 2 ? (nb <= 2 ? 3 : 2) : nb <= 5 ? 4 : nb <= 7 ? 3 : 2; }
+
 template <int NB, int GB, int NT, int QP>
 struct AttendShape
 {
@@ -182,7 +189,7 @@ __device__ __forceinline__ void weigh(uint32_t (&pv)[NT][PP][2], float (&lows)[N
 
 // NB: blocks of 32 channels.  GB: blocks of a group.  NT: tiles of eight columns.
 template <class T, int NB, int GB, int NT>
-__global__ void __launch_bounds__(FA_THREADS)
+__global__ void __launch_bounds__(FA_THREADS, attend_on_sm(NB, NT))
 four_attend_kernel(const AttendParams p)
 {
 	constexpr int QP = Parts<T>::Q, PP = Parts<T>::P;
@@ -202,9 +209,11 @@ four_attend_kernel(const AttendParams p)
 	float * s_l = s_m + FA_WARPS * COLS, * s_by = s_l + FA_WARPS * COLS;
 	float * s_top = s_by + FA_WARPS * COLS, * s_all = s_top + COLS;                   // [column]
 
-	const int b = blockIdx.z, head = blockIdx.y / p.tiles, tile = blockIdx.y % p.tiles, split = blockIdx.x;
+	if (p.partial != nullptr) { pdl_trigger(); }              // the kernel that joins may be launched; it waits for this one's end
+
+	const int b = blockIdx.z, head = p.tiles == 1 ? blockIdx.y : blockIdx.y / p.tiles, tile = p.tiles == 1 ? 0 : blockIdx.y % p.tiles, split = blockIdx.x;
 	const int col0 = tile * COLS, cols = min(COLS, p.r.tokens * p.share - col0);
-	const Span span = span_of(p, b, col0 / p.share, (col0 + cols - 1) / p.share);
+	const Span span = span_of(p, b, row_of(p, col0), row_of(p, col0 + cols - 1));
 	const int per = steps_of_split(span, p.splits);
 	const int begin = (int)min((long long)span.last, span.first + (long long)split * per), end = min(span.last, begin + per);
 
@@ -279,30 +288,25 @@ four_attend_kernel(const AttendParams p)
 	#pragma unroll
 	for (int i = 0; i < FA_STAGES - 1; ++i) { request(i); }
 
-	// ---- the queries: a warp takes a column, a lane eight channels
-	for (int c = warp; c < COLS; c += FA_WARPS)
+	// ---- the queries: a lane takes eight channels, half a warp a column (a whole one where there are more than 128 channels)
+	constexpr int SIDE = NB <= 4 ? 16 : 32;
+	const int side = lane % SIDE;
+	#pragma unroll
+	for (int c0 = 0; c0 < COLS; c0 += FA_THREADS / SIDE)
 	{
-		const int i = (col0 + c) / p.share, h = head * p.share + (col0 + c) % p.share;
-		if (c >= cols || i >= span.count)                     // (sees nothing)
-		{
-			for (int j = lane; j < QP * NB * 4; j += 32) { *(uint4 *)(s_q + (j / (NB * 4) * COLS + c) * S::Q_PITCH + j % (NB * 4) * 16) = make_uint4(0, 0, 0, 0); }
-			if (lane < GROUPS) { s_qsum[lane * COLS + c] = 0.0f; }
-			if (lane == 0)
-			{
-				s_qf[c] = 0.0f;
-				s_from[c] = s_to[c] = 0;
-			}
-			continue;
-		}
+		const int c = c0 + threadIdx.x / SIDE;
+		if (c0 + FA_THREADS / SIDE > COLS && c >= COLS) { break; }
+		const int i = row_of(p, col0 + c), h = head * p.share + col0 + c - i * p.share;
+		const bool there = c < cols && i < span.count;        // (others see nothing)
 		float v[8];
-		eight_f32(load8((const T *)p.q.data + b * p.q.stride_sequence + i * p.q.stride_token + h * p.q.stride_head + lane * 8,
-				lane < NB * 4 ? 8 : 0, p.wide_q != 0), v);
-		uint32_t largest = 0;
+		eight_f32(load8((const T *)p.q.data + b * p.q.stride_sequence + i * p.q.stride_token + h * p.q.stride_head + side * 8,
+				there && side < NB * 4 ? 8 : 0, p.wide_q != 0), v);
+		float most = 0.0f, part = 0.0f, factor, inverse;
 		#pragma unroll
-		for (int e = 0; e < 8; ++e) { largest = max(largest, __float_as_uint(fabsf(v[e]))); }
-		largest = __reduce_max_sync(0xffffffffu, largest);
-		float factor, inverse, part = 0.0f;
-		fit_f16(largest, factor, inverse);
+		for (int e = 0; e < 8; ++e) { most = max_nan(most, fabsf(v[e])); }
+		#pragma unroll
+		for (int m = 1; m < SIDE; m <<= 1) { most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, m)); }
+		fit_f16(__float_as_uint(most) & 0x7fffffffu, factor, inverse);
 		#pragma unroll
 		for (int e = 0; e < 8; ++e)
 		{
@@ -311,14 +315,14 @@ four_attend_kernel(const AttendParams p)
 		}
 		#pragma unroll
 		for (int m = 1; m < GB * 4; m <<= 1) { part += __shfl_xor_sync(0xffffffffu, part, m); }
-		if (lane < NB * 4 && lane % (GB * 4) == 0) { s_qsum[lane / (GB * 4) * COLS + c] = part * (1.0f / How::UNIT); }
-		if (lane == 0)
+		if (side < NB * 4 && side % (GB * 4) == 0) { s_qsum[side / (GB * 4) * COLS + c] = part * (1.0f / How::UNIT); }
+		if (side == 0)
 		{
 			s_qf[c] = inverse * (How::UNIT * p.scale_log2);
-			s_to[c] = min(span.end, span.at + i + 1);
-			s_from[c] = p.window > 0 ? max(0, span.at + i + 1 - p.window) : 0;
+			s_to[c] = there ? min(span.end, span.at + i + 1) : 0;
+			s_from[c] = there && p.window > 0 ? max(0, span.at + i + 1 - p.window) : 0;
 		}
-		if (lane < NB * 4)
+		if (side < NB * 4)
 		{
 			float high[8], rest[8];
 			#pragma unroll
@@ -328,7 +332,7 @@ four_attend_kernel(const AttendParams p)
 				if (QP == 2) { split_f16(high[e], high[e], rest[e]); }
 			}
 			// the four lanes of a row read GB words each of a group: those of a place lie side by side
-			unsigned char * at = s_q + c * S::Q_PITCH + (lane / (4 * GB) * (4 * GB) + lane % GB * 4 + lane / GB % 4) * 16;
+			unsigned char * at = s_q + c * S::Q_PITCH + (side / (4 * GB) * (4 * GB) + side % GB * 4 + side / GB % 4) * 16;
 			*reinterpret_cast<uint4 *>(at) = make_uint4(pair_f16(high[0], high[4]), pair_f16(high[2], high[6]), pair_f16(high[1], high[5]), pair_f16(high[3], high[7]));
 			if (QP == 2)
 			{
@@ -338,7 +342,7 @@ four_attend_kernel(const AttendParams p)
 	}
 	__syncthreads();
 	// Positions that every column of a token sees: no step inside them asks again
-	const int row_first = col0 / p.share, row_last = min((col0 + cols - 1) / p.share, span.count - 1);
+	const int row_first = row_of(p, col0), row_last = min(row_of(p, col0 + cols - 1), span.count - 1);
 	const int all_to = min(span.end, span.at + row_first + 1), all_from = p.window > 0 ? max(0, span.at + row_last + 1 - p.window) : 0;
 
 	float o[GROUPS][GB][2][NT][4] = {};                       // [group][word][even, odd channels][tile][channel of g: columns 2t, 2t+1; of g + 8]
@@ -650,11 +654,9 @@ four_attend_kernel(const AttendParams p)
 				#pragma unroll
 				for (int j = 0; j < GB; ++j)
 				{
-					float * to = u + c * S::U_PITCH + (gr * 4 * GB + (g & 3) * GB + j) * 8 + (g >> 2) * 4;
-					to[0] = o[gr][j][0][nt][e] * by + low;
-					to[2] = o[gr][j][0][nt][2 + e] * by + low;
-					to[1] = o[gr][j][1][nt][e] * by + low;
-					to[3] = o[gr][j][1][nt][2 + e] * by + low;
+					float4 * to = (float4 *)(u + c * S::U_PITCH + (gr * 4 * GB + (g & 3) * GB + j) * 8 + (g >> 2) * 4);
+					const auto & even = o[gr][j][0][nt], & odd = o[gr][j][1][nt];
+					*to = make_float4(even[e] * by + low, odd[e] * by + low, even[2 + e] * by + low, odd[2 + e] * by + low);
 				}
 			}
 		}
@@ -709,7 +711,7 @@ four_attend_kernel(const AttendParams p)
 	cluster.sync();
 	for (int i = rank * FA_THREADS + threadIdx.x; i < cols * quads; i += ranks * FA_THREADS)
 	{
-		const int c = i / quads, q = i - c * quads, row = (col0 + c) / p.share, h = head * p.share + (col0 + c) % p.share;
+		const int c = i / quads, q = i - c * quads, row = row_of(p, col0 + c), h = head * p.share + col0 + c - row * p.share;
 		float m = -INFINITY, l = 0.0f;
 		float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 		for (int r = 0; r < ranks; ++r) { m = fmaxf(m, cluster.map_shared_rank(s_top, r)[c]); }
@@ -725,59 +727,72 @@ four_attend_kernel(const AttendParams p)
 	cluster.sync();                                           // nobody leaves while its sums are read
 }
 
-// A warp takes a column's 128 channels: joins what the splits left.
+// Joins what the splits left, a block a column: what each split counts for is worked out once, then every warp adds up every eighth split,
+// whose loads are all on their way at once.  Starts while the splits are still at work (its launch would take as long as its work).
+constexpr int FJ_WARPS = 8, FJ_THREADS = 32 * FJ_WARPS, FJ_SPLITS = 1024;
+
 template <class T>
-__global__ void __launch_bounds__(FA_THREADS)
+__global__ void __launch_bounds__(FJ_THREADS)
 four_attend_join_kernel(const AttendParams p, int cols_of_tile)
 {
-	const int dim = p.c.dim, quads = dim / 4;
+	const int dim = p.c.dim, quads = dim / 4, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 	const int b = blockIdx.z, head = blockIdx.y, col = blockIdx.x, tile = col / cols_of_tile, c = col - tile * cols_of_tile;
-	const int row = col / p.share, h = head * p.share + col % p.share;
+	const int row = row_of(p, col), h = head * p.share + col - row * p.share;
 	const int col0 = tile * cols_of_tile, cols = min(cols_of_tile, p.r.tokens * p.share - col0);
-	const Span span = span_of(p, b, col0 / p.share, (col0 + cols - 1) / p.share);
+	const Span span = span_of(p, b, row_of(p, col0), row_of(p, col0 + cols - 1));
 	const int per = steps_of_split(span, p.splits), used = (span.last - span.first + per - 1) / per;
 	const size_t pitch = (size_t)cols_of_tile * (dim + 4);
 	const float * from = p.partial + ((size_t)(b * p.c.kv_heads + head) * p.tiles + tile) * p.splits * pitch;
 	const float * tops = from + cols_of_tile * dim + c, * totals = tops + cols_of_tile;
-	// every warp joins every fourth split, then the four of them meet
-	__shared__ float s_m[FA_WARPS], s_l[FA_WARPS];
-	__shared__ float4 s_v[FA_WARPS][64];
-	const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+	__shared__ float s_by[FJ_SPLITS], s_m[FJ_WARPS], s_l[FJ_WARPS];
+	__shared__ float4 s_v[FJ_WARPS][64];
+	pdl_wait();
+
 	float m = -INFINITY, l = 0.0f;
-	for (int s = warp + lane * FA_WARPS; s < used; s += 32 * FA_WARPS) { m = fmaxf(m, tops[s * pitch]); }
+	for (int s = threadIdx.x; s < used; s += FJ_THREADS)
+	{
+		const float top = tops[s * pitch];
+		s_by[s] = top;
+		m = fmaxf(m, top);
+	}
 	#pragma unroll
 	for (int i = 1; i < 32; i <<= 1) { m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i)); }
-	float4 v[2] = {};
-	for (int s = warp; s < used; s += FA_WARPS)
+	if (lane == 0) { s_m[warp] = m; }
+	__syncthreads();
+	#pragma unroll
+	for (int w = 0; w < FJ_WARPS; ++w) { m = fmaxf(m, s_m[w]); }
+	for (int s = threadIdx.x; s < used; s += FJ_THREADS)
 	{
-		const float by = weight_of(tops[s * pitch], m);
-		if (by == 0.0f) { continue; }
-		l += by * totals[s * pitch];
+		const float by = weight_of(s_by[s], m);
+		s_by[s] = by;
+		l += by == 0.0f ? 0.0f : by * totals[s * pitch];
+	}
+	#pragma unroll
+	for (int i = 1; i < 32; i <<= 1) { l += __shfl_xor_sync(0xffffffffu, l, i); }
+	if (lane == 0) { s_l[warp] = l; }
+	__syncthreads();
+	float4 v[2] = {};
+	#pragma unroll 8
+	for (int s = warp; s < used; s += FJ_WARPS)
+	{
 		#pragma unroll
 		for (int j = 0; j < 2; ++j)
 		{
-			if (lane + j * 32 < quads) { add_weighted(v[j], by, *(const float4 *)(from + s * pitch + c * dim + (lane + j * 32) * 4)); }
+			if (lane + j * 32 < quads) { add_weighted(v[j], s_by[s], *(const float4 *)(from + s * pitch + c * dim + (lane + j * 32) * 4)); }
 		}
-	}
-	if (lane == 0)
-	{
-		s_m[warp] = m;
-		s_l[warp] = l;
 	}
 	s_v[warp][lane] = v[0];
 	s_v[warp][lane + 32] = v[1];
 	__syncthreads();
-	for (int q = threadIdx.x; q < quads; q += FA_THREADS)
+	for (int q = threadIdx.x; q < quads; q += FJ_THREADS)
 	{
-		m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
 		l = 0.0f;
 		float4 all = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 		#pragma unroll
-		for (int w = 0; w < FA_WARPS; ++w)
+		for (int w = 0; w < FJ_WARPS; ++w)
 		{
-			const float by = weight_of(s_m[w], m);
-			l += by == 0.0f ? 0.0f : by * s_l[w];
-			add_weighted(all, by, s_v[w][q]);
+			l += s_l[w];
+			add_weighted(all, 1.0f, s_v[w][q]);
 		}
 		write_out<T>(p, b, row, h, q * 4, row >= span.count, m, l, all);
 	}
@@ -803,11 +818,19 @@ static AttendPlan plan_attend(const xnor_b200_kv4_cache & c, const xnor_b200_kv4
 	a.tiles = (int)(tiles < INT_MAX ? tiles : INT_MAX);
 	long long most = (long long)r.max_pages * c.page;                          // positions that a tile may see
 	if (window > 0 && most > (long long)window + r.tokens) { most = (long long)window + r.tokens; }
-	const int nb = c.dim / 32, on_sm = a.nt == 2 ? (nb <= 2 ? 3 : 2) : nb <= 2 ? 5 : nb <= 5 ? 4 : nb <= 7 ? 3 : 2;       // CTAs (registers, shared memory)
-	const long long steps = (most + 15) / 16, resident = (long long)sm_count() * on_sm;
-	long long splits = resident / base, room = steps / (4 * FA_WARPS);
-	if (splits > room) { splits = room; }
-	if (splits < 1) { splits = 1; }
+	const long long steps = (most + 15) / 16, sms = sm_count();
+	// A CTA costs about 2 us of an SM's time before and after its steps, and hides latency for the others: up to two on an SM as long as
+	// each of their warps has a pair of steps, more where the steps are many (8 heads of 128 channels by 64, one sequence, us at 2 / 3 / 4
+	// CTAs on an SM: 16384 positions 13.5 / - / 16.6, 65536 25.6 / - / 27.9, 131072 42.7 / 42.1 / 43.5, 262144 74.7 / - / 70.9).
+	const int on_sm = attend_on_sm(c.dim / 32, a.nt);
+	long long splits = 1;
+	for (int k = 1; k <= on_sm; ++k)
+	{
+		const long long s = k * sms / base, least = k <= 2 ? 2 * FA_WARPS : k == 3 ? 32 : 60;
+		if (s > splits && (k <= 2 || s * least <= steps)) { splits = s; }
+		if (k <= 2 && splits * least > steps) { splits = steps / least > 1 ? steps / least : 1; }
+	}
+	if (splits > FJ_SPLITS) { splits = FJ_SPLITS; }
 	a.cluster = splits <= 8;
 #ifdef FOUR_SWEEP
 	if (g_splits) { splits = g_splits; a.cluster = g_cluster != 0; }
@@ -839,7 +862,13 @@ static int launch_attend(const AttendParams & p, const AttendPlan & plan, cudaSt
 	if (e != cudaSuccess) { return cuda_fail(e); }
 	if (!plan.cluster)
 	{
-		four_attend_join_kernel<T><<<dim3((unsigned)(p.r.tokens * p.share), (unsigned)p.c.kv_heads, (unsigned)p.r.batch), FA_THREADS, 0, stream>>>(p, NT * 8);
+		cfg.gridDim = dim3((unsigned)(p.r.tokens * p.share), (unsigned)p.c.kv_heads, (unsigned)p.r.batch);
+		cfg.blockDim = dim3(FJ_THREADS, 1, 1);
+		cfg.dynamicSmemBytes = 0;
+		attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+		attr[0].val.programmaticStreamSerializationAllowed = 1;
+		const cudaError_t j = cudaLaunchKernelEx(&cfg, four_attend_join_kernel<T>, p, NT * 8);
+		if (j != cudaSuccess) { return cuda_fail(j); }
 	}
 	return check_launch();
 }

@@ -38,6 +38,20 @@ inline size_t four_size(int t) { return t == XNOR_B200_F32 ? 4 : 2; }
 
 #ifdef __CUDACC__
 
+// The smaller and the larger value; NaN where there is one.
+__device__ __forceinline__ float min_nan(float a, float b)
+{
+	float r;
+	asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+	return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+	float r;
+	asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+	return r;
+}
+
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }

@@ -71,7 +71,7 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[W], const void * p)
 }
 
 template <class T, int NT, int MT, int WARPS, int GROUP, int XB>
-__global__ void __launch_bounds__(32 * WARPS)
+__global__ void __launch_bounds__(32 * WARPS, 16 / WARPS)
 four_product_kernel(const ProductParams p)
 {
 	using S = ProductShape<T, NT, MT, WARPS, GROUP, XB>;

@@ -17,19 +17,6 @@ namespace xnor
 
 constexpr int FR_THREADS = 128;
 
-__device__ __forceinline__ float min_nan(float a, float b)
-{
-	float r;
-	asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-	return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b)
-{
-	float r;
-	asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-	return r;
-}
-
 __device__ __forceinline__ float reciprocal(float v)
 {
 	float r;
