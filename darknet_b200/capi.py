@@ -29,7 +29,7 @@ EXPORTS = (
     "xnor_b200_float_conv_map_prepare", "xnor_b200_float_conv_map", "xnor_b200_float_conv_map_yolo", "xnor_b200_float_conv_1x1_tc", "xnor_b200_yolo_activate", "xnor_b200_region_activate", "xnor_b200_conv_forward_io", "xnor_b200_conv_takes_masks", "xnor_b200_tap_major_weights",
     "xnor_b200_yolo_detections", "xnor_b200_nms_sort", "xnor_b200_detection_rows", "xnor_b200_detect", "xnor_b200_rows_to_host",
     "xnor_b200_avgpool", "xnor_b200_softmax", "xnor_b200_run_ops", "xnor_b200_float_conv3_words", "xnor_b200_float_conv_tc", "xnor_b200_float_conv_tc_launches", "xnor_b200_float_conv_tc_prepare", "xnor_b200_float_conv_tc_weights_bytes", "xnor_b200_conv_words", "xnor_b200_conv_words_plan", "xnor_b200_conv_words_weights", "xnor_b200_conv_words_weights_bytes", "xnor_b200_sign_words", "xnor_b200_grid_block_words", "xnor_b200_grid_front",
-    "xnor_b200_w4_code_bytes", "xnor_b200_w4_scale_bytes", "xnor_b200_w4_quantize", "xnor_b200_w4_forward",
+    "xnor_b200_w4_code_bytes", "xnor_b200_w4_scale_bytes", "xnor_b200_w4_quantize", "xnor_b200_w4_scratch_bytes", "xnor_b200_w4_forward",
     "xnor_b200_kv4_append", "xnor_b200_kv4_read", "xnor_b200_kv4_attend_scratch_bytes", "xnor_b200_kv4_attend",
     "xnor_b200_measure_popc_peak", "xnor_b200_measure_bmma_peak", "xnor_b200_measure_umma_i8_peak", "xnor_b200_measure_umma_mxf4_peak",
 )
@@ -233,7 +233,9 @@ def lib() -> C.CDLL:
     L.xnor_b200_w4_scale_bytes.restype = sz
     L.xnor_b200_w4_scale_bytes.argtypes = [wp]
     L.xnor_b200_w4_quantize.argtypes = [wp, vp, ci, ll, vp, vp, vp]
-    L.xnor_b200_w4_forward.argtypes = [wp, vp, ci, ci, ll, vp, vp, vp, vp, ll, vp]
+    L.xnor_b200_w4_scratch_bytes.restype = sz
+    L.xnor_b200_w4_scratch_bytes.argtypes = [wp, ci, ci]
+    L.xnor_b200_w4_forward.argtypes = [wp, vp, ci, ci, ll, vp, vp, vp, vp, ll, vp, sz, vp]
     L.xnor_b200_kv4_append.argtypes = [kp, rp, tp, tp, vp]
     L.xnor_b200_kv4_read.argtypes = [kp, rp, tp, tp, vp]
     L.xnor_b200_kv4_attend_scratch_bytes.restype = sz

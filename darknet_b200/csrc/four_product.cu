@@ -10,6 +10,8 @@
 // for nobody.  The slices of the same filters are a cluster: their sums meet in shared memory, in a fixed order, so results do not vary.
 #include <cooperative_groups.h>
 
+#include <climits>
+
 #include "four_common.cuh"
 
 namespace xnor
@@ -33,9 +35,11 @@ struct ProductParams
 	int row_bytes, groups;        // of one filter
 	int slice;                    // blocks of 256 of one CTA of a cluster
 	int steps;                    // of a warp's ring
+	const unsigned char * ready;  // x as the kernel holds it in shared memory, made beforehand: [tile of rows][block of 256]
 };
 
-// NT: tiles of eight rows.  MT: tiles of 16 filters of a warp.  XB: blocks of x converted at a time.
+// NT: tiles of eight rows.  MT: tiles of 16 filters of a warp.  XB: blocks of x converted at a time.  READY: x was converted by a kernel
+// of its own (four_x_kernel).
 template <class T, int NT, int MT, int WARPS, int GROUP, int XB>
 struct ProductShape
 {
@@ -70,7 +74,64 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[W], const void * p)
 	else { w[0] = *(const uint32_t *)p; }
 }
 
-template <class T, int NT, int MT, int WARPS, int GROUP, int XB>
+// A row's block of 256 to its place in a buffer of x (a warp, a lane eight neighbours): fp16 parts, the power of two, the groups' sums.
+template <class T, int GROUP, int ROWS>
+__device__ __forceinline__ void convert_row(const Eight<T> & raw, unsigned char * buffer, int xb, int x_rows, int row, unsigned char * numbers, int blocks, int lane)
+{
+	using How = Codes<T>;
+	constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, W = GROUP / 32, GROUPS = FP_K / GROUP;
+	float * inverses = (float *)numbers, * sums = inverses + blocks * ROWS;
+	float v[8];
+	eight_f32(raw, v);
+	float most = 0.0f, part = 0.0f;
+	#pragma unroll
+	for (int e = 0; e < 8; ++e)
+	{
+		most = max_nan(most, fabsf(v[e]));
+		part += v[e];
+	}
+	const uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
+	#pragma unroll
+	for (int m = 1; m < GROUP / 8; m <<= 1) { part += __shfl_xor_sync(0xffffffffu, part, m); }
+	if (lane % (GROUP / 8) == 0) { sums[(xb * GROUPS + lane / (GROUP / 8)) * ROWS + row] = part; }
+	float factor, inverse;
+	fit_f16(largest, factor, inverse);
+	if (lane == 0) { inverses[xb * ROWS + row] = inverse * How::UNIT; }
+	// (what is not finite makes its own column of the products NaN, and the inverse does so anyway)
+	float high[8], rest[8];
+	const float odd_factor = factor * How::ODD;
+	#pragma unroll
+	for (int e = 0; e < 8; ++e)
+	{
+		high[e] = v[e] * (e & 1 ? odd_factor : factor);
+		if (PARTS == 2) { split_f16(high[e], high[e], rest[e]); }
+	}
+	unsigned char * at = buffer + (xb * PARTS * x_rows + row) * FP_X_BYTES + (lane / (4 * W) * (4 * W) + lane % W * 4 + lane / W % 4) * 16;
+	*reinterpret_cast<uint4 *>(at) = make_uint4(pair_f16(high[0], high[4]), pair_f16(high[2], high[6]), pair_f16(high[1], high[5]), pair_f16(high[3], high[7]));
+	if (PARTS == 2)
+	{
+		*reinterpret_cast<uint4 *>(at + x_rows * FP_X_BYTES) = make_uint4(pair_f16(rest[0], rest[4]), pair_f16(rest[2], rest[6]), pair_f16(rest[1], rest[5]), pair_f16(rest[3], rest[7]));
+	}
+}
+
+// x converted once for all CTAs of a large product: a block of 256 neighbours of a tile of rows a CTA, as buffer_bytes() lays it out.
+template <class T, int NT, int GROUP>
+__global__ void __launch_bounds__(256)
+four_x_kernel(const ProductParams p, unsigned char * ready)
+{
+	using S = ProductShape<T, NT, 2, 8, GROUP, 1>;
+	const int row0 = blockIdx.y * S::ROWS, rows = min(S::ROWS, p.rows - row0), x_rows = min(S::ROWS, p.rows), lane = threadIdx.x % 32;
+	unsigned char * buffer = ready + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * S::buffer_bytes(x_rows);
+	pdl_trigger();                                            // the product may be launched; it waits for this kernel's end
+	for (int row = threadIdx.x / 32; row < rows; row += 8)
+	{
+		const int k0 = blockIdx.x * FP_K + lane * 8;
+		convert_row<T, GROUP, S::ROWS>(load8((const T *)p.x + (k0 < p.k ? (row0 + row) * p.ldx + k0 : 0), p.k - k0, p.wide != 0), buffer, 0, x_rows, row,
+				buffer + S::x_bytes(x_rows), 1, lane);
+	}
+}
+
+template <class T, int NT, int MT, int WARPS, int GROUP, int XB, bool READY>
 __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS)
 four_product_kernel(const ProductParams p)
 {
@@ -143,70 +204,58 @@ four_product_kernel(const ProductParams p)
 	};
 	auto convert_x = [&](int chunk, unsigned char * buffer)
 	{
-		float * inverses = (float *)(buffer + S::x_bytes(x_rows)), * sums = inverses + XB * ROWS;
 		#pragma unroll
 		for (int i = 0; i < S::TASKS; ++i)
 		{
 			const int task = i * WARPS + warp, xb = task / rows, row = task - xb * rows;
 			if (xb >= XB || chunk + xb >= last) { continue; }
-			float v[8];
-			eight_f32(raw[i], v);
-			uint32_t largest = 0;
-			float part = 0.0f;
-			#pragma unroll
-			for (int e = 0; e < 8; ++e)
-			{
-				largest = max(largest, __float_as_uint(fabsf(v[e])));
-				part += v[e];
-			}
-			largest = __reduce_max_sync(0xffffffffu, largest);
-			#pragma unroll
-			for (int m = 1; m < GROUP / 8; m <<= 1) { part += __shfl_xor_sync(0xffffffffu, part, m); }
-			if (lane % (GROUP / 8) == 0) { sums[(xb * GROUPS + lane / (GROUP / 8)) * ROWS + row] = part; }
-			float factor, inverse;
-			fit_f16(largest, factor, inverse);
-			if (lane == 0) { inverses[xb * ROWS + row] = inverse * How::UNIT; }
-			float high[8], rest[8];
-			const float odd_factor = factor * How::ODD;
-			#pragma unroll
-			for (int e = 0; e < 8; ++e)
-			{
-				high[e] = factor == 0.0f ? 0.0f : v[e] * (e & 1 ? odd_factor : factor);
-				if (PARTS == 2) { split_f16(high[e], high[e], rest[e]); }
-			}
-			unsigned char * at = buffer + (xb * PARTS * x_rows + row) * FP_X_BYTES + (lane / (4 * W) * (4 * W) + lane % W * 4 + lane / W % 4) * 16;
-			*reinterpret_cast<uint4 *>(at) = make_uint4(pair_f16(high[0], high[4]), pair_f16(high[2], high[6]), pair_f16(high[1], high[5]), pair_f16(high[3], high[7]));
-			if (PARTS == 2)
-			{
-				*reinterpret_cast<uint4 *>(at + x_rows * FP_X_BYTES) = make_uint4(pair_f16(rest[0], rest[4]), pair_f16(rest[2], rest[6]), pair_f16(rest[1], rest[5]), pair_f16(rest[3], rest[7]));
-			}
+			convert_row<T, GROUP, ROWS>(raw[i], buffer, xb, x_rows, row, buffer + S::x_bytes(x_rows), XB, lane);
 		}
 	};
 
-	load_x(first);
+	// x that was made beforehand: copied with the codes of its block
+	auto copy_x = [&](int block, unsigned char * buffer)
+	{
+		const unsigned char * from = p.ready + ((size_t)blockIdx.y * ((p.k + FP_K - 1) / FP_K) + block) * S::buffer_bytes(x_rows);
+		for (int i = threadIdx.x * 16; i < S::buffer_bytes(x_rows); i += S::THREADS * 16) { copy16(four_smem(buffer) + i, from + i, true); }
+	};
+
+	if (!READY) { load_x(first); }
 	for (int i = 0; i < p.steps - 1; ++i) { request(); }
+	if (READY)
+	{
+		pdl_wait();
+		if (first < last) { copy_x(first, buffers); }
+		copies_close();
+	}
 	uint32_t * zeros = (uint32_t *)(buffers + 2 * S::buffer_bytes(x_rows));
 	for (int i = threadIdx.x; i < FP_X_BYTES / 4; i += S::THREADS) { zeros[i] = 0; }
-	convert_x(first, buffers);
+	if (!READY) { convert_x(first, buffers); }
 
 	float sum[MT][NT][4] = {};
 	int stage = 0, which = 0;
 	for (int chunk = first; chunk < last; chunk += XB)
 	{
+		if (READY) { copies_wait<0>(); }
 		__syncthreads();                                      // this chunk's x is there, and nobody reads the buffer of the one before
 		const unsigned char * buffer = buffers + which * S::buffer_bytes(x_rows);
 		which ^= 1;
-		if (chunk + XB < last) { load_x(chunk + XB); }
+		if (chunk + XB < last)
+		{
+			if (READY) { copy_x(chunk + 1, buffers + which * S::buffer_bytes(x_rows)); }
+			else { load_x(chunk + XB); }
+		}
 		const float * inverses = (const float *)(buffer + S::x_bytes(x_rows)), * sums = inverses + XB * ROWS;
 		#pragma unroll 1
 		for (int xb = 0; xb < XB && chunk + xb < last; ++xb)
 		{
 			request();
 			// of the copies asked for so far (a step each), all but the last steps - 1 have to be there
-			if (p.steps == 6) { copies_wait<5>(); }
-			else if (p.steps == 4) { copies_wait<3>(); }
-			else if (p.steps == 3) { copies_wait<2>(); }
-			else { copies_wait<1>(); }
+			if (!READY)
+			{
+				if (p.steps == 3) { copies_wait<2>(); }
+				else { copies_wait<1>(); }
+			}
 			__syncwarp();
 			const unsigned char * step = ring + stage * S::STEP_BYTES;
 			stage = stage + 1 == p.steps ? 0 : stage + 1;
@@ -300,7 +349,7 @@ four_product_kernel(const ProductParams p)
 			}
 			__syncwarp();
 		}
-		if (chunk + XB < last) { convert_x(chunk + XB, buffers + which * S::buffer_bytes(x_rows)); }
+		if (!READY && chunk + XB < last) { convert_x(chunk + XB, buffers + which * S::buffer_bytes(x_rows)); }
 	}
 
 	// Columns of rows that are not there hold what shared memory held: never stored.
@@ -337,85 +386,157 @@ four_product_kernel(const ProductParams p)
 static int g_ranks = 0, g_steps = 0, g_shape = 0;
 #endif
 
-template <class T, int NT, int MT, int WARPS, int GROUP>
-static int launch_product(ProductParams & p, cudaStream_t stream)
+// Large products of many rows: every CTA would convert all of x again, a fifth of its work (16384 x 16384 by 16 rows of bf16: 55 us, 46 with
+// a kernel for that; fp32 rows, whose parts are twice as much to copy, gain nothing: 8192 x 8192 by 12 rows 38 against 26).
+static bool wants_ready(int n, int k, int dtype, int rows)
 {
-	constexpr int XB = NT == 1 ? 2 : 1;
+#ifdef FOUR_SWEEP
+	if (g_shape) { return g_shape >= 5; }
+#endif
+	return rows > 8 && dtype != XNOR_B200_F32 && (long long)n * k >= (1LL << 27);
+}
+
+template <class T, int NT, int MT, int WARPS, int GROUP, bool READY>
+static int launch_product(ProductParams & p, void * scratch, cudaStream_t stream)
+{
+	constexpr int XB = NT == 1 && !READY ? 2 : 1;
 	using S = ProductShape<T, NT, MT, WARPS, GROUP, XB>;
 	const int tiles = (p.n + S::FILTERS - 1) / S::FILTERS, blocks = (p.k + FP_K - 1) / FP_K;
-	const auto kernel = four_product_kernel<T, NT, MT, WARPS, GROUP, XB>;
-	int ranks = 1;
-	while (ranks < 8 && tiles * ranks < 2 * sm_count() && blocks >= 2 * ranks) { ranks *= 2; }
-	p.steps = 4;
+	const auto kernel = four_product_kernel<T, NT, MT, WARPS, GROUP, XB, READY>;
+	// Slices: as few blocks as possible one after the other, with two CTAs on an SM at a time (and shared memory for two: two steps of
+	// 256 filters, three of 128).  Clusters of 5 and 7 find fewer places.
+	int ranks = 1, best = INT_MAX;
+	for (const int r : {1, 2, 3, 4, 6, 8})
+	{
+		const long long waves = ((long long)tiles * r + 2 * sm_count() - 1) / (2 * sm_count());
+		const long long cost = waves * ((blocks + r - 1) / r);
+		if (r <= blocks && cost < best)
+		{
+			best = (int)cost;
+			ranks = r;
+		}
+	}
+	p.steps = MT == 2 ? 2 : 3;
 #ifdef FOUR_SWEEP
 	if (g_ranks) { ranks = g_ranks; }
-	if (g_steps) { p.steps = g_steps; }
+	if (g_steps && !READY) { p.steps = g_steps; }
 #endif
 	p.slice = (blocks + ranks - 1) / ranks;
-	if (p.slice < p.steps) { p.steps = p.slice < 3 ? 2 : 3; }
+	if (p.slice < p.steps) { p.steps = 2; }
 	const size_t smem = S::smem(p.rows < S::ROWS ? p.rows : S::ROWS, p.steps);
 	const int rc = ensure_dynamic_smem((const void *)kernel, smem);
 	if (rc != XNOR_B200_OK) { return rc; }
+	const unsigned row_tiles = (unsigned)((p.rows + NT * 8 - 1) / (NT * 8));
+	if (READY)
+	{
+		p.ready = (const unsigned char *)scratch;
+		four_x_kernel<T, NT, GROUP><<<dim3((unsigned)blocks, row_tiles), 256, 0, stream>>>(p, (unsigned char *)scratch);
+		const int x_rc = check_launch();
+		if (x_rc != XNOR_B200_OK) { return x_rc; }
+	}
 	cudaLaunchConfig_t cfg = {};
-	cfg.gridDim = dim3((unsigned)(tiles * ranks), (unsigned)((p.rows + NT * 8 - 1) / (NT * 8)), 1);
+	cfg.gridDim = dim3((unsigned)(tiles * ranks), row_tiles, 1);
 	cfg.blockDim = dim3(S::THREADS, 1, 1);
 	cfg.dynamicSmemBytes = smem;
 	cfg.stream = stream;
-	cudaLaunchAttribute attr[1];
+	cudaLaunchAttribute attr[2];
 	attr[0].id = cudaLaunchAttributeClusterDimension;
 	attr[0].val.clusterDim.x = (unsigned)ranks;
 	attr[0].val.clusterDim.y = 1;
 	attr[0].val.clusterDim.z = 1;
+	attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	attr[1].val.programmaticStreamSerializationAllowed = 1;
 	cfg.attrs = attr;
-	cfg.numAttrs = 1;
+	cfg.numAttrs = READY ? 2 : 1;
 	const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
 	return e == cudaSuccess ? check_launch() : cuda_fail(e);
 }
 
 template <class T, int NT, int GROUP>
-static int launch_product_shape(ProductParams & p, cudaStream_t stream)
+static int launch_product_shape(ProductParams & p, int dtype, void * scratch, cudaStream_t stream)
 {
 #ifdef FOUR_SWEEP
-	if (g_shape == 1) { return launch_product<T, NT, 1, 4, GROUP>(p, stream); }
-	if (g_shape == 2) { return launch_product<T, NT, 2, 4, GROUP>(p, stream); }
-	if (g_shape == 3) { return launch_product<T, NT, 2, 8, GROUP>(p, stream); }
-	if (g_shape == 4) { return launch_product<T, NT, 1, 8, GROUP>(p, stream); }
+	if (g_shape == 3) { return launch_product<T, NT, 2, 8, GROUP, false>(p, scratch, stream); }
+	if (g_shape == 4) { return launch_product<T, NT, 1, 8, GROUP, false>(p, scratch, stream); }
 #endif
-	return launch_product<T, NT, 1, 4, GROUP>(p, stream);
+	if constexpr (sizeof(T) == 2)
+	{
+		if constexpr (NT == 2)
+		{
+			if (wants_ready(p.n, p.k, dtype, p.rows)) { return launch_product<T, NT, 2, 8, GROUP, true>(p, scratch, stream); }
+		}
+		// 256 filters of a CTA share its x and its loads of x, 128 fill the SMs where there are few, and are all that the registers of fp32
+		// rows and the sums of small groups leave room for (us with 256 / 128: one row 16384 x 16384 33 / 41, 8192 x 8192 12.2 / 13.4, 4096 x
+		// 4096 6.9 / 5.4; groups of 32, 4096 x 16384 by 8 rows 17.4 / 16.9; fp32, 8192 x 8192 by 12 rows 28 / 26)
+		const int blocks = (p.k + FP_K - 1) / FP_K;
+		if constexpr (GROUP > 32)
+		{
+			if ((long long)((p.n + 255) / 256) * (blocks < 8 ? blocks : 8) >= 256) { return launch_product<T, NT, 2, 8, GROUP, false>(p, scratch, stream); }
+		}
+	}
+	return launch_product<T, NT, 1, 8, GROUP, false>(p, scratch, stream);
 }
 
 template <class T, int NT>
-static int launch_product_group(ProductParams & p, int group, cudaStream_t stream)
+static int launch_product_group(ProductParams & p, int dtype, int group, void * scratch, cudaStream_t stream)
 {
 	switch (group)
 	{
-		case 32: return launch_product_shape<T, NT, 32>(p, stream);
-		case 64: return launch_product_shape<T, NT, 64>(p, stream);
-		default: return launch_product_shape<T, NT, 128>(p, stream);
+		case 32: return launch_product_shape<T, NT, 32>(p, dtype, scratch, stream);
+		case 64: return launch_product_shape<T, NT, 64>(p, dtype, scratch, stream);
+		default: return launch_product_shape<T, NT, 128>(p, dtype, scratch, stream);
 	}
 }
 
 template <class T>
-static int launch_product_rows(ProductParams & p, int group, cudaStream_t stream)
+static int launch_product_rows(ProductParams & p, int dtype, int group, void * scratch, cudaStream_t stream)
 {
-	if (p.rows <= 8) { return launch_product_group<T, 1>(p, group, stream); }
-	return launch_product_group<T, 2>(p, group, stream);
+	if (p.rows <= 8) { return launch_product_group<T, 1>(p, dtype, group, scratch, stream); }
+	return launch_product_group<T, 2>(p, dtype, group, scratch, stream);
+}
+
+// Bytes of one block of x of a tile of 16 rows as the kernel holds it.
+static size_t ready_bytes(int group, int rows)
+{
+	const int x_rows = rows < 16 ? rows : 16;
+	return (size_t)x_rows * FP_X_BYTES + 16 * 4 * (1 + FP_K / group);
 }
 
 }  // namespace xnor
 
 using namespace xnor;
 
+static int check_product(const xnor_b200_w4_desc * d, int dtype, int rows)
+{
+	if (d == nullptr) { return XNOR_B200_ERR_NULL; }
+	if (d->n <= 0 || d->k <= 0 || !four_group_ok(d->group) || (d->activation != XNOR_B200_LINEAR && d->activation != XNOR_B200_LEAKY)
+			|| !four_dtype_ok(dtype) || rows <= 0) { return XNOR_B200_ERR_INVALID; }
+	if (d->k > XNOR_B200_W4_MAX_K || rows > XNOR_B200_W4_MAX_ROWS || d->n > XNOR_B200_W4_MAX_N) { return XNOR_B200_ERR_TOO_LARGE; }
+	return XNOR_B200_OK;
+}
+
+extern "C" size_t xnor_b200_w4_scratch_bytes(const xnor_b200_w4_desc * d, int dtype, int rows)
+{
+	if (check_product(d, dtype, rows) != XNOR_B200_OK || !wants_ready(d->n, d->k, dtype, rows)) { return 0; }
+	return (size_t)((rows + 15) / 16) * ((d->k + FP_K - 1) / FP_K) * ready_bytes(d->group, rows);
+}
+
 extern "C" int xnor_b200_w4_forward(const xnor_b200_w4_desc * d, const void * x, int dtype, int rows, long long ldx, const uint8_t * codes,
-		const void * scales, const float * biases, void * output, long long ldo, void * stream)
+		const void * scales, const float * biases, void * output, long long ldo, void * scratch, size_t scratch_bytes, void * stream)
 {
 	if (d == nullptr || x == nullptr || codes == nullptr || scales == nullptr || output == nullptr) { return XNOR_B200_ERR_NULL; }
-	if (d->n <= 0 || d->k <= 0 || !four_group_ok(d->group) || (d->activation != XNOR_B200_LINEAR && d->activation != XNOR_B200_LEAKY)
-			|| !four_dtype_ok(dtype) || rows <= 0 || ldx < 0 || ldo < d->n) { return XNOR_B200_ERR_INVALID; }
-	if (d->k > XNOR_B200_W4_MAX_K || rows > XNOR_B200_W4_MAX_ROWS || d->n > XNOR_B200_W4_MAX_N) { return XNOR_B200_ERR_TOO_LARGE; }
+	const int rc = check_product(d, dtype, rows);
+	if (rc != XNOR_B200_OK) { return rc; }
+	if (ldx < 0 || ldo < d->n) { return XNOR_B200_ERR_INVALID; }
 	const size_t size = four_size(dtype);
 	if (((uintptr_t)codes & 15) != 0 || ((uintptr_t)scales & 3) != 0 || ((uintptr_t)biases & 3) != 0 || ((uintptr_t)x & (size - 1)) != 0
 			|| ((uintptr_t)output & (size - 1)) != 0) { return XNOR_B200_ERR_ALIGNMENT; }
+	if (wants_ready(d->n, d->k, dtype, rows))
+	{
+		if (scratch == nullptr) { return XNOR_B200_ERR_NULL; }
+		if (scratch_bytes < xnor_b200_w4_scratch_bytes(d, dtype, rows)) { return XNOR_B200_ERR_SCRATCH; }
+		if (((uintptr_t)scratch & 15) != 0) { return XNOR_B200_ERR_ALIGNMENT; }
+	}
 	ProductParams p = {};
 	p.codes = codes;
 	p.scales = (const uint32_t *)scales;
@@ -434,9 +555,9 @@ extern "C" int xnor_b200_w4_forward(const xnor_b200_w4_desc * d, const void * x,
 	const cudaStream_t s = (cudaStream_t)stream;
 	switch (dtype)
 	{
-		case XNOR_B200_F32: return launch_product_rows<float>(p, d->group, s);
-		case XNOR_B200_F16: return launch_product_rows<__half>(p, d->group, s);
-		default: return launch_product_rows<__nv_bfloat16>(p, d->group, s);
+		case XNOR_B200_F32: return launch_product_rows<float>(p, dtype, d->group, scratch, s);
+		case XNOR_B200_F16: return launch_product_rows<__half>(p, dtype, d->group, scratch, s);
+		default: return launch_product_rows<__nv_bfloat16>(p, dtype, d->group, scratch, s);
 	}
 }
 

@@ -35,7 +35,7 @@ class _Calls:
 
     def __getattr__(self, name: str):
         vp, ci, ll = C.c_void_p, C.c_int, C.c_longlong
-        for entry, args in (("w4_forward", [vp, vp, ci, ci, ll, vp, vp, vp, vp, ll, vp]), ("kv4_append", [vp] * 5), ("kv4_read", [vp] * 5),
+        for entry, args in (("w4_forward", [vp, vp, ci, ci, ll, vp, vp, vp, vp, ll, vp, C.c_size_t, vp]), ("w4_scratch_bytes", [vp, ci, ci]), ("kv4_append", [vp] * 5), ("kv4_read", [vp] * 5),
                             ("kv4_attend", [vp, vp, vp, ci, C.c_float, ci, vp, vp, vp, C.c_size_t, vp]),
                             ("kv4_attend_scratch_bytes", [vp, vp, ci, ci])):
             f = capi.lib()["xnor_b200_" + entry]
@@ -136,8 +136,14 @@ def forward_connected4(m: Matrix4, x: torch.Tensor, biases: Optional[torch.Tenso
         out = x.new_empty((rows, n))
     if rows == 0:
         return out
+    nbytes, scratch = 0, None
+    if rows > 8:                                              # (fewer never need any)
+        nbytes = _calls.w4_scratch_bytes(desc, dtype, rows)
+        if nbytes:
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     rc = _calls.w4_forward(desc, x.data_ptr(), dtype, rows, x.stride(0) if rows > 1 else m.k, m.codes.data_ptr(), m.scales.data_ptr(),
-                           None if biases is None else biases.data_ptr(), out.data_ptr(), out.stride(0) if rows > 1 else n, _raw_stream(index))
+                           None if biases is None else biases.data_ptr(), out.data_ptr(), out.stride(0) if rows > 1 else n,
+                           None if scratch is None else scratch.data_ptr(), nbytes, _raw_stream(index))
     if rc:
         capi.check(rc, "xnor_b200_w4_forward")
     return out

@@ -610,9 +610,12 @@ XNOR_B200_API int xnor_b200_w4_quantize(const xnor_b200_w4_desc * desc, const vo
 /* forward_connected_layer_gpu (src-lib/connected_layer.cpp) with such weights: output[r][i] = act(sum_j x[r][j] * value[i][j] + biases[i])
  * for `rows` rows of x, ldx elements apart, to rows ldo elements apart, both of type `dtype`; biases fp32 [n] or NULL.  Sums are fp32,
  * rounded once.  A row of x that holds an infinity or a NaN gives NaN.  Made for few rows (one pass over the weights serves 16).
- * output overlaps no input. */
+ * output overlaps no input.  scratch: xnor_b200_w4_scratch_bytes() bytes (0 for all but large products of many rows: may be NULL), 16-byte
+ * aligned, of this call alone until it has run; needs no initialisation. */
+XNOR_B200_API size_t xnor_b200_w4_scratch_bytes(const xnor_b200_w4_desc * desc, int dtype, int rows);
 XNOR_B200_API int xnor_b200_w4_forward(const xnor_b200_w4_desc * desc, const void * x, int dtype, int rows, long long ldx,
-		const uint8_t * codes, const void * scales, const float * biases, void * output, long long ldo, void * stream);
+		const uint8_t * codes, const void * scales, const float * biases, void * output, long long ldo, void * scratch, size_t scratch_bytes,
+		void * stream);
 
 /* Keys and values of tokens in pages of `page` tokens (a multiple of 16): codes [pages][kv_heads][page][dim/2] bytes, scales
  * [pages][kv_heads][page][dim/group][2] fp16, all four 16-byte aligned.  dim: a multiple of 32, at most XNOR_B200_KV4_MAX_DIM, and

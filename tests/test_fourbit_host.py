@@ -43,8 +43,8 @@ def test_sizes(L):
 def test_products_refuse(L):
     d = capi.W4Desc(16, 64, 32, 0)
 
-    def forward(d=d, x=256, dtype=0, rows=1, ldx=64, codes=256, scales=256, biases=None, out=256, ldo=16):
-        return L.xnor_b200_w4_forward(None if d is None else C.byref(d), x, dtype, rows, ldx, codes, scales, biases, out, ldo, None)
+    def forward(d=d, x=256, dtype=0, rows=1, ldx=64, codes=256, scales=256, biases=None, out=256, ldo=16, scratch=None, nbytes=0):
+        return L.xnor_b200_w4_forward(None if d is None else C.byref(d), x, dtype, rows, ldx, codes, scales, biases, out, ldo, scratch, nbytes, None)
 
     for null in ("d", "x", "codes", "scales", "out"):
         assert forward(**{null: None}) == 2
@@ -55,6 +55,14 @@ def test_products_refuse(L):
         assert forward(**odd) == 5, odd
     assert forward(rows=(1 << 16) + 1) == 6
     assert forward(d=capi.W4Desc(16, (1 << 24) + 1, 32, 0)) == 6
+    # a large product of many rows converts x once, into scratch memory
+    large, small = capi.W4Desc(1 << 14, 1 << 13, 64, 0), capi.W4Desc(1 << 14, 1 << 12, 64, 0)
+    need = L.xnor_b200_w4_scratch_bytes(C.byref(large), 1, 9)
+    assert need >= 9 * (1 << 13) * 2 and L.xnor_b200_w4_scratch_bytes(C.byref(large), 2, 17) > 2 * need
+    assert L.xnor_b200_w4_scratch_bytes(C.byref(large), 1, 8) == 0 and L.xnor_b200_w4_scratch_bytes(C.byref(small), 1, 16) == 0
+    assert L.xnor_b200_w4_scratch_bytes(C.byref(large), 5, 16) == 0 and L.xnor_b200_w4_scratch_bytes(None, 1, 16) == 0
+    many = dict(d=large, dtype=1, rows=9, ldx=1 << 13, ldo=1 << 14)
+    assert forward(**many) == 2 and forward(**many, scratch=256, nbytes=need - 1) == 3 and forward(**many, scratch=264, nbytes=need) == 5
     assert L.xnor_b200_w4_quantize(C.byref(d), None, 0, 64, 256, 256, None) == 2
     assert L.xnor_b200_w4_quantize(C.byref(d), 256, 7, 64, 256, 256, None) == 1
     assert L.xnor_b200_w4_quantize(C.byref(d), 256, 0, 64, 264, 256, None) == 5

@@ -124,6 +124,25 @@ def test_product_of_a_long_row(dtype):
     check_product(m, x, F.forward_connected4(m, x))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("n, k, group, rows", [(16500, 8200, 64, 9), (8300, 16200, 128, 16), (16384, 8192, 32, 35)])
+def test_large_products_of_many_rows(dtype, n, k, group, rows):
+    """Those convert x beforehand.  What they give is compared with calls of eight rows, which do not, filter by filter: both are within
+    check_product's bound of the same value; the bound itself is looked at for some filters."""
+    m = matrix(n, k, group, rows)
+    whole = torch.randn(rows, k + 8, generator=rng(k)).to(dtype).cuda()
+    for x in (whole[:, :k], whole[:, 3:k + 3]):
+        y = F.forward_connected4(m, x)
+        assert capi.lib().xnor_b200_w4_scratch_bytes(capi.W4Desc(n, k, group, 0), 1, rows) > 0
+        picked = torch.arange(0, n, 211)
+        part = F.Matrix4(m.codes[picked.cuda()].contiguous(), m.scales[picked.cuda()].contiguous(), k, group)
+        check_product(part, x, y[:, picked.cuda()])
+        few = torch.cat([F.forward_connected4(m, x[i:i + 8]) for i in range(0, rows, 8)])
+        assert ((y.float() - few.float()).abs() <= few.float().abs() * 2 * R.HALF_STEP[dtype] + 2e-3).all()
+        for _ in range(2):
+            assert torch.equal(F.forward_connected4(m, x), y)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 def test_product_with_bias_and_leaky(dtype):
     m = matrix(100, 300, 32, 1)
