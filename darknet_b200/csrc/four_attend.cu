@@ -42,6 +42,7 @@ struct AttendParams
 	float scale_log2;             // scale * log2(e)
 	int heads, share;             // heads of queries, and how many of them a head of keys serves
 	int window, splits, tiles;    // tiles of columns
+	int room;                     // positions that a row of the table has pages for
 	int wide_q;
 };
 
@@ -57,20 +58,21 @@ struct Span
 // The token that a column asks for (one token: no division; this and its like are a good part of a short call).
 __device__ __forceinline__ int row_of(const AttendParams & p, int col) { return p.r.tokens == 1 ? 0 : col / p.share; }
 
+// The first position that a token at `at` sees.
+__device__ __forceinline__ int seen_from(int window, int at) { return window > 0 && at >= window ? at - window + 1 : 0; }
+
 __device__ __forceinline__ Span span_of(const AttendParams & p, int b, int i0, int i1)
 {
 	Span s;
-	const int count = p.r.counts != nullptr ? __ldg(p.r.counts + b) : p.r.tokens;
+	const int count = p.r.counts != nullptr ? max(__ldg(p.r.counts + b), 0) : p.r.tokens;
 	s.count = min(count, p.r.tokens);
 	const int length = max(__ldg(p.r.lengths + b), 0);
-	const long long at = (long long)length - count, room = (long long)p.r.max_pages * p.c.page;
-	s.at = (int)max(at, -0x40000000LL);                   // (rows that far in front of a sequence see nothing either way)
-	s.end = (int)min((long long)length, room);
+	s.at = length - count;
+	s.end = min(length, p.room);
 	i1 = min(i1, s.count - 1);
-	const long long to = i1 < i0 ? 0 : min((long long)s.end, at + i1 + 1);
-	const long long from = p.window > 0 ? max(0LL, at + i0 + 1 - p.window) : 0;
-	s.first = (int)(from / 16);
-	s.last = to > from ? (int)((to + 15) / 16) : s.first;
+	const int to = i1 < i0 ? 0 : min(s.end, s.at + i1 + 1), from = i1 < i0 ? 0 : seen_from(p.window, s.at + i0);
+	s.first = from / 16;
+	s.last = to > from ? (to - 1) / 16 + 1 : s.first;
 	return s;
 }
 
@@ -93,11 +95,10 @@ __device__ __forceinline__ float weight_of(float m, float top) { return m == -IN
 
 __device__ __forceinline__ void add_weighted(float4 & v, float by, const float4 & u)
 {
-	// (what counts for nothing may be anything)
-	v.x += by == 0.0f ? 0.0f : by * u.x;
-	v.y += by == 0.0f ? 0.0f : by * u.y;
-	v.z += by == 0.0f ? 0.0f : by * u.z;
-	v.w += by == 0.0f ? 0.0f : by * u.w;
+	v.x += by * u.x;
+	v.y += by * u.y;
+	v.z += by * u.z;
+	v.w += by * u.w;
 }
 
 // Four channels of a row, from its sums at maximum m and their total l.
@@ -106,10 +107,11 @@ __device__ __forceinline__ void write_out(const AttendParams & p, int b, int row
 {
 	none |= m == -INFINITY;
 	T * to = (T *)p.out.data + b * p.out.stride_sequence + row * p.out.stride_token + head * p.out.stride_head + d;
-	to[0] = from_f32<T>(none ? 0.0f : v.x / l);
-	to[1] = from_f32<T>(none ? 0.0f : v.y / l);
-	to[2] = from_f32<T>(none ? 0.0f : v.z / l);
-	to[3] = from_f32<T>(none ? 0.0f : v.w / l);
+	const float by = 1.0f / l;
+	to[0] = from_f32<T>(none ? 0.0f : v.x * by);
+	to[1] = from_f32<T>(none ? 0.0f : v.y * by);
+	to[2] = from_f32<T>(none ? 0.0f : v.z * by);
+	to[3] = from_f32<T>(none ? 0.0f : v.w * by);
 	if (p.lse != nullptr && d == 0)
 	{
 		p.lse[((size_t)b * p.r.tokens + row) * p.heads + head] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
@@ -130,7 +132,7 @@ template <> struct Parts<float> { static constexpr int Q = 2, P = 2; };
 // A stage holds 32 positions: rows of keys' codes, rows of values' codes, scales.  A lane reads GB words of a row of a group; the pitches
 // put rows that are read at a time into different banks.
 // CTAs that an SM holds: 128 registers a thread for most shapes, shared memory for the widest.
-__host__ __device__ constexpr int attend_on_sm(int nb, int nt) { return nt == 2 ? (nb <= 2 ? 3 : 2) : nb <= 5 ? 4 : nb <= 7 ? 3 : 2; }
+__host__ __device__ constexpr int attend_on_sm(int nb, int nt) { return nt >= 2 ? (nb <= 2 && nt == 2 ? 3 : 2) : nb <= 5 ? 4 : nb <= 7 ? 3 : 2; }
 
 template <int NB, int GB, int NT, int QP>
 struct AttendShape
@@ -215,7 +217,7 @@ four_attend_kernel(const AttendParams p)
 	const int col0 = tile * COLS, cols = min(COLS, p.r.tokens * p.share - col0);
 	const Span span = span_of(p, b, row_of(p, col0), row_of(p, col0 + cols - 1));
 	const int per = steps_of_split(span, p.splits);
-	const int begin = (int)min((long long)span.last, span.first + (long long)split * per), end = min(span.last, begin + per);
+	const int begin = min(span.last, span.first + split * per), end = min(span.last, begin + per);
 
 	// ---- the ring.  A step is 16 positions of one page; a warp takes two at a time.
 	const int page_steps = p.c.page / 16;
@@ -320,7 +322,7 @@ four_attend_kernel(const AttendParams p)
 		{
 			s_qf[c] = inverse * (How::UNIT * p.scale_log2);
 			s_to[c] = there ? min(span.end, span.at + i + 1) : 0;
-			s_from[c] = there && p.window > 0 ? max(0, span.at + i + 1 - p.window) : 0;
+			s_from[c] = there ? seen_from(p.window, span.at + i) : 0;
 		}
 		if (side < NB * 4)
 		{
@@ -343,7 +345,7 @@ four_attend_kernel(const AttendParams p)
 	__syncthreads();
 	// Positions that every column of a token sees: no step inside them asks again
 	const int row_first = row_of(p, col0), row_last = min(row_of(p, col0 + cols - 1), span.count - 1);
-	const int all_to = min(span.end, span.at + row_first + 1), all_from = p.window > 0 ? max(0, span.at + row_last + 1 - p.window) : 0;
+	const int all_to = min(span.end, span.at + row_first + 1), all_from = seen_from(p.window, span.at + row_last);
 
 	float o[GROUPS][GB][2][NT][4] = {};                       // [group][word][even, odd channels][tile][channel of g: columns 2t, 2t+1; of g + 8]
 	float lows[GROUPS][NT][2] = {};                           // sum(p * low_v) of this lane's positions
@@ -691,7 +693,11 @@ four_attend_kernel(const AttendParams p)
 		if (threadIdx.x >= FA_THREADS / quads * quads) { break; }
 		float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 		#pragma unroll
-		for (int w = 0; w < FA_WARPS; ++w) { add_weighted(v, s_by[w * COLS + c], *(const float4 *)(first_u + w * WARP_FLOATS + c * S::U_PITCH + q * 4)); }
+		for (int w = 0; w < FA_WARPS; ++w)
+		{
+			// (what counts for nothing has seen nothing: its sums are 0)
+			add_weighted(v, s_by[w * COLS + c], *(const float4 *)(first_u + w * WARP_FLOATS + c * S::U_PITCH + q * 4));
+		}
 		if (joined) { *(float4 *)(first_u + c * S::U_PITCH + q * 4) = v; }
 		else if (begin < end) { *(float4 *)(partial + c * DIM + q * 4) = v; }
 	}
@@ -813,7 +819,16 @@ static AttendPlan plan_attend(const xnor_b200_kv4_cache & c, const xnor_b200_kv4
 {
 	AttendPlan a;
 	const long long columns = (long long)r.tokens * (heads / c.kv_heads);
-	a.nt = columns > 8 && c.dim <= 128 ? 2 : 1;
+	// tiles of columns: every tile goes over the cache and makes operands of its codes (which is some two thirds of a tile of eight)
+	a.nt = 1;
+	if (c.dim <= 128)
+	{
+		for (int nt = 2; nt <= 3; ++nt)
+		{
+			const long long cost = (columns + nt * 8 - 1) / (nt * 8) * (2 + nt), least = (columns + a.nt * 8 - 1) / (a.nt * 8) * (2 + a.nt);
+			if (cost < least) { a.nt = nt; }
+		}
+	}
 	const long long tiles = (columns + a.nt * 8 - 1) / (a.nt * 8), base = tiles * c.kv_heads * r.batch;
 	a.tiles = (int)(tiles < INT_MAX ? tiles : INT_MAX);
 	long long most = (long long)r.max_pages * c.page;                          // positions that a tile may see
@@ -879,6 +894,7 @@ static int launch_attend_columns(const AttendParams & p, const AttendPlan & plan
 	if constexpr (NB <= 4)
 	{
 		if (plan.nt == 2) { return launch_attend<T, NB, GB, 2>(p, plan, stream); }
+		if (plan.nt == 3) { return launch_attend<T, NB, GB, 3>(p, plan, stream); }
 	}
 	return launch_attend<T, NB, GB, 1>(p, plan, stream);
 }
@@ -954,6 +970,8 @@ extern "C" int xnor_b200_kv4_attend(const xnor_b200_kv4_cache * cache, const xno
 	p.heads = heads;
 	p.share = heads / cache->kv_heads;
 	p.window = window;
+	const long long room = (long long)rows->max_pages * cache->page;
+	p.room = room < INT_MAX ? (int)room : INT_MAX;
 	p.splits = plan.splits;
 	p.tiles = plan.tiles;
 	p.wide_q = ((uintptr_t)q->data & 15) == 0 && q->stride_sequence * (long long)size % 16 == 0 && q->stride_token * (long long)size % 16 == 0
