@@ -6,10 +6,11 @@
 // quotient up in fp32 on the way gives the same scale as one rounding of the exact quotient: each step's result is the smallest fp32 value
 // not below, and an fp16 value (times 15) is one of those.  NaN counts as 0, and what fp16 cannot hold as its largest value.
 //
-// A thread owns eight neighbours, one word of codes; the 4, 8 or 16 threads of a group find its minimum and maximum by shuffles.  Bound by
-// what a thread has to do (some 120 instructions for 16 bytes in) rather than by memory, so: the quotient is a product with 1/scale, whose
-// nearest integer is the bits of its sum with 1.5 * 2^23, and the remainder tells whether it is close to a half, where the division is done
-// after all; what fp16 cannot hold and NaN show in the minimum and the maximum.
+// A thread owns 16 neighbours, two words of codes; the 2, 4 or 8 threads of a group find its minimum and maximum by shuffles.  Bound by
+// what a thread has to do rather than by memory, so: the minimum and the maximum of 16-bit values are taken in pairs; the scale is one
+// product and a check; the quotient is a product with 1/scale, whose nearest integer is the bits of its sum with 1.5 * 2^23, and the
+// remainder tells whether it is close to a half, where the division is done after all; what fp16 cannot hold and NaN show in the minimum
+// and the maximum.  4 x 2048 tokens of 8 heads of 128 fp16 channels, keys and values: 29 us with divisions and 8 neighbours a thread.
 #include "four_common.cuh"
 
 namespace xnor
@@ -24,24 +25,56 @@ __device__ __forceinline__ float reciprocal(float v)
 	return r;
 }
 
-// Eight neighbours of a group, `there` of them real, to a word of codes; every lane of the group returns (scale, low).
-__device__ __forceinline__ uint32_t quantize8(float (&v)[8], int there, int group_lanes, __half2 & pair)
+// Least and largest of eight neighbours, NaN where there is one.
+__device__ __forceinline__ void least_and_largest(const Eight<float> & e, float & low, float & top)
 {
-	float low = INFINITY, top = -INFINITY;
+	const float * v = reinterpret_cast<const float *>(e.raw);
+	low = top = v[0];
 	#pragma unroll
-	for (int i = 0; i < 8; ++i)
+	for (int i = 1; i < 8; ++i)
 	{
-		low = there == 8 || i < there ? min_nan(low, v[i]) : low;
-		top = there == 8 || i < there ? max_nan(top, v[i]) : top;
+		low = min_nan(low, v[i]);
+		top = max_nan(top, v[i]);
 	}
-	if (there > 0 && !(low >= -65504.0f && top <= 65504.0f))
+}
+__device__ __forceinline__ void least_and_largest(const Eight<__half> & e, float & low, float & top)
+{
+	const __half2 * v = reinterpret_cast<const __half2 *>(e.raw);
+	const float2 l = __half22float2(__hmin2_nan(__hmin2_nan(v[0], v[1]), __hmin2_nan(v[2], v[3])));
+	const float2 t = __half22float2(__hmax2_nan(__hmax2_nan(v[0], v[1]), __hmax2_nan(v[2], v[3])));
+	low = min_nan(l.x, l.y);
+	top = max_nan(t.x, t.y);
+}
+__device__ __forceinline__ void least_and_largest(const Eight<__nv_bfloat16> & e, float & low, float & top)
+{
+	const __nv_bfloat162 * v = reinterpret_cast<const __nv_bfloat162 *>(e.raw);
+	const float2 l = __bfloat1622float2(__hmin2_nan(__hmin2_nan(v[0], v[1]), __hmin2_nan(v[2], v[3])));
+	const float2 t = __bfloat1622float2(__hmax2_nan(__hmax2_nan(v[0], v[1]), __hmax2_nan(v[2], v[3])));
+	low = min_nan(l.x, l.y);
+	top = max_nan(t.x, t.y);
+}
+
+// 16 neighbours of a group, `there` of them real, to two words of codes; every lane of the group returns (scale, low).
+template <class T>
+__device__ __forceinline__ uint2 quantize16(const Eight<T> & e0, const Eight<T> & e1, int there, int group_lanes, __half2 & pair)
+{
+	float v[16], low, top, more_low, more_top;
+	eight_f32(e0, reinterpret_cast<float (&)[8]>(v[0]));
+	eight_f32(e1, reinterpret_cast<float (&)[8]>(v[8]));
+	least_and_largest(e0, low, top);
+	least_and_largest(e1, more_low, more_top);
+	low = min_nan(low, more_low);
+	top = max_nan(top, more_top);
+	if (there < 16 || !(low >= -65504.0f && top <= 65504.0f))
 	{
 		low = INFINITY;
 		top = -INFINITY;
-		for (int i = 0; i < 8; ++i)
+		#pragma unroll
+		for (int i = 0; i < 16; ++i)
 		{
 			v[i] = v[i] != v[i] ? 0.0f : fminf(fmaxf(v[i], -65504.0f), 65504.0f);
-			if (i < there) { low = fminf(low, v[i]); top = fmaxf(top, v[i]); }
+			low = i < there ? fminf(low, v[i]) : low;
+			top = i < there ? fmaxf(top, v[i]) : top;
 		}
 	}
 	for (int m = 1; m < group_lanes; m <<= 1)
@@ -59,26 +92,27 @@ __device__ __forceinline__ uint32_t quantize8(float (&v)[8], int there, int grou
 	const float step = __half2float(s), by = step > 0.0f ? reciprocal(step) : 0.0f;
 	pair = __halves2half2(s, l);
 	// the bits of 1.5 * 2^23 + code are 0x4b400000 + code: times 16^i they add up to the word and a constant
-	uint32_t word = 0u - 0x4b400000u * 0x11111111u;
+	uint32_t word[2] = {0u - 0x4b400000u * 0x11111111u, 0u - 0x4b400000u * 0x11111111u};
 	float furthest = 0.0f;
 	#pragma unroll
-	for (int i = 0; i < 8; ++i)
+	for (int i = 0; i < 16; ++i)
 	{
 		const float d = v[i] - base, t = fmaf(d, by, 12582912.0f), c = t - 12582912.0f;
 		furthest = fmaxf(furthest, fabsf(fmaf(-c, step, d)));
-		word += __float_as_uint(t) * (1u << (4 * i));
+		word[i / 8] += __float_as_uint(t) * (1u << (4 * (i % 8)));
 	}
 	// (1/scale and the product are off by less than 2^-22 of a quotient below 16; a scale of 0 has nothing further than 0)
-	if (there < 8 || furthest > step * (0.5f - 0x1p-17f))
+	if (there < 16 || furthest > step * (0.5f - 0x1p-17f))
 	{
-		word = 0;
-		for (int i = 0; i < 8; ++i)
+		word[0] = word[1] = 0;
+		#pragma unroll
+		for (int i = 0; i < 16; ++i)
 		{
 			const float q = step > 0.0f && i < there ? rintf(__fdiv_rn(v[i] - base, step)) : 0.0f;
-			word |= (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f) << (4 * i);
+			word[i / 8] |= (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f) << (4 * (i % 8));
 		}
 	}
-	return word;
+	return make_uint2(word[0], word[1]);
 }
 
 // One block a row; k need not fill the last group, nor the last 16 bytes of codes (0 there).
@@ -86,16 +120,15 @@ template <class T>
 __global__ void __launch_bounds__(FR_THREADS)
 four_weights_kernel(const T * __restrict__ weights, long long ld, int k, int group, uint32_t * __restrict__ codes, __half2 * __restrict__ scales, int wide)
 {
-	const int words = (int)(four_row_bytes(k) / 4), groups = (k + group - 1) / group, lanes = group / 8;
+	const int twos = (int)(four_row_bytes(k) / 8), groups = (k + group - 1) / group, lanes = group / 16;
 	const T * row = weights + (long long)blockIdx.x * ld;
 	for (int w0 = 0; w0 < groups * lanes; w0 += FR_THREADS)
 	{
-		const int w = w0 + threadIdx.x, there = max(0, min(8, k - 8 * w));
-		float v[8];
-		eight_f32(load8(row + 8 * (long long)w, there, wide != 0), v);
+		const int w = w0 + threadIdx.x, there = max(0, min(16, k - 16 * w));
+		const Eight<T> e0 = load8(row + 16 * (long long)w, there, wide != 0), e1 = load8(row + 16 * (long long)w + 8, there - 8, wide != 0);
 		__half2 pair;
-		const uint32_t word = quantize8(v, there, lanes, pair);
-		if (w < words) { codes[(size_t)blockIdx.x * words + w] = word; }
+		const uint2 two = quantize16(e0, e1, there, lanes, pair);
+		if (w < twos) { ((uint2 *)codes)[(size_t)blockIdx.x * twos + w] = two; }
 		if (w % lanes == 0 && w < groups * lanes) { scales[(size_t)blockIdx.x * groups + w / lanes] = pair; }
 	}
 }
@@ -153,23 +186,24 @@ kv4_append_kernel(const RowsParams p)
 	find_row(p.c, p.r, b, k.i, page, place);
 	if (page < 0) { return; }
 	const xnor_b200_kv4_tensor & t = p.t[half];
-	const int words = p.c.dim / 8, lanes = p.c.group / 8, groups = p.c.dim / p.c.group;
+	const int twos = p.c.dim / 16, lanes = p.c.group / 16, groups = p.c.dim / p.c.group, shift = p.c.group == 32 ? 1 : p.c.group == 64 ? 2 : 3;
 	const T * src = (const T *)t.data + b * t.stride_sequence + k.i * t.stride_token;
 	const size_t row0 = (size_t)page * p.c.kv_heads * p.c.page + place;
-	uint32_t * codes = (uint32_t *)(half ? p.c.v_codes : p.c.k_codes);
+	uint2 * codes = (uint2 *)(half ? p.c.v_codes : p.c.k_codes);
 	__half2 * scales = (__half2 *)(half ? p.c.v_scales : p.c.k_scales);
+	const int all = p.words / 2;
 	#pragma unroll 2
-	for (int w0 = 0; w0 < p.words; w0 += k.step)
+	for (int w0 = 0; w0 < all; w0 += k.step)
 	{
-		const int w = w0 + k.first, head = (int)__umulhi((uint32_t)w, p.by_words), word = w - head * words;
-		float v[8];
-		eight_f32(load8(src + head * t.stride_head + 8 * word, w < p.words ? 8 : 0, p.wide[half] != 0), v);
+		const int w = w0 + k.first, head = (int)__umulhi((uint32_t)w * 2, p.by_words), two = w - head * twos;
+		const T * from = src + head * t.stride_head + 16 * two;
+		const Eight<T> e0 = load8(from, w < all ? 8 : 0, p.wide[half] != 0), e1 = load8(from + 8, w < all ? 8 : 0, p.wide[half] != 0);
 		__half2 pair;
-		const uint32_t c = quantize8(v, 8, lanes, pair);
-		if (w >= p.words) { continue; }
+		const uint2 c = quantize16(e0, e1, 16, lanes, pair);
+		if (w >= all) { continue; }
 		const size_t row = row0 + (size_t)head * p.c.page;
-		codes[row * words + word] = c;
-		if ((word & (lanes - 1)) == 0) { scales[row * groups + word * 8 / p.c.group] = pair; }
+		codes[row * twos + two] = c;
+		if ((two & (lanes - 1)) == 0) { scales[row * groups + (two >> shift)] = pair; }
 	}
 }
 
