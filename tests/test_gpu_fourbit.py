@@ -172,14 +172,16 @@ def test_product_of_values_of_any_size(dtype):
     assert (np.abs(double(y) - want)[fits] <= tolerance[fits]).all()
 
 
-def test_a_row_that_is_not_finite_gives_nan_and_no_other_does():
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows", [5, 13])
+def test_a_row_that_is_not_finite_gives_nan_and_no_other_does(dtype, rows):
     m = matrix(70, 600, 64, 2)
     for bad in (math.inf, -math.inf, math.nan):
-        x = torch.randn(5, 600, generator=rng(1)).cuda()
+        x = torch.randn(rows, 600, generator=rng(1)).to(dtype).cuda()
         x[1, 300] = bad
         y = F.forward_connected4(m, x)
         assert torch.isnan(y[1]).all()
-        rest = [0, 2, 3, 4]
+        rest = [i for i in range(rows) if i != 1]
         check_product(m, x[rest], y[rest])
 
 
@@ -326,6 +328,49 @@ def test_attention_of_several_tokens(dtype, tokens, share, window):
     q = torch.randn(6, tokens, 3 * share, 128, generator=rng(tokens)).to(dtype).cuda()
     check_attend(s, q, window=window)
     check_attend(s, q, counts=[0, 1, tokens, 1, max(1, tokens // 2), tokens], window=window)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("dim, group", [(32, 32), (64, 32), (64, 64), (96, 32), (128, 32), (128, 128), (192, 32), (256, 128)])
+@pytest.mark.parametrize("tokens, share", [(2, 6), (4, 6), (5, 5)])
+def test_columns_of_every_width(dtype, dim, group, tokens, share):
+    """12, 24 and 25 columns of a head of keys: two and three tiles of eight, and one more than fits."""
+    s = Sequences([150, 3, 64, 0], 2, dim, group, 16, seed=dim + tokens)
+    q = torch.randn(4, tokens, 2 * share, dim, generator=rng(tokens)).to(dtype).cuda()
+    check_attend(s, q, counts=[tokens, 2, 1, 1], window=90)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_scales_below_zero(dtype):
+    s = Sequences([200, 33], 2, 64, 32, 16, seed=6)
+    for scales in (s.cache.k_scales, s.cache.v_scales):
+        scales[..., 0] *= torch.where(torch.rand(scales.shape[:-1], generator=rng(1)) < 0.5, -1.0, 1.0).half().cuda()
+    check_attend(s, torch.randn(2, 1, 6, 64, generator=rng(2)).to(dtype).cuda())
+    m = matrix(90, 500, 32, 2)
+    m.scales[..., 0] *= -1
+    x = torch.randn(4, 500, generator=rng(3)).to(dtype).cuda()
+    check_product(m, x, F.forward_connected4(m, x))
+
+
+def test_lengths_beyond_the_table():
+    """A sequence that is longer than its table has pages for: the positions behind them are nowhere."""
+    s = Sequences([64, 40], 2, 64, 32, 16, seed=5)
+    s.lengths = [70, 2 ** 31 - 1]
+    check_attend(s, torch.randn(2, 3, 4, 64, generator=rng(2)).cuda())
+    s.lengths = [70, 66]
+    table, lengths = s.device()
+    before = s.buffers()
+    k = torch.randn(2, 8, 2, 64, generator=rng(3)).cuda()
+    F.append4(s.cache, k, k, table, lengths)
+    rows = R.find(s.table, s.lengths, None, 8, 16, s.pages)
+    assert sorted(rows) == [(0, 0), (0, 1)]
+    got, _ = F.read4(s.cache, table, lengths, 8)
+    assert got[0, :2].abs().min() >= 0 and not got[0, 2:].any() and not got[1].any()
+    changed = (before[0] != s.buffers()[0]).any((1, 3))
+    assert {(p, i) for p, i in zip(*np.nonzero(changed))} <= set(rows.values())
+    s.lengths = [-3, 0]
+    out = F.attend4(s.cache, torch.randn(2, 3, 4, 64).cuda(), *s.device())
+    assert not out.any()
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
@@ -564,6 +609,37 @@ def test_two_graphs_of_long_sequences_side_by_side():
     torch.cuda.synchronize()
     for _, out, want, _, _ in sets:
         assert torch.equal(out, want)
+
+
+def test_calls_find_their_device(monkeypatch):
+    """Where another device is the current one, a call makes its tensors' device the current one and goes on."""
+    m = matrix(30, 64, 32, 0)
+    x = torch.randn(2, 64, device="cuda")
+    s = Sequences([20, 3], 2, 64, 32)
+    table, lengths = s.device()
+    q, k = torch.randn(2, 1, 4, 64, device="cuda"), torch.randn(2, 1, 2, 64, device="cuda")
+
+    def calls():
+        F.append4(s.cache, k, k, table, lengths)
+        return [F.forward_connected4(m, x), F.attend4(s.cache, q, table, lengths), *F.read4(s.cache, table, lengths, 1)]
+
+    want, current, asked = calls(), F._current_device, []
+
+    def another():
+        asked.append(len(asked))
+        return 1 if len(asked) % 2 else current()
+
+    monkeypatch.setattr(F, "_current_device", another)
+    for a, b in zip(calls(), want):
+        assert torch.equal(a, b)
+    assert len(asked) == 8
+
+
+def test_handles_keep_what_they_were_made_with():
+    m, s = matrix(30, 64, 32, 0), Sequences([20, 3], 2, 64, 32)
+    for handle, name in ((m, "codes"), (m, "k"), (s.cache, "v_scales"), (s.cache, "pages")):
+        with pytest.raises(AttributeError):
+            setattr(handle, name, getattr(handle, name))
 
 
 def test_refusals_name_the_fault():
