@@ -43,7 +43,7 @@ struct AttendParams
 	int heads, share;             // heads of queries, and how many of them a head of keys serves
 	int window, splits, tiles;    // tiles of columns
 	int room;                     // positions that a row of the table has pages for
-	int wide_q;
+	int wide_q, wide_out;         // rows start on 16 bytes; four channels of a row on their size
 };
 
 // What a tile of columns sees of its sequence.  Tokens of rows i0 .. i1.
@@ -108,10 +108,17 @@ __device__ __forceinline__ void write_out(const AttendParams & p, int b, int row
 	none |= m == -INFINITY;
 	T * to = (T *)p.out.data + b * p.out.stride_sequence + row * p.out.stride_token + head * p.out.stride_head + d;
 	const float by = 1.0f / l;
-	to[0] = from_f32<T>(none ? 0.0f : v.x * by);
-	to[1] = from_f32<T>(none ? 0.0f : v.y * by);
-	to[2] = from_f32<T>(none ? 0.0f : v.z * by);
-	to[3] = from_f32<T>(none ? 0.0f : v.w * by);
+	struct alignas(4 * sizeof(T)) Four { T v[4]; } four;
+	four.v[0] = from_f32<T>(none ? 0.0f : v.x * by);
+	four.v[1] = from_f32<T>(none ? 0.0f : v.y * by);
+	four.v[2] = from_f32<T>(none ? 0.0f : v.z * by);
+	four.v[3] = from_f32<T>(none ? 0.0f : v.w * by);
+	if (p.wide_out) { *reinterpret_cast<Four *>(to) = four; }
+	else
+	{
+		#pragma unroll
+		for (int i = 0; i < 4; ++i) { to[i] = four.v[i]; }
+	}
 	if (p.lse != nullptr && d == 0)
 	{
 		p.lse[((size_t)b * p.r.tokens + row) * p.heads + head] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
@@ -698,7 +705,12 @@ four_attend_kernel(const AttendParams p)
 			// (what counts for nothing has seen nothing: its sums are 0)
 			add_weighted(v, s_by[w * COLS + c], *(const float4 *)(first_u + w * WARP_FLOATS + c * S::U_PITCH + q * 4));
 		}
-		if (joined) { *(float4 *)(first_u + c * S::U_PITCH + q * 4) = v; }
+		if (joined && p.splits == 1)
+		{
+			const int row = row_of(p, col0 + c);
+			write_out<T>(p, b, row, head * p.share + col0 + c - row * p.share, q * 4, row >= span.count, s_top[c], s_all[c], v);
+		}
+		else if (joined) { *(float4 *)(first_u + c * S::U_PITCH + q * 4) = v; }
 		else if (begin < end) { *(float4 *)(partial + c * DIM + q * 4) = v; }
 	}
 
@@ -712,6 +724,7 @@ four_attend_kernel(const AttendParams p)
 		}
 		return;
 	}
+	if (p.splits == 1) { return; }
 	const cg::cluster_group cluster = cg::this_cluster();
 	const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
 	cluster.sync();
@@ -974,8 +987,13 @@ extern "C" int xnor_b200_kv4_attend(const xnor_b200_kv4_cache * cache, const xno
 	p.room = room < INT_MAX ? (int)room : INT_MAX;
 	p.splits = plan.splits;
 	p.tiles = plan.tiles;
-	p.wide_q = ((uintptr_t)q->data & 15) == 0 && q->stride_sequence * (long long)size % 16 == 0 && q->stride_token * (long long)size % 16 == 0
-			&& q->stride_head * (long long)size % 16 == 0;
+	const auto fits = [size](const xnor_b200_kv4_tensor & t, long long bytes)
+	{
+		return (uintptr_t)t.data % bytes == 0 && t.stride_sequence * (long long)size % bytes == 0 && t.stride_token * (long long)size % bytes == 0
+				&& t.stride_head * (long long)size % bytes == 0;
+	};
+	p.wide_q = fits(*q, 16);
+	p.wide_out = fits(*output, (long long)size * 4);
 	const cudaStream_t s = (cudaStream_t)stream;
 	switch (q->dtype)
 	{
