@@ -1,7 +1,8 @@
-"""Builds libxnor_b200.so (the CUDA kernels and their C ABI) in-tree with nvcc for sm_100a.
+"""Builds libxnor_b200.so (the CUDA kernels and their C ABI) in-tree with nvcc for sm_100a, and _fourbit.so (the host side of
+darknet_b200.fourbit's calls into it) with the host compiler.
 
 Usage: ``python -m darknet_b200.build [--force] [--verbose]``.  nvcc cross-compiles, so no GPU is
-needed.  The library is rebuilt when any source or header is newer than the existing .so.
+needed.  The libraries are rebuilt when any source or header is newer than the existing ones.
 """
 from __future__ import annotations
 
@@ -16,6 +17,8 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_PATH = os.path.join(PKG_DIR, "libxnor_b200.so")
+BINDINGS = os.path.join(PKG_DIR, "bindings")
+BINDING_PATH = os.path.join(PKG_DIR, "_fourbit.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -37,23 +40,41 @@ def sources() -> list[str]:
 
 
 def _stale() -> bool:
-    if not os.path.exists(LIB_PATH):
+    if not os.path.exists(LIB_PATH) or not os.path.exists(BINDING_PATH):
         return True
-    built = os.path.getmtime(LIB_PATH)
-    deps = sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.hpp")) \
+    built = min(os.path.getmtime(LIB_PATH), os.path.getmtime(BINDING_PATH))
+    deps = sources() + glob.glob(os.path.join(BINDINGS, "*.cpp")) + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.hpp")) \
         + glob.glob(os.path.join(INCLUDE, "*.h"))
     return any(os.path.getmtime(d) > built for d in deps)
 
 
+def _binding(obj: str) -> tuple[list[str], list[str]]:
+    """The commands that compile and link _fourbit.so: torch's headers for the tensors it is handed, the C ABI for everything else."""
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
+    compile_ = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                "-I", INCLUDE, "-isystem", os.path.join(root, "include"), "-isystem", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                "-isystem", cuda, "-I", sysconfig.get_paths()["include"], "-c", os.path.join(BINDINGS, "fourbit_calls.cpp"), "-o", obj]
+    link = ["g++", "-shared", "-o", BINDING_PATH, obj, "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
+            "-L", PKG_DIR, "-lxnor_b200", "-Wl,-rpath,$ORIGIN"]
+    return compile_, link
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile every CUDA source into libxnor_b200.so; returns its path."""
+    """Compile every CUDA source into libxnor_b200.so and the binding beside it; returns the library's path."""
     if not force and not _stale():
         return LIB_PATH
     objs = []
     obj_dir = os.path.join(PKG_DIR, "build")
     os.makedirs(obj_dir, exist_ok=True)
     nvcc = _nvcc()
-    procs = []
+    binding_obj = os.path.join(obj_dir, "fourbit_calls.o")
+    binding_compile, binding_link = _binding(binding_obj)
+    procs = [("fourbit_calls.cpp", subprocess.Popen(binding_compile, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))]
     for src in sources():
         obj = os.path.join(obj_dir, os.path.basename(src) + ".o")
         objs.append(obj)
@@ -75,6 +96,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         raise RuntimeError("nvcc failed; see messages above")
     link = [nvcc, "--shared", "-o", LIB_PATH] + objs
     subprocess.check_call(link)
+    subprocess.check_call(binding_link)
     return LIB_PATH
 
 

@@ -13,7 +13,6 @@ current stream of the tensors' device and may be captured into a CUDA graph.
 from __future__ import annotations
 
 import ctypes as C
-import struct
 from typing import Optional
 
 import torch
@@ -23,25 +22,21 @@ from . import capi
 _DTYPES = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
 _GROUPS = (32, 64, 128)
 
-# A decoding step is a few small kernels, so what a call costs on the host counts: its structs are packed as bytes, in the layout of
-# capi's (which takes a third of the time that filling those takes), and its checks are one expression each; only when that fails
-# _refuse_* look for the fault.
-_CACHE, _ROWS, _TENSOR = struct.Struct("=QQQQiiiii4x").pack, struct.Struct("=iii4xQQQ").pack, struct.Struct("=Qi4xqqq").pack
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
-
 
 class _Calls:
-    """The library's entry points, as functions that take packed structs."""
+    """bindings/fourbit_calls.cpp, loaded at the first call: a decoding step is a few small kernels, so what a call costs on the host counts.
+    Its functions read the tensors, make what is not given and call the library.  They return None where an argument is not what it has to
+    be: _refuse_* then look for the fault and name it."""
 
     def __getattr__(self, name: str):
-        vp, ci, ll = C.c_void_p, C.c_int, C.c_longlong
-        for entry, args in (("w4_forward", [vp, vp, ci, ci, ll, vp, vp, vp, vp, ll, vp, C.c_size_t, vp]), ("w4_scratch_bytes", [vp, ci, ci]), ("kv4_append", [vp] * 5), ("kv4_read", [vp] * 5),
-                            ("kv4_attend", [vp, vp, vp, ci, C.c_float, ci, vp, vp, vp, C.c_size_t, vp]),
-                            ("kv4_attend_scratch_bytes", [vp, vp, ci, ci])):
-            f = capi.lib()["xnor_b200_" + entry]
-            f.argtypes = args
-            f.restype = C.c_size_t if entry.endswith("bytes") else ci
-            setattr(self, entry, f)
+        capi.lib()
+        try:
+            from . import _fourbit
+        except ImportError as e:
+            raise FileNotFoundError(f"_fourbit.so is missing or does not load ({e}): it has not been built (python -m darknet_b200.build). "
+                                    "There is no CPU or PyTorch fallback for this path.") from e
+        for f in ("product", "append", "read", "attend"):
+            setattr(self, f, getattr(_fourbit, f))
         return object.__getattribute__(self, name)
 
 
@@ -83,8 +78,7 @@ class Matrix4(_Fixed):
             raise ValueError(f"scales must be contiguous fp16 [{codes.shape[0]}][{(k + group - 1) // group}][2]")
         if scales.device != codes.device:
             raise ValueError(f"codes on {codes.device}, scales on {scales.device}")
-        self.__dict__.update(codes=codes, scales=scales, n=codes.shape[0], k=k, group=group, device=codes.device, _index=codes.get_device(),
-                             _descs={a: bytes(capi.W4Desc(codes.shape[0], k, group, a)) for a in (capi.LINEAR, capi.LEAKY)})
+        self.__dict__.update(codes=codes, scales=scales, n=codes.shape[0], k=k, group=group, device=codes.device, _native=(codes, scales, k, group))
 
 
 def quantize_weights4(weights: torch.Tensor, group: int) -> Matrix4:
@@ -106,16 +100,15 @@ def quantize_weights4(weights: torch.Tensor, group: int) -> Matrix4:
 
 
 def _refuse_product(m: Matrix4, x, biases, activation, out) -> None:
+    _on(m.device, x, biases, out)
     if x.dim() != 2 or x.shape[1] != m.k or (x.stride(1) != 1 and m.k != 1):
         raise ValueError(f"x must be [rows][{m.k}] with contiguous rows")
     _dtype(x, "x")
-    if activation not in m._descs:
-        raise ValueError("activation must be capi.LINEAR or capi.LEAKY")
     if biases is not None and (biases.dtype != torch.float32 or biases.shape != (m.n,) or not biases.is_contiguous()):
         raise ValueError(f"biases must be contiguous fp32 [{m.n}]")
     if out is not None and (out.dtype != x.dtype or out.shape != (x.shape[0], m.n) or (out.stride(1) != 1 and m.n != 1)):
         raise ValueError(f"out must be {x.dtype} [{x.shape[0]}][{m.n}] with contiguous rows")
-    _on(m.device, x, m.codes, m.scales, biases, out)
+    raise ValueError("activation must be capi.LINEAR or capi.LEAKY, x of fewer than 2^31 rows")
 
 
 def forward_connected4(m: Matrix4, x: torch.Tensor, biases: Optional[torch.Tensor] = None, activation: int = capi.LINEAR,
@@ -123,30 +116,12 @@ def forward_connected4(m: Matrix4, x: torch.Tensor, biases: Optional[torch.Tenso
     """act(x @ W.T + biases) for x [rows][k] (rows contiguous, any distance apart), W the packed matrix: xnor_b200_w4_forward.
     biases: fp32 [n].  out: [rows][n] of x's type, rows contiguous; made where it is not given.  One pass over the weights serves up to
     16 rows."""
-    index, shape, dtype, desc, n = m._index, x.shape, _DTYPES.get(x.dtype), m._descs.get(activation), m.n
-    if (index < 0 or dtype is None or desc is None or out is not None or len(shape) != 2 or shape[1] != m.k or x.get_device() != index
-            or not x.is_contiguous()
-            or (biases is not None and (biases.dtype is not torch.float32 or biases.shape != (n,) or not biases.is_contiguous() or biases.get_device() != index))):
+    y = _calls.product(m._native, x, biases, activation, out)
+    if y is None:
         _refuse_product(m, x, biases, activation, out)
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return forward_connected4(m, x, biases, activation, out)
-    rows = shape[0]
-    if out is None:
-        out = x.new_empty((rows, n))
-    if rows == 0:
-        return out
-    nbytes, scratch = 0, None
-    if rows > 8:                                              # (fewer never need any)
-        nbytes = _calls.w4_scratch_bytes(desc, dtype, rows)
-        if nbytes:
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    rc = _calls.w4_forward(desc, x.data_ptr(), dtype, rows, x.stride(0) if rows > 1 else m.k, m.codes.data_ptr(), m.scales.data_ptr(),
-                           None if biases is None else biases.data_ptr(), out.data_ptr(), out.stride(0) if rows > 1 else n,
-                           None if scratch is None else scratch.data_ptr(), nbytes, _raw_stream(index))
-    if rc:
-        capi.check(rc, "xnor_b200_w4_forward")
-    return out
+    if type(y) is int:
+        capi.check(y, "xnor_b200_w4_forward")
+    return y
 
 
 class Cache4(_Fixed):
@@ -169,14 +144,8 @@ class Cache4(_Fixed):
                 raise ValueError(f"scales must be contiguous fp16 {[pages, kv_heads, page, dim // group, 2]}")
             if codes.device != k_codes.device or scales.device != k_codes.device:
                 raise ValueError("all four buffers must be on one device")
-        # _scratch: bytes of scratch memory by the sizes of a call
         self.__dict__.update(k_codes=k_codes, k_scales=k_scales, v_codes=v_codes, v_scales=v_scales, pages=pages, kv_heads=kv_heads, page=page,
-                             dim=dim, group=group, device=k_codes.device, _index=k_codes.get_device(), _scale=dim ** -0.5, _scratch={})
-
-    def _struct(self) -> bytes:
-        """Packed for every call, so that it never names memory that a tensor has given up."""
-        return _CACHE(self.k_codes.data_ptr(), self.k_scales.data_ptr(), self.v_codes.data_ptr(), self.v_scales.data_ptr(), self.pages,
-                      self.kv_heads, self.page, self.dim, self.group)
+                             dim=dim, group=group, device=k_codes.device, _native=(k_codes, k_scales, v_codes, v_scales, group))
 
 
 def new_cache4(pages: int, kv_heads: int, page: int, dim: int, group: int, device="cuda:0") -> Cache4:
@@ -189,73 +158,43 @@ def new_cache4(pages: int, kv_heads: int, page: int, dim: int, group: int, devic
                   buffer(dim // group, 2, dtype=torch.float16), group)
 
 
-def _rows(c: Cache4, batch: int, tokens: int, table: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor]) -> bytes:
-    """struct xnor_b200_kv4_rows of a call, checked."""
-    index, shape = c._index, table.shape
-    if (index < 0 or len(shape) != 2 or shape[0] != batch or shape[1] == 0 or table.dtype is not torch.int32 or not table.is_contiguous()
-            or lengths.dtype is not torch.int32 or lengths.shape != (batch,) or not lengths.is_contiguous() or table.get_device() != index
-            or lengths.get_device() != index
-            or (counts is not None and (counts.dtype is not torch.int32 or counts.shape != (batch,) or not counts.is_contiguous() or counts.get_device() != index))):
-        if len(shape) != 2 or shape[0] != batch or shape[1] == 0 or table.dtype != torch.int32 or not table.is_contiguous():
-            raise ValueError(f"table must be contiguous int32 [{batch}][pages of a sequence]")
-        for name, t in (("lengths", lengths), ("counts", counts)):
-            if t is not None and (t.dtype != torch.int32 or t.shape != (batch,) or not t.is_contiguous()):
-                raise ValueError(f"{name} must be contiguous int32 [{batch}]")
-        _on(c.device, table, lengths, counts)
-    return _ROWS(batch, tokens, shape[1], table.data_ptr(), lengths.data_ptr(), 0 if counts is None else counts.data_ptr())
-
-
-def _tensor(t: torch.Tensor, dtype: int, index: int, what: str) -> bytes:
-    """struct xnor_b200_kv4_tensor of a tensor of four dimensions on device `index`."""
-    a, b, c, d = t.stride()
-    if d != 1 and t.shape[3] != 1:
-        raise ValueError(f"the last dimension of {what} must be contiguous")
-    if t.get_device() != index or index < 0:
-        raise ValueError(f"{what} on {t.device}: all of a call's tensors are on one CUDA device, the cache's")
-    return _TENSOR(t.data_ptr(), dtype, a, b, c)
+def _refuse_rows(c: Cache4, batch: int, table, lengths, counts) -> None:
+    _on(c.device, table, lengths, counts)
+    if table.dim() != 2 or table.shape[0] != batch or table.shape[1] == 0 or table.dtype != torch.int32 or not table.is_contiguous():
+        raise ValueError(f"table must be contiguous int32 [{batch}][pages of a sequence]")
+    for name, t in (("lengths", lengths), ("counts", counts)):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (batch,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous int32 [{batch}]")
 
 
 def append4(c: Cache4, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor] = None) -> None:
     """Packs the newest tokens' keys and values [batch][tokens][kv_heads][dim] into their pages: xnor_b200_kv4_append.  lengths: what each
     sequence holds with them; counts: how many of the rows are tokens (default: all), the first ones of each sequence.  table: int32
     [batch][pages of a sequence].  No two rows may share a place."""
-    shape, dtype = k.shape, _DTYPES.get(k.dtype)
-    if dtype is None or len(shape) != 4 or shape[2] != c.kv_heads or shape[3] != c.dim or v.shape != shape or v.dtype is not k.dtype:
+    done = _calls.append(c._native, k, v, table, lengths, counts)
+    if done is None:
+        _on(c.device, k, v)
         _dtype(k, "k")
-        raise ValueError(f"k and v must be [batch][tokens][{c.kv_heads}][{c.dim}] of one type")
-    index = c._index
-    kt, vt, rows = _tensor(k, dtype, index, "k"), _tensor(v, dtype, index, "v"), _rows(c, shape[0], shape[1], table, lengths, counts)
-    if k.numel() == 0:
-        return
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return append4(c, k, v, table, lengths, counts)
-    rc = _calls.kv4_append(c._struct(), rows, kt, vt, _raw_stream(index))
-    if rc:
-        capi.check(rc, "xnor_b200_kv4_append")
+        if k.dim() != 4 or k.shape[2:] != (c.kv_heads, c.dim) or v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError(f"k and v must be [batch][tokens][{c.kv_heads}][{c.dim}] of one type")
+        _refuse_rows(c, k.shape[0], table, lengths, counts)
+        raise ValueError("the last dimension of k and v must be contiguous")
+    if type(done) is int:
+        capi.check(done, "xnor_b200_kv4_append")
 
 
 def read4(c: Cache4, table: torch.Tensor, lengths: torch.Tensor, tokens: int, counts: Optional[torch.Tensor] = None, dtype=torch.float32):
     """What the cache holds for the last `tokens` positions (or counts[b] of them) of every sequence, as keys and values [batch][tokens][kv_heads][dim]:
     xnor_b200_kv4_read.  Rows that stand for no token are 0."""
-    if dtype not in _DTYPES:
-        raise ValueError(f"dtype must be fp32, fp16 or bf16, not {dtype}")
-    if table.dim() != 2 or tokens < 0:
-        raise ValueError("table must be int32 [batch][pages of a sequence], tokens at least 0")
-    index, batch = c._index, table.shape[0]
-    rows = _rows(c, batch, tokens, table, lengths, counts)
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return read4(c, table, lengths, tokens, counts, dtype)
-    k = torch.empty((batch, tokens, c.kv_heads, c.dim), dtype=dtype, device=c.device)
-    v = torch.empty_like(k)
-    if batch and tokens:
-        head = c.dim
-        strides = (_DTYPES[dtype], tokens * c.kv_heads * head, c.kv_heads * head, head)
-        rc = _calls.kv4_read(c._struct(), rows, _TENSOR(k.data_ptr(), *strides), _TENSOR(v.data_ptr(), *strides), _raw_stream(index))
-        if rc:
-            capi.check(rc, "xnor_b200_kv4_read")
-    return k, v
+    both = _calls.read(c._native, table, lengths, tokens, counts, _DTYPES.get(dtype, -1))
+    if both is None:
+        if dtype not in _DTYPES:
+            raise ValueError(f"dtype must be fp32, fp16 or bf16, not {dtype}")
+        _refuse_rows(c, table.shape[0], table, lengths, counts)
+        raise ValueError("tokens must be a number, at least 0")
+    if type(both) is int:
+        capi.check(both, "xnor_b200_kv4_read")
+    return both
 
 
 def attend4(c: Cache4, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor] = None,
@@ -264,35 +203,18 @@ def attend4(c: Cache4, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tens
     comes first): xnor_b200_kv4_attend.  scale: 1/sqrt(dim) where not given.  window: positions that a token sees, itself among them
     (0: all).  Rows that see nothing are 0.  out: as q; made where it is not given.  lse: fp32 [batch][tokens][heads], contiguous, receives
     the logarithm of each row's sum of exponentials."""
-    index, shape, dtype = c._index, q.shape, _DTYPES.get(q.dtype)
-    if dtype is None or len(shape) != 4 or shape[3] != c.dim or shape[2] == 0 or shape[2] % c.kv_heads or window < 0:
+    y = _calls.attend(c._native, q, table, lengths, counts, scale, window, out, lse)
+    if y is None:
+        _on(c.device, q, out, lse)
         _dtype(q, "q")
-        raise ValueError(f"q must be [batch][tokens][heads][{c.dim}], heads a multiple of {c.kv_heads}; window at least 0")
-    if out is not None and (out.shape != shape or out.dtype != q.dtype):
-        raise ValueError(f"out must be {q.dtype} {list(shape)}")
-    if out is not None and torch._debug_has_internal_overlap(out) == 1:
-        raise ValueError("out has rows that share memory")
-    if lse is not None and (lse.shape != shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.get_device() != index):
-        raise ValueError(f"lse must be contiguous fp32 {list(shape[:3])} on the cache's device")
-    batch, tokens, heads = shape[0], shape[1], shape[2]
-    rows, qt = _rows(c, batch, tokens, table, lengths, counts), _tensor(q, dtype, index, "q")
-    if _current_device() != index:
-        with torch.cuda.device(index):
-            return attend4(c, q, table, lengths, counts, scale, window, out, lse)
-    if out is None:
-        out = torch.empty_like(q)
-    if batch == 0 or tokens == 0:
-        return out
-    ot = _tensor(out, dtype, index, "out")
-    cache, sizes = c._struct(), (batch, tokens, table.shape[1], heads, window)
-    nbytes = c._scratch.get(sizes)
-    if nbytes is None:
-        if len(c._scratch) >= 1024:
-            c._scratch.clear()
-        nbytes = c._scratch[sizes] = _calls.kv4_attend_scratch_bytes(cache, rows, heads, window)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=c.device) if nbytes else None
-    rc = _calls.kv4_attend(cache, rows, qt, heads, c._scale if scale is None else scale, window, ot, None if lse is None else lse.data_ptr(),
-                           None if scratch is None else scratch.data_ptr(), nbytes, _raw_stream(index))
-    if rc:
-        capi.check(rc, "xnor_b200_kv4_attend")
-    return out
+        if q.dim() != 4 or q.shape[3] != c.dim or q.shape[2] == 0 or q.shape[2] % c.kv_heads or q.stride(3) != 1:
+            raise ValueError(f"q must be [batch][tokens][heads][{c.dim}], heads a multiple of {c.kv_heads}, the last dimension contiguous")
+        _refuse_rows(c, q.shape[0], table, lengths, counts)
+        if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1 or torch._debug_has_internal_overlap(out) == 1):
+            raise ValueError(f"out must be {q.dtype} {list(q.shape)}, the last dimension contiguous, no memory used twice")
+        if lse is not None and (lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous()):
+            raise ValueError(f"lse must be contiguous fp32 {list(q.shape[:3])}")
+        raise ValueError("window must be a number, at least 0")
+    if type(y) is int:
+        capi.check(y, "xnor_b200_kv4_attend")
+    return y

@@ -120,13 +120,23 @@ def test_attention_refuses(L):
     assert L.xnor_b200_kv4_attend_scratch_bytes(c, r, 3, 0) == 0
 
 
-def test_packed_structs_are_the_librarys():
-    c = capi.Kv4Cache(1, 2, 3, 4, 5, 6, 7, 8, 9)
-    assert F._CACHE(1, 2, 3, 4, 5, 6, 7, 8, 9) == bytes(c)
-    r = capi.Kv4Rows(1, 2, 3, 4, 5, 6)
-    assert F._ROWS(1, 2, 3, 4, 5, 6) == bytes(r)
-    t = capi.Kv4Tensor(1, 2, 3, -4, 5)
-    assert F._TENSOR(1, 2, 3, -4, 5) == bytes(t)
+def test_a_missing_binding_fails_loudly(monkeypatch):
+    import sys
+    calls = F._Calls()
+    monkeypatch.setitem(sys.modules, "darknet_b200._fourbit", None)
+    monkeypatch.delattr("darknet_b200._fourbit", raising=False)
+    with pytest.raises(FileNotFoundError, match="no CPU or PyTorch fallback"):
+        calls.product
+
+
+def test_bindings_take_nothing_else():
+    from darknet_b200 import _fourbit
+    t = torch.zeros(2, 2)
+    for f in (_fourbit.product, _fourbit.append, _fourbit.read, _fourbit.attend):
+        assert f() is None and f(t) is None and f(None, None, None, None, None, None) is None
+        for n in (5, 6, 9):
+            assert f(*["x"] * n) is None and f(*[t] * n) is None and f((t,) * 5, *[t] * (n - 1)) is None
+            assert f((t, t, 2, 32), *[None] * (n - 1)) is None
 
 
 def test_tensors_off_the_gpu_are_refused():

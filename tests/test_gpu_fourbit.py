@@ -595,8 +595,10 @@ def test_two_graphs_of_long_sequences_side_by_side():
         q = torch.randn(1, 1, 4, 64, generator=rng(seed)).half().cuda()
         table, lengths = s.device()
         want = F.attend4(s.cache, q, table, lengths)
-        assert capi.lib().xnor_b200_kv4_attend_scratch_bytes(capi.Kv4Cache.from_buffer_copy(s.cache._struct()),
-                                                              capi.Kv4Rows.from_buffer_copy(F._rows(s.cache, 1, 1, table, lengths, None)), 4, 0) > 0
+        c = s.cache
+        assert capi.lib().xnor_b200_kv4_attend_scratch_bytes(
+            capi.Kv4Cache(*(t.data_ptr() for t in c._native[:4]), c.pages, c.kv_heads, c.page, c.dim, c.group),
+            capi.Kv4Rows(1, 1, table.shape[1], table.data_ptr(), lengths.data_ptr(), None), 4, 0) > 0
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             out = F.attend4(s.cache, q, table, lengths)
@@ -609,30 +611,6 @@ def test_two_graphs_of_long_sequences_side_by_side():
     torch.cuda.synchronize()
     for _, out, want, _, _ in sets:
         assert torch.equal(out, want)
-
-
-def test_calls_find_their_device(monkeypatch):
-    """Where another device is the current one, a call makes its tensors' device the current one and goes on."""
-    m = matrix(30, 64, 32, 0)
-    x = torch.randn(2, 64, device="cuda")
-    s = Sequences([20, 3], 2, 64, 32)
-    table, lengths = s.device()
-    q, k = torch.randn(2, 1, 4, 64, device="cuda"), torch.randn(2, 1, 2, 64, device="cuda")
-
-    def calls():
-        F.append4(s.cache, k, k, table, lengths)
-        return [F.forward_connected4(m, x), F.attend4(s.cache, q, table, lengths), *F.read4(s.cache, table, lengths, 1)]
-
-    want, current, asked = calls(), F._current_device, []
-
-    def another():
-        asked.append(len(asked))
-        return 1 if len(asked) % 2 else current()
-
-    monkeypatch.setattr(F, "_current_device", another)
-    for a, b in zip(calls(), want):
-        assert torch.equal(a, b)
-    assert len(asked) == 8
 
 
 def test_handles_keep_what_they_were_made_with():
@@ -657,6 +635,9 @@ def test_refusals_name_the_fault():
                   lambda: F.attend4(s.cache, q, table[:1], lengths), lambda: F.attend4(s.cache, q, table, lengths, window=-1),
                   lambda: F.attend4(s.cache, q, table, lengths, out=q[:, :, :, :32]), lambda: F.attend4(s.cache, q[..., :32], table, lengths),
                   lambda: F.attend4(s.cache, q, table, lengths, out=q[:, :, :1].expand(-1, -1, 4, -1)),
+                  lambda: F.attend4(s.cache, q, table, lengths, window=0.5), lambda: F.read4(s.cache, table, lengths, -1),
+                  lambda: F.read4(s.cache, table, lengths, 1, dtype=torch.float64), lambda: F.forward_connected4(m, x, biases=x[0, :8].half()),
+                  lambda: F.attend4(s.cache, q.transpose(2, 3).contiguous().transpose(2, 3), table, lengths),
                   lambda: F.attend4(s.cache, q, table, lengths, lse=torch.zeros(2, 1, 4, device="cuda").half())):
         with pytest.raises(ValueError):
             wrong()
