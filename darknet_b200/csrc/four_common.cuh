@@ -38,6 +38,30 @@ inline size_t four_size(int t) { return t == XNOR_B200_F32 ? 4 : 2; }
 
 #ifdef __CUDACC__
 
+// Every kernel of a call but the load-time ones starts with pdl_wait() and pdl_trigger() and is launched through this: its CTAs take their
+// places while the kernel in front of it on the stream finishes, and do nothing before it has.  A decoding step is a chain of such kernels.
+// cluster: CTAs of a cluster, along x.
+template <class Kernel, class... Args>
+int launch_four(Kernel kernel, dim3 grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t stream, const Args & ... args)
+{
+	cudaLaunchConfig_t cfg = {};
+	cfg.gridDim = grid;
+	cfg.blockDim = dim3(threads, 1, 1);
+	cfg.dynamicSmemBytes = smem;
+	cfg.stream = stream;
+	cudaLaunchAttribute attr[2];
+	attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	attr[0].val.programmaticStreamSerializationAllowed = 1;
+	attr[1].id = cudaLaunchAttributeClusterDimension;
+	attr[1].val.clusterDim.x = cluster;
+	attr[1].val.clusterDim.y = 1;
+	attr[1].val.clusterDim.z = 1;
+	cfg.attrs = attr;
+	cfg.numAttrs = cluster > 1 ? 2 : 1;
+	const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+	return e == cudaSuccess ? check_launch() : cuda_fail(e);
+}
+
 // The smaller and the larger value; NaN where there is one.
 __device__ __forceinline__ float min_nan(float a, float b)
 {

@@ -122,6 +122,7 @@ four_x_kernel(const ProductParams p, unsigned char * ready)
 	using S = ProductShape<T, NT, 2, 8, GROUP, 1>;
 	const int row0 = blockIdx.y * S::ROWS, rows = min(S::ROWS, p.rows - row0), x_rows = min(S::ROWS, p.rows), lane = threadIdx.x % 32;
 	unsigned char * buffer = ready + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * S::buffer_bytes(x_rows);
+	pdl_wait();
 	pdl_trigger();                                            // the product may be launched; it waits for this kernel's end
 	for (int row = threadIdx.x / 32; row < rows; row += 8)
 	{
@@ -220,11 +221,18 @@ four_product_kernel(const ProductParams p)
 		for (int i = threadIdx.x * 16; i < S::buffer_bytes(x_rows); i += S::THREADS * 16) { copy16(four_smem(buffer) + i, from + i, true); }
 	};
 
-	if (!READY) { load_x(first); }
+	// (READY: this kernel's predecessor is four_x_kernel, which lets it start behind everything that wrote the weights)
+	if (!READY)
+	{
+		pdl_wait();
+		pdl_trigger();
+		load_x(first);
+	}
 	for (int i = 0; i < p.steps - 1; ++i) { request(); }
 	if (READY)
 	{
 		pdl_wait();
+		pdl_trigger();
 		if (first < last) { copy_x(first, buffers); }
 		copies_close();
 	}
@@ -430,26 +438,10 @@ static int launch_product(ProductParams & p, void * scratch, cudaStream_t stream
 	if (READY)
 	{
 		p.ready = (const unsigned char *)scratch;
-		four_x_kernel<T, NT, GROUP><<<dim3((unsigned)blocks, row_tiles), 256, 0, stream>>>(p, (unsigned char *)scratch);
-		const int x_rc = check_launch();
+		const int x_rc = launch_four(four_x_kernel<T, NT, GROUP>, dim3((unsigned)blocks, row_tiles), 256, 0, 1, stream, p, (unsigned char *)scratch);
 		if (x_rc != XNOR_B200_OK) { return x_rc; }
 	}
-	cudaLaunchConfig_t cfg = {};
-	cfg.gridDim = dim3((unsigned)(tiles * ranks), row_tiles, 1);
-	cfg.blockDim = dim3(S::THREADS, 1, 1);
-	cfg.dynamicSmemBytes = smem;
-	cfg.stream = stream;
-	cudaLaunchAttribute attr[2];
-	attr[0].id = cudaLaunchAttributeClusterDimension;
-	attr[0].val.clusterDim.x = (unsigned)ranks;
-	attr[0].val.clusterDim.y = 1;
-	attr[0].val.clusterDim.z = 1;
-	attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-	attr[1].val.programmaticStreamSerializationAllowed = 1;
-	cfg.attrs = attr;
-	cfg.numAttrs = READY ? 2 : 1;
-	const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
-	return e == cudaSuccess ? check_launch() : cuda_fail(e);
+	return launch_four(kernel, dim3((unsigned)(tiles * ranks), row_tiles), S::THREADS, smem, (unsigned)ranks, stream, p);
 }
 
 template <class T, int NT, int GROUP>

@@ -179,6 +179,8 @@ template <class T>
 __global__ void __launch_bounds__(FR_THREADS)
 kv4_append_kernel(const RowsParams p)
 {
+	pdl_wait();
+	pdl_trigger();
 	const int half = blockIdx.z, b = blockIdx.y;
 	const RowsTask k = task_of(p);
 	if (k.i >= p.r.tokens) { return; }
@@ -221,6 +223,8 @@ template <class T>
 __global__ void __launch_bounds__(FR_THREADS)
 kv4_read_kernel(const RowsParams p)
 {
+	pdl_wait();
+	pdl_trigger();
 	const int half = blockIdx.z, b = blockIdx.y;
 	const RowsTask k = task_of(p);
 	if (k.i >= p.r.tokens) { return; }
@@ -341,10 +345,9 @@ extern "C" int xnor_b200_kv4_append(const xnor_b200_kv4_cache * cache, const xno
 	if (rc != XNOR_B200_OK) { return rc; }
 	const dim3 grid((unsigned)(p.warps == 1 ? (rows->tokens - 1) / (FR_THREADS / 32) + 1 : rows->tokens), (unsigned)rows->batch, 2);
 	const cudaStream_t s = (cudaStream_t)stream;
-	if (k->dtype == XNOR_B200_F32) { kv4_append_kernel<float><<<grid, FR_THREADS, 0, s>>>(p); }
-	else if (k->dtype == XNOR_B200_F16) { kv4_append_kernel<__half><<<grid, FR_THREADS, 0, s>>>(p); }
-	else { kv4_append_kernel<__nv_bfloat16><<<grid, FR_THREADS, 0, s>>>(p); }
-	return check_launch();
+	if (k->dtype == XNOR_B200_F32) { return launch_four(kv4_append_kernel<float>, grid, FR_THREADS, 0, 1, s, p); }
+	if (k->dtype == XNOR_B200_F16) { return launch_four(kv4_append_kernel<__half>, grid, FR_THREADS, 0, 1, s, p); }
+	return launch_four(kv4_append_kernel<__nv_bfloat16>, grid, FR_THREADS, 0, 1, s, p);
 }
 
 extern "C" int xnor_b200_kv4_read(const xnor_b200_kv4_cache * cache, const xnor_b200_kv4_rows * rows, const xnor_b200_kv4_tensor * k,
@@ -355,8 +358,7 @@ extern "C" int xnor_b200_kv4_read(const xnor_b200_kv4_cache * cache, const xnor_
 	if (rc != XNOR_B200_OK) { return rc; }
 	const dim3 grid((unsigned)(p.warps == 1 ? (rows->tokens - 1) / (FR_THREADS / 32) + 1 : rows->tokens), (unsigned)rows->batch, 2);
 	const cudaStream_t s = (cudaStream_t)stream;
-	if (k->dtype == XNOR_B200_F32) { kv4_read_kernel<float><<<grid, FR_THREADS, 0, s>>>(p); }
-	else if (k->dtype == XNOR_B200_F16) { kv4_read_kernel<__half><<<grid, FR_THREADS, 0, s>>>(p); }
-	else { kv4_read_kernel<__nv_bfloat16><<<grid, FR_THREADS, 0, s>>>(p); }
-	return check_launch();
+	if (k->dtype == XNOR_B200_F32) { return launch_four(kv4_read_kernel<float>, grid, FR_THREADS, 0, 1, s, p); }
+	if (k->dtype == XNOR_B200_F16) { return launch_four(kv4_read_kernel<__half>, grid, FR_THREADS, 0, 1, s, p); }
+	return launch_four(kv4_read_kernel<__nv_bfloat16>, grid, FR_THREADS, 0, 1, s, p);
 }
