@@ -166,15 +166,32 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[W], const void * p)
 	else { w[0] = *(const uint32_t *)p; }
 }
 
+// The (scale, low) pairs of a position, of all its groups.
+template <int GROUPS>
+__device__ __forceinline__ void load_pairs(uint32_t (&w)[GROUPS], const uint32_t * p)
+{
+	if constexpr (GROUPS == 1 || GROUPS == 2 || GROUPS == 4) { load_words<GROUPS>(w, p); }
+	else if constexpr (GROUPS == 8)
+	{
+		load_words<4>(reinterpret_cast<uint32_t (&)[4]>(w[0]), p);
+		load_words<4>(reinterpret_cast<uint32_t (&)[4]>(w[4]), p + 4);
+	}
+	else
+	{
+		#pragma unroll
+		for (int i = 0; i < GROUPS; ++i) { w[i] = p[i]; }
+	}
+}
+
 // Weights of 16 positions with the scales of a group: operands of the product with the codes, and the sums of weight * low.  WILD: a
 // weight of 0 counts as nothing, whatever the scale (a branch that is hardly ever taken costs less than selecting every time).
 template <bool WILD, int NT, int PP>
-__device__ __forceinline__ void weigh(uint32_t (&pv)[NT][PP][2], float (&lows)[NT][2], const float (&w)[NT][4], const uint32_t (&pairs)[2], float unit)
+__device__ __forceinline__ void weigh(uint32_t (&pv)[NT][PP][2], float (&lows)[NT][2], const float (&w)[NT][4], uint32_t pair0, uint32_t pair1, float unit)
 {
 	#pragma unroll
 	for (int r = 0; r < 2; ++r)
 	{
-		float2 sl = halves(pairs[r]);
+		float2 sl = halves(r == 0 ? pair0 : pair1);
 		sl.y += 8.0f * sl.x;
 		sl.x *= unit;
 		#pragma unroll
@@ -376,6 +393,13 @@ four_attend_kernel(const AttendParams p)
 
 		// ---- scores
 		float s[2][NT][4] = {};
+		uint32_t sk[2][2][GROUPS];
+		#pragma unroll
+		for (int h = 0; h < 2; ++h)
+		{
+			#pragma unroll
+			for (int r = 0; r < 2; ++r) { load_pairs<GROUPS>(sk[h][r], k_pairs + (h * 16 + r * 8) * GROUPS); }
+		}
 		#pragma unroll
 		for (int gr = 0; gr < GROUPS; ++gr)
 		{
@@ -418,7 +442,7 @@ four_attend_kernel(const AttendParams p)
 			#pragma unroll
 			for (int h = 0; h < 2; ++h)
 			{
-				float2 sl0 = halves(k_pairs[h * 16 * GROUPS + gr]), sl1 = halves(k_pairs[(h * 16 + 8) * GROUPS + gr]);
+				float2 sl0 = halves(sk[h][0][gr]), sl1 = halves(sk[h][1][gr]);
 				sl0.y += How::SHIFT * sl0.x;
 				sl1.y += How::SHIFT * sl1.x;
 				#pragma unroll
@@ -447,16 +471,12 @@ four_attend_kernel(const AttendParams p)
 		}
 
 		// ---- what is not seen: neither its score nor its scales count, whatever they are
-		uint32_t sv[GROUPS][2][2];
+		uint32_t sv[2][2][GROUPS];
 		#pragma unroll
-		for (int gr = 0; gr < GROUPS; ++gr)
+		for (int h = 0; h < 2; ++h)
 		{
 			#pragma unroll
-			for (int h = 0; h < 2; ++h)
-			{
-				#pragma unroll
-				for (int r = 0; r < 2; ++r) { sv[gr][h][r] = v_pairs[(h * 16 + r * 8) * GROUPS + gr]; }
-			}
+			for (int r = 0; r < 2; ++r) { load_pairs<GROUPS>(sv[h][r], v_pairs + (h * 16 + r * 8) * GROUPS); }
 		}
 		bool wild = false;                                    // a scale that one column sees and another does not is not finite
 		const bool edge = step * 16 < all_from || step * 16 + 32 > all_to || there != 3;
@@ -485,8 +505,8 @@ four_attend_kernel(const AttendParams p)
 					#pragma unroll
 					for (int gr = 0; gr < GROUPS; ++gr)
 					{
-						sv[gr][h][r] = any ? sv[gr][h][r] : 0;
-						wild |= (sv[gr][h][r] & 0x7c00u) == 0x7c00u || (sv[gr][h][r] & 0x7c000000u) == 0x7c000000u;
+						sv[h][r][gr] = any ? sv[h][r][gr] : 0;
+						wild |= (sv[h][r][gr] & 0x7c00u) == 0x7c00u || (sv[h][r][gr] & 0x7c000000u) == 0x7c000000u;
 					}
 				}
 			}
@@ -509,7 +529,7 @@ four_attend_kernel(const AttendParams p)
 			for (int gr = 0; gr < GROUPS; ++gr)
 			{
 				#pragma unroll
-				for (int r = 0; r < 2; ++r) { widest = __hmax2(widest, __habs2(as_half2(sv[gr][h][r]))); }
+				for (int r = 0; r < 2; ++r) { widest = __hmax2(widest, __habs2(as_half2(sv[h][r][gr]))); }
 			}
 		}
 		move |= (as_word(widest) & 0xffffu) > unit_top;
@@ -523,7 +543,7 @@ four_attend_kernel(const AttendParams p)
 				#pragma unroll
 				for (int i = 0; i < 4; ++i)
 				{
-					const uint32_t bits = sv[gr][i / 2][i % 2] & 0x7fffu;
+					const uint32_t bits = sv[i / 2][i % 2][gr] & 0x7fffu;
 					largest = max(largest, bits < 0x7c00u ? bits : 0);
 				}
 			}
@@ -603,8 +623,8 @@ four_attend_kernel(const AttendParams p)
 			for (int h = 0; h < 2; ++h)
 			{
 				uint32_t pv[NT][PP][2];
-				if (wild) { weigh<true, NT, PP>(pv, lows[gr], s[h], sv[gr][h], unit); }
-				else { weigh<false, NT, PP>(pv, lows[gr], s[h], sv[gr][h], unit); }
+				if (wild) { weigh<true, NT, PP>(pv, lows[gr], s[h], sv[h][0][gr], sv[h][1][gr], unit); }
+				else { weigh<false, NT, PP>(pv, lows[gr], s[h], sv[h][0][gr], sv[h][1][gr], unit); }
 				uint32_t w[4][GB];
 				#pragma unroll
 				for (int i = 0; i < 4; ++i)
