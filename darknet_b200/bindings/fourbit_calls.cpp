@@ -108,6 +108,7 @@ PyObject * product(PyObject *, PyObject * const * args, Py_ssize_t n_args)
 		if (n_args != 5 || !PyTuple_Check(args[0]) || PyTuple_GET_SIZE(args[0]) != 4) { Py_RETURN_NONE; }
 		if (!take(PyTuple_GET_ITEM(args[0], 0), codes) || !take(PyTuple_GET_ITEM(args[0], 1), scales) || !take(args[1], x) || !take(args[2], biases)
 				|| !take(args[4], given) || codes == nullptr || scales == nullptr || x == nullptr || !PyLong_Check(args[3])) { Py_RETURN_NONE; }
+		if (codes->dim() != 2) { Py_RETURN_NONE; }
 		const int64_t n = codes->size(0), k = whole(PyTuple_GET_ITEM(args[0], 2));
 		const c10::Device d = codes->device();
 		const int type = type_of(*x);
@@ -153,6 +154,7 @@ bool take_cache(PyObject * o, xnor_b200_kv4_cache & c, std::optional<c10::Device
 		if (!on(*v, *d)) { return false; }
 	}
 	const at::IntArrayRef s = t[0]->sizes();
+	if (s.size() != 4) { return false; }
 	c = {(uint8_t *)t[0]->data_ptr(), t[1]->data_ptr(), (uint8_t *)t[2]->data_ptr(), t[3]->data_ptr(), (int)s[0], (int)s[1], (int)s[2], (int)(2 * s[3]),
 			(int)whole(PyTuple_GET_ITEM(o, 4))};
 	return s[0] <= INT_MAX && s[1] <= INT_MAX && s[2] <= INT_MAX;

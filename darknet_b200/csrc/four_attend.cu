@@ -9,10 +9,6 @@ namespace xnor
 
 int validate_kv4(const xnor_b200_kv4_cache * c, const xnor_b200_kv4_rows * r);
 
-#ifdef FOUR_SWEEP
-static int g_splits = 0, g_cluster = 0;
-#endif
-
 static AttendPlan plan_attend(const xnor_b200_kv4_cache & c, const xnor_b200_kv4_rows & r, int heads, int window)
 {
 	AttendPlan a;
@@ -45,9 +41,6 @@ static AttendPlan plan_attend(const xnor_b200_kv4_cache & c, const xnor_b200_kv4
 	}
 	if (splits > FJ_SPLITS) { splits = FJ_SPLITS; }
 	a.cluster = splits <= 8;
-#ifdef FOUR_SWEEP
-	if (g_splits) { splits = g_splits; a.cluster = g_cluster != 0; }
-#endif
 	a.splits = (int)splits;
 	return a;
 }
@@ -120,7 +113,3 @@ extern "C" int xnor_b200_kv4_attend(const xnor_b200_kv4_cache * cache, const xno
 		default: return launch_attend_bf16(p, plan, s);
 	}
 }
-
-#ifdef FOUR_SWEEP
-extern "C" __attribute__((visibility("default"))) void four_sweep(int splits, int cluster, int) { g_splits = splits; g_cluster = cluster; }
-#endif

@@ -2,18 +2,24 @@
 //
 //   out = sum_j softmax_j(scale * q . k_j) v_j over the positions j that the token sees, its own and those before it (the last `window`)
 //
-// Bound by the cache's way from memory: every row is read once, for all heads of queries that share it.  A query (head, token) is a
-// column; a warp takes 16 positions at a time, its columns eight by eight, and both products run on the tensor cores with the codes as
-// they lie (four_common.cuh):
+// Every row of the cache is read once for all heads of queries that share it.  A query (head, token) is a column; a warp takes two steps of 16
+// positions at a time, its columns eight by eight, and both products run on the tensor cores with the codes as they lie (four_common.cuh):
 //   scores  [16 positions x 8 columns] = codes of k . q         then  scale_k * that + low_k * sum(q), group by group
-//   out     [16 channels x 8 columns] += codes of v . (p * scale_v), and sum(p * low_v) beside it in fp32
-// q and p * scale_v are fp16 next to powers of two of their own (q: of the column; scale_v: of the largest so far), fp32 and fp16 calls
+//   out     [16 channels x 8 columns] += (codes of v - 8) . (p * scale_v), and sum(p * (low_v + 8 * scale_v)) beside it in fp32
+// (around the middle code, or long flat sums would be lost in what the tensor cores cut off: 131072 positions by one CTA came out 5% off).
+// q and p * scale_v are fp16 next to powers of two of their own (q: of the column; scale_v: of the largest so far); fp32 and fp16 calls
 // split p * scale_v into two parts, fp32 calls q too.  The running maximum moves only when a score passes it by more than 2^8, so most
 // steps neither exchange it nor rescale.
 //
-// A CTA has four warps that share a run of positions, step by step, each with a ring of its own; then their sums meet in shared memory.
+// A CTA has four warps that share a run of positions, two steps by two, each with a ring of its own; then their sums meet in shared memory.
 // Long sequences are split over CTAs: up to eight of them are a cluster and meet in its shared memory, more leave their sums in the
 // scratch buffer and a second kernel joins them.  Everything is summed in a fixed order.
+//
+// What bounds it: issue slots.  32 positions of 128 channels in one group take some 590 instructions of a warp for the 4.4 KB they come
+// in, 176 of them the masks and shifts of the codes (on a pipe of half the rate); one sequence of 131072 tokens, 8 heads of keys and 64 of
+// queries, is read at 4.9 TB/s once it runs, 3.5 TB/s from launch to end (40 us; the copy rate is 6.5 TB/s).  Before and after its steps
+// a CTA costs 1000 instructions a warp: calls of few positions are that and a chain of four loads (lengths, table, codes, sums): 6 us.
+// Tried and slower: five CTAs on an SM (96 registers: 50 against 45 us), three stages (52).
 #pragma once
 
 #include <cooperative_groups.h>

@@ -1,13 +1,18 @@
 // Products of a few rows with a 4-bit matrix: out[r][i] = act( sum_j x[r][j] * (low[i][j/g] + scale[i][j/g] * code[i][j]) + bias[i] ).
 //
-// forward_connected_layer of Darknet (src-lib/connected_layer.cpp) with packed weights, one to some sixteen rows.  Bound by the codes'
-// way from memory.  A group's sum is scale * sum(x * code) + low * sum(x): the codes go into the tensor cores as they lie
-// (four_common.cuh), a warp owning 16 filters, and scale and low come in once a group.  x is converted once a block of 256 neighbours, to
-// fp16 next to a power of two of the block's own (fp32: to two fp16 parts, multiplied one after the other), which loses nothing of a
-// 16-bit x.
+// forward_connected_layer of Darknet (src-lib/connected_layer.cpp) with packed weights, one to some sixteen rows.  A group's sum is
+// scale * sum(x * code) + low * sum(x): the codes go into the tensor cores as they lie (four_common.cuh), and scale and low come in once a
+// group.  x is converted once a block of 256 neighbours, to fp16 next to a power of two of the block's own (fp32: to two fp16 parts,
+// multiplied one after the other), which loses nothing of a 16-bit x.
 //
-// A CTA has four warps, 64 filters, and a slice of the neighbours; each warp copies its own codes into a ring of its own, so warps wait
-// for nobody.  The slices of the same filters are a cluster: their sums meet in shared memory, in a fixed order, so results do not vary.
+// A CTA has eight warps of 16 or 32 filters and a slice of the neighbours; each warp copies its own codes into a ring of its own, so that
+// only the conversion of x, a turn ahead, is waited for.  The slices of the same filters are a cluster: their sums meet in shared memory, in
+// a fixed order, so results do not vary.
+//
+// What bounds it: one row of 16384 x 16384 runs at 4.3 TB/s (33 us; the copy rate is 6.5 TB/s) with issue slots half full, 16 rows of bf16
+// at 3.1 (46 us): the tensor pipe 38% busy, clusters of four on 132 of 148 SMs, the barrier of a block.  Tried and slower by 16 rows: seven
+// warps, whose 74 clusters do not fit at a time (66 us), barriers every other block with twice the room for x (52).  Up to 4096 x 4096
+// (8 MB from the L2, 5 us) it is a chain of latencies: launch, x, codes, the cluster's sums.
 #include <cooperative_groups.h>
 
 #include <climits>
@@ -390,17 +395,10 @@ four_product_kernel(const ProductParams p)
 	cluster.sync();                                                                   // nobody leaves while its sums are read
 }
 
-#ifdef FOUR_SWEEP
-static int g_ranks = 0, g_steps = 0, g_shape = 0;
-#endif
-
 // Large products of many rows: every CTA would convert all of x again, a fifth of its work (16384 x 16384 by 16 rows of bf16: 55 us, 46 with
 // a kernel for that; fp32 rows, whose parts are twice as much to copy, gain nothing: 8192 x 8192 by 12 rows 38 against 26).
 static bool wants_ready(int n, int k, int dtype, int rows)
 {
-#ifdef FOUR_SWEEP
-	if (g_shape) { return g_shape >= 5; }
-#endif
 	return rows > 8 && dtype != XNOR_B200_F32 && (long long)n * k >= (1LL << 27);
 }
 
@@ -425,10 +423,6 @@ static int launch_product(ProductParams & p, void * scratch, cudaStream_t stream
 		}
 	}
 	p.steps = MT == 2 ? 2 : 3;
-#ifdef FOUR_SWEEP
-	if (g_ranks) { ranks = g_ranks; }
-	if (g_steps && !READY) { p.steps = g_steps; }
-#endif
 	p.slice = (blocks + ranks - 1) / ranks;
 	if (p.slice < p.steps) { p.steps = 2; }
 	const size_t smem = S::smem(p.rows < S::ROWS ? p.rows : S::ROWS, p.steps);
@@ -447,10 +441,6 @@ static int launch_product(ProductParams & p, void * scratch, cudaStream_t stream
 template <class T, int NT, int GROUP>
 static int launch_product_shape(ProductParams & p, int dtype, void * scratch, cudaStream_t stream)
 {
-#ifdef FOUR_SWEEP
-	if (g_shape == 3) { return launch_product<T, NT, 2, 8, GROUP, false>(p, scratch, stream); }
-	if (g_shape == 4) { return launch_product<T, NT, 1, 8, GROUP, false>(p, scratch, stream); }
-#endif
 	if constexpr (sizeof(T) == 2)
 	{
 		if constexpr (NT == 2)
@@ -552,7 +542,3 @@ extern "C" int xnor_b200_w4_forward(const xnor_b200_w4_desc * d, const void * x,
 		default: return launch_product_rows<__nv_bfloat16>(p, dtype, d->group, scratch, s);
 	}
 }
-
-#ifdef FOUR_SWEEP
-extern "C" __attribute__((visibility("default"))) void four_sweep(int ranks, int steps, int shape) { g_ranks = ranks; g_steps = steps; g_shape = shape; }
-#endif

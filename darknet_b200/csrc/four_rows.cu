@@ -10,7 +10,8 @@
 // what a thread has to do rather than by memory, so: the minimum and the maximum of 16-bit values are taken in pairs; the scale is one
 // product and a check; the quotient is a product with 1/scale, whose nearest integer is the bits of its sum with 1.5 * 2^23, and the
 // remainder tells whether it is close to a half, where the division is done after all; what fp16 cannot hold and NaN show in the minimum
-// and the maximum.  4 x 2048 tokens of 8 heads of 128 fp16 channels, keys and values: 29 us with divisions and 8 neighbours a thread.
+// and the maximum.  4 x 2048 tokens (three quarters of them new) of 8 heads of 128 fp16 channels, keys and values: 16 us, 2.0 TB/s; 29 with
+// divisions and 8 neighbours a thread.  The other way 10 us, 3.3 TB/s.
 #include "four_common.cuh"
 
 namespace xnor

@@ -120,7 +120,7 @@ def test_attention_refuses(L):
     assert L.xnor_b200_kv4_attend_scratch_bytes(c, r, 3, 0) == 0
 
 
-def test_a_missing_binding_fails_loudly(monkeypatch):
+def test_a_missing_binding_fails_loudly(L, monkeypatch):
     import sys
     calls = F._Calls()
     monkeypatch.setitem(sys.modules, "darknet_b200._fourbit", None)
@@ -129,7 +129,7 @@ def test_a_missing_binding_fails_loudly(monkeypatch):
         calls.product
 
 
-def test_bindings_take_nothing_else():
+def test_bindings_take_nothing_else(L):
     from darknet_b200 import _fourbit
     t = torch.zeros(2, 2)
     for f in (_fourbit.product, _fourbit.append, _fourbit.read, _fourbit.attend):
@@ -139,7 +139,7 @@ def test_bindings_take_nothing_else():
             assert f((t, t, 2, 32), *[None] * (n - 1)) is None
 
 
-def test_tensors_off_the_gpu_are_refused():
+def test_tensors_off_the_gpu_are_refused(L):
     codes, scales = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, 2, dtype=torch.float16)
     m = F.Matrix4(codes, scales, 64, 32)
     with pytest.raises(ValueError, match="CUDA device"):
