@@ -620,6 +620,76 @@ def test_handles_keep_what_they_were_made_with():
             setattr(handle, name, getattr(handle, name))
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_a_whole_prompt(dtype):
+    """Hundreds of new tokens of ragged sequences at once, appended and attended to, with and without a window."""
+    s = Sequences([0, 330, 301, 300, 7, 640], 2, 64, 32, 48, seed=3)
+    counts = [0, 300, 300, 300, 7, 120]
+    n = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    table, lengths = s.device()
+    k, v = (torch.randn(6, 300, 2, 64, generator=rng(i)).to(dtype).cuda() for i in (1, 2))
+    F.append4(s.cache, k, v, table, lengths, n)
+    q = torch.randn(6, 300, 6, 64, generator=rng(3)).to(dtype).cuda()
+    check_attend(s, q, counts=counts)
+    check_attend(s, q, counts=counts, window=77)
+
+
+def test_a_graph_that_forks():
+    """Calls on two streams of one capture, each behind the other's: launches that overlap their predecessor wait for all they depend on."""
+    m = [matrix(256, 256, 64, i) for i in range(4)]
+    s = Sequences([900, 40], 2, 64, 32, 64, seed=2)
+    table, lengths = s.device()
+    x = torch.randn(2, 256, generator=rng(1)).half().cuda()
+    side = torch.cuda.Stream()
+
+    def work(fork):
+        a = F.forward_connected4(m[0], x)
+        if fork:
+            side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side if fork else torch.cuda.current_stream()):
+            b = F.attend4(s.cache, a.view(2, 1, 4, 64), table, lengths)
+            b = F.forward_connected4(m[1], b.view(2, 256))
+        c = F.forward_connected4(m[2], a * 0.5)
+        if fork:
+            torch.cuda.current_stream().wait_stream(side)
+        return F.forward_connected4(m[3], (b + c) * 0.01)
+
+    work(False)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work(True)
+    for i in range(20):
+        x.copy_(torch.randn(2, 256, generator=rng(i)))
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, work(False))
+
+
+def test_calls_behind_one_another_see_what_was_written():
+    """A long chain of short calls, each of which reads what the one before wrote, against the same calls one at a time."""
+    m = [matrix(192, 192, 32, i) for i in range(3)]
+    s = Sequences([64], 1, 64, 32, 16, seed=1)
+    table, lengths = s.device()
+
+    def chain(wait):
+        x = torch.randn(1, 192, generator=rng(7)).cuda()
+        for i in range(200):
+            x = F.forward_connected4(m[i % 3], x) * 0.05
+            kv = x[:, :128].view(1, 1, 2, 64)
+            F.append4(s.cache, kv[:, :, :1], kv[:, :, 1:], table, lengths)
+            k, v = F.read4(s.cache, table, lengths, 1)
+            a = F.attend4(s.cache, x[:, 128:].view(1, 1, 1, 64), table, lengths)
+            x = torch.cat((k.view(1, 64), v.view(1, 64), a.view(1, 64)), 1)
+            if wait:
+                torch.cuda.synchronize()
+        return x
+
+    want = chain(True)
+    for _ in range(3):
+        assert torch.equal(chain(False), want)
+
+
 def test_refusals_name_the_fault():
     m = matrix(8, 64, 32, 0)
     x = torch.zeros(2, 64, device="cuda")
