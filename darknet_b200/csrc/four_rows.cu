@@ -93,30 +93,31 @@ __device__ __forceinline__ uint2 quantize16(const Eight<T> & e0, const Eight<T> 
 	const float step = __half2float(s), by = step > 0.0f ? reciprocal(step) : 0.0f;
 	pair = __halves2half2(s, l);
 	// the bits of 1.5 * 2^23 + code are 0x4b400000 + code: times 16^i they add up to the word and a constant
+	//
+	// Next to a half the quotient (off by less than 2^-21 of what is below 16, with the difference's rounding) may have gone the wrong way.
+	// The remainder says so: the difference less what it lost in rounding, exactly; where it is a half the even code is the nearest.  A scale
+	// of 0 has no remainder.
 	uint32_t word[2] = {0u - 0x4b400000u * 0x11111111u, 0u - 0x4b400000u * 0x11111111u};
-	float furthest = 0.0f;
+	const float near = step * (0.5f - 0x1p-16f);
 	#pragma unroll
 	for (int i = 0; i < 16; ++i)
 	{
-		const float d = v[i] - base, t = fmaf(d, by, 12582912.0f), c = t - 12582912.0f;
-		furthest = fmaxf(furthest, fabsf(fmaf(-c, step, d)));
-		word[i / 8] += __float_as_uint(t) * (1u << (4 * (i % 8)));
-	}
-	// Next to a half the quotient (off by less than 2^-22 of what is below 16) may have gone the wrong way; the remainder, which is exact, says
-	// so, and where it is a half the even code is the nearest.  A scale of 0 has nothing further than 0.
-	if (there < 16 || furthest > step * (0.5f - 0x1p-17f))
-	{
-		const float half = 0.5f * step;
-		word[0] = word[1] = 0;
-		#pragma unroll
-		for (int i = 0; i < 16; ++i)
+		const float d = v[i] - base, t = fmaf(d, by, 12582912.0f), rest = fmaf(-(t - 12582912.0f), step, d);
+		uint32_t bits_of = __float_as_uint(t);
+		if (fabsf(rest) > near)
 		{
-			const float d = v[i] - base, t = fmaf(d, by, 12582912.0f), rest = fmaf(-(t - 12582912.0f), step, d);
-			uint32_t c = __float_as_uint(t) & 15;
-			c += rest > half || (rest == half && (c & 1)) ? 1 : 0;
-			c -= rest < -half || (rest == -half && (c & 1)) ? 1 : 0;
-			word[i / 8] |= (step > 0.0f && i < there ? c : 0) << (4 * (i % 8));
+			const float back = d - v[i], lost = (v[i] - (d - back)) - (base + back);                  // v - low = d + lost
+			const float over = (rest - 0.5f * step) + lost, under = (rest + 0.5f * step) + lost;
+			const bool odd = bits_of & 1;
+			bits_of += over > 0.0f || (over == 0.0f && odd) ? 1 : under < 0.0f || (under == 0.0f && odd) ? -1 : 0;
+			asm volatile("");                                     // (a branch that is hardly ever taken)
 		}
+		word[i / 8] += bits_of * (1u << (4 * (i % 8)));
+	}
+	if (there < 16)                                           // what is not there is 0
+	{
+		word[0] &= there >= 8 ? 0xffffffffu : (1u << (4 * max(there, 0))) - 1;
+		word[1] &= there <= 8 ? 0 : (1u << (4 * (there - 8))) - 1;
 	}
 	return make_uint2(word[0], word[1]);
 }
@@ -200,7 +201,7 @@ kv4_append_kernel(const RowsParams p)
 	uint2 * codes = (uint2 *)(half ? p.c.v_codes : p.c.k_codes);
 	__half2 * scales = (__half2 *)(half ? p.c.v_scales : p.c.k_scales);
 	const int all = p.words / 2;
-	#pragma unroll 2
+	#pragma unroll 1
 	for (int w0 = 0; w0 < all; w0 += k.step)
 	{
 		const int w = w0 + k.first, head = (int)__umulhi((uint32_t)w * 2, p.by_words), two = w - head * twos;

@@ -68,6 +68,40 @@ def test_weights_of_extreme_values():
     check_packed(R.unpack(m.codes.cpu().numpy(), 64), m.scales.cpu().numpy(), double(rows), 64)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_values_next_to_a_half_take_the_nearest_code(group):
+    """fp32 values a last bit beside the middle of two codes, whose difference from low has no room for that bit; and the middle itself, which
+    takes the even code.  low -1, scale 1/8."""
+    rows = torch.full((8, group), -1.0)
+    rows[:, 1] = 0.875
+    for i, half in enumerate((7.5, 8.5)):
+        middle = torch.tensor(-1.0 + half / 8)
+        for j, v in enumerate((middle, torch.nextafter(middle, torch.tensor(9.0)), torch.nextafter(middle, torch.tensor(-9.0)))):
+            rows[3 * i + j, 2:] = v
+    rows[6, 2:] = -1.0 + 0.5 / 8                             # (0: even)
+    rows[7, 2:] = torch.nextafter(torch.tensor(-1.0 + 14.5 / 8), torch.tensor(9.0))
+    m = F.quantize_weights4(rows.cuda(), group)
+    codes, scales = R.quantize(double(rows), group)
+    assert codes[:, 2].tolist() == [8, 8, 7, 8, 9, 8, 0, 15]
+    np.testing.assert_array_equal(R.unpack(m.codes.cpu().numpy(), group), codes)
+    np.testing.assert_array_equal(m.scales.cpu().numpy(), scales)
+    s = Sequences([8], 1, 128, group, 16)
+    table, lengths = s.device()
+    k = rows.repeat(1, 128 // group).view(1, 8, 1, 128).cuda()
+    F.append4(s.cache, k, -k, table, lengths)
+    got, _ = F.read4(s.cache, table, lengths, 8)
+    assert torch.equal(got.view(8, 128)[:, :group].cpu(), torch.from_numpy(-1.0 + codes / 8).float())
+
+
+def test_random_codes_are_the_definitions_all_of_them():
+    """Two million values: some of any such number lie next to a half."""
+    rows = torch.randn(4096, 512, generator=rng(12))
+    m = F.quantize_weights4(rows.cuda(), 64)
+    codes, scales = R.quantize(double(rows), 64)
+    np.testing.assert_array_equal(m.scales.cpu().numpy(), scales)
+    np.testing.assert_array_equal(R.unpack(m.codes.cpu().numpy(), 512), codes)
+
+
 @pytest.mark.parametrize("offset, pad", [(0, 0), (1, 3), (3, 8)])
 def test_weights_with_strides(offset, pad):
     whole = torch.randn(6, 77 + pad + offset, generator=rng(4), dtype=torch.float32).half().cuda()
