@@ -69,9 +69,9 @@ __device__ __forceinline__ int seen_from(int window, int at) { return window > 0
 __device__ __forceinline__ Span span_of(const AttendParams & p, int b, int i0, int i1)
 {
 	Span s;
-	const int count = p.r.counts != nullptr ? max(__ldg(p.r.counts + b), 0) : p.r.tokens;
+	const int count = p.r.counts != nullptr ? max(p.r.counts[b], 0) : p.r.tokens;
 	s.count = min(count, p.r.tokens);
-	const int length = max(__ldg(p.r.lengths + b), 0);
+	const int length = max(p.r.lengths[b], 0);
 	s.at = length - count;
 	s.end = min(length, p.room);
 	i1 = min(i1, s.count - 1);
@@ -257,8 +257,8 @@ four_attend_kernel(const AttendParams p)
 	int next_id[2];
 	auto look_up = [&]()
 	{
-		next_id[0] = next < end ? __ldg(table + next_page) : -1;
-		next_id[1] = next + 1 < end ? __ldg(table + next_page + (next_sub + 1 >= page_steps)) : -1;
+		next_id[0] = next < end ? table[next_page] : -1;
+		next_id[1] = next + 1 < end ? table[next_page + (next_sub + 1 >= page_steps)] : -1;
 	};
 	// what a lane copies of a step: COPIES times 16 bytes of keys' and of values' codes, and of the scales (keys' first, then values')
 	constexpr int COPIES = (NB + 1) / 2, STEP_CODES = 8 * DIM, STEP_SCALES = 64 * GROUPS;       // bytes of a step in memory

@@ -40,6 +40,8 @@ inline size_t four_size(int t) { return t == XNOR_B200_F32 ? 4 : 2; }
 
 // Every kernel of a call but the load-time ones starts with pdl_wait() and pdl_trigger() and is launched through this: its CTAs take their
 // places while the kernel in front of it on the stream finishes, and do nothing before it has.  A decoding step is a chain of such kernels.
+// So what a call reads may still be written while its kernels are there already: they read it by ordinary loads, not by those (__ldg, a
+// __restrict__ pointer) that are for memory which nobody writes as long as the kernel lives.
 // cluster: CTAs of a cluster, along x.
 template <class Kernel, class... Args>
 int launch_four(Kernel kernel, dim3 grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t stream, const Args & ... args)
@@ -94,16 +96,16 @@ __device__ __forceinline__ Eight<T> load8(const T * p, int there, bool wide)
 	Eight<T> v;
 	if (wide && there >= 8)
 	{
-		v.raw[0] = __ldg(reinterpret_cast<const uint4 *>(p));
-		if (sizeof(T) == 4) { v.raw[sizeof(T) / 2 - 1] = __ldg(reinterpret_cast<const uint4 *>(p) + 1); }
+		v.raw[0] = reinterpret_cast<const uint4 *>(p)[0];
+		if (sizeof(T) == 4) { v.raw[sizeof(T) / 2 - 1] = reinterpret_cast<const uint4 *>(p)[1]; }
 		return v;
 	}
 	uint32_t * w = reinterpret_cast<uint32_t *>(v.raw);
 	#pragma unroll
 	for (int i = 0; i < 8; ++i)
 	{
-		if (sizeof(T) == 4) { w[i] = i < there ? __ldg(reinterpret_cast<const uint32_t *>(p) + i) : 0; continue; }
-		const uint32_t h = i < there ? __ldg(reinterpret_cast<const uint16_t *>(p) + i) : 0;
+		if (sizeof(T) == 4) { w[i] = i < there ? reinterpret_cast<const uint32_t *>(p)[i] : 0; continue; }
+		const uint32_t h = i < there ? reinterpret_cast<const uint16_t *>(p)[i] : 0;
 		if (i % 2 == 0) { w[i / 2] = h; }
 		else { w[i / 2] |= h << 16; }
 	}

@@ -388,7 +388,7 @@ four_product_kernel(const ProductParams p)
 		if (f >= S::FILTERS || filter >= p.n) { continue; }
 		float v = 0.0f;
 		for (int r = 0; r < ranks; ++r) { v += cluster.map_shared_rank(s_out, r)[row * PITCH + f]; }
-		if (p.biases != nullptr) { v += __ldg(p.biases + filter); }
+		if (p.biases != nullptr) { v += p.biases[filter]; }
 		if (p.leaky && !(v > 0.0f)) { v *= 0.1f; }
 		((T *)p.out)[(row0 + row) * p.ldo + filter] = from_f32<T>(v);
 	}

@@ -143,14 +143,14 @@ four_weights_kernel(const T * __restrict__ weights, long long ld, int k, int gro
 // The page and the place of row i of sequence b; page < 0: there is none.
 __device__ __forceinline__ void find_row(const xnor_b200_kv4_cache & c, const xnor_b200_kv4_rows & r, int b, int i, int & page, int & place)
 {
-	const int count = r.counts != nullptr ? __ldg(r.counts + b) : r.tokens;
-	const long long at = (long long)__ldg(r.lengths + b) - count + i;
+	const int count = r.counts != nullptr ? r.counts[b] : r.tokens;
+	const long long at = (long long)r.lengths[b] - count + i;
 	page = -1;
 	place = 0;
 	if (i >= count || at < 0 || at > 0x7fffffffLL) { return; }               // (a length is below 2^31)
 	const uint32_t of = (uint32_t)at / (uint32_t)c.page;
 	if (of >= (uint32_t)r.max_pages) { return; }
-	const int p = __ldg(r.table + (size_t)b * r.max_pages + of);
+	const int p = r.table[(size_t)b * r.max_pages + of];
 	if (p >= 0 && p < c.pages) { page = p; place = (int)((uint32_t)at - of * (uint32_t)c.page); }
 }
 
@@ -243,25 +243,38 @@ kv4_read_kernel(const RowsParams p)
 	const size_t row0 = (size_t)max(page, 0) * p.c.kv_heads * p.c.page + place;
 	const uint32_t * codes = (const uint32_t *)(half ? p.c.v_codes : p.c.k_codes);
 	const uint32_t * scales = (const uint32_t *)(half ? p.c.v_scales : p.c.k_scales);
-	#pragma unroll 4
-	for (int w = k.first; w < p.words; w += k.step)
+	// four words at a time, all loaded before the first is stored (the compiler does not move a load in front of a store)
+	constexpr int AHEAD = 4;
+	#pragma unroll 1
+	for (int w0 = k.first; w0 < p.words; w0 += AHEAD * k.step)
 	{
-		const int head = (int)__umulhi((uint32_t)w, p.by_words), word = w - head * words;
-		float v[8] = {};
-		if (page >= 0)
+		uint32_t c[AHEAD] = {}, pair[AHEAD] = {};
+		#pragma unroll
+		for (int j = 0; j < AHEAD; ++j)
 		{
+			const int w = w0 + j * k.step, head = (int)__umulhi((uint32_t)w, p.by_words), word = w - head * words;
+			if (page < 0 || w >= p.words) { continue; }
 			const size_t row = row0 + (size_t)head * p.c.page;
-			const uint32_t c = __ldg(codes + row * words + word), up = upper(c);
-			const float2 sl = halves(__ldg(scales + row * groups + (word >> shift)));
-			const float2 pairs[4] = {even_values(c), odd_values(c), even_values(up), odd_values(up)};       // 0 and 4, 1 and 5, 2 and 6, 3 and 7
+			c[j] = codes[row * words + word];
+			pair[j] = scales[row * groups + (word >> shift)];
+		}
+		#pragma unroll
+		for (int j = 0; j < AHEAD; ++j)
+		{
+			const int w = w0 + j * k.step, head = (int)__umulhi((uint32_t)w, p.by_words), word = w - head * words;
+			if (w >= p.words) { break; }
+			float v[8];
+			const uint32_t up = upper(c[j]);
+			const float2 sl = halves(pair[j]);
+			const float2 pairs[4] = {even_values(c[j]), odd_values(c[j]), even_values(up), odd_values(up)};     // 0 and 4, 1 and 5, 2 and 6, 3 and 7
 			#pragma unroll
 			for (int e = 0; e < 4; ++e)
 			{
 				v[e] = __fmaf_rn(sl.x, pairs[e].x, sl.y);
 				v[e + 4] = __fmaf_rn(sl.x, pairs[e].y, sl.y);
 			}
+			store8(dst + head * t.stride_head + 8 * word, p.wide[half] != 0, v);
 		}
-		store8(dst + head * t.stride_head + 8 * word, p.wide[half] != 0, v);
 	}
 }
 

@@ -29,3 +29,15 @@ def test_waits_for_tensor_memory_loads_hold_the_registers(path):
         text = re.sub(r"//[^\n]*", "", fh.read())
     for rest in text.split('"tcgen05.wait::ld')[1:]:
         assert re.match(r'[^"]*"\s*:\s*"\+r"', rest), rest[:120]
+
+
+@pytest.mark.parametrize("path", sorted(glob.glob(os.path.join(CSRC, "four_*"))), ids=os.path.basename)
+def test_kernels_launched_behind_one_another_read_by_ordinary_loads(path):
+    """Their CTAs are resident while the kernel in front still writes what they go on to read.  The non-coherent path (__ldg, ld.global.nc, what
+    the compiler makes of a const __restrict__ pointer) is for memory that is read-only for as long as the kernel lives."""
+    with open(path) as fh:
+        text = re.sub(r"//[^\n]*", "", fh.read())
+    assert "__ldg(" not in text and "ld.global.nc" not in text
+    for kernel in text.split("__global__")[1:]:
+        if "pdl_wait()" in kernel.split("__global__")[0]:
+            assert "__restrict__" not in kernel[:kernel.index("{")]
