@@ -346,10 +346,10 @@ four_attend_kernel(const AttendParams p)
 		}
 		#pragma unroll
 		for (int m = 1; m < GB * 4; m <<= 1) { part += __shfl_xor_sync(0xffffffffu, part, m); }
-		if (side < NB * 4 && side % (GB * 4) == 0) { s_qsum[side / (GB * 4) * COLS + c] = part * (1.0f / How::UNIT); }
+		if (side < NB * 4 && side % (GB * 4) == 0) { s_qsum[side / (GB * 4) * COLS + c] = part; }
 		if (side == 0)
 		{
-			s_qf[c] = inverse * (How::UNIT * p.scale_log2);
+			s_qf[c] = inverse * p.scale_log2;
 			s_to[c] = there ? min(span.end, span.at + i + 1) : 0;
 			s_from[c] = there ? seen_from(p.window, span.at + i) : 0;
 		}
@@ -451,6 +451,8 @@ four_attend_kernel(const AttendParams p)
 				float2 sl0 = halves(sk[h][0][gr]), sl1 = halves(sk[h][1][gr]);
 				sl0.y += How::SHIFT * sl0.x;
 				sl1.y += How::SHIFT * sl1.x;
+				sl0.x *= How::UNIT;
+				sl1.x *= How::UNIT;
 				#pragma unroll
 				for (int nt = 0; nt < NT; ++nt)
 				{

@@ -7,7 +7,8 @@
 // Codes reach the tensor cores as they are: the word masked with 0x000F000F is two fp16 subnormals, code 0 and code 4, each code * 2^-24
 // exactly; masked with 0x00F000F0 it is codes 1 and 5 times 2^-20; shifted down by eight the same masks give 2 and 6, 3 and 7.  So eight
 // codes cost five integer operations and no conversion, the products are exact, and their sums are fp32.  The other operand pairs the
-// same neighbours, the odd ones divided by 16, and the factor 2^24 goes into the group's scale.
+// same neighbours, the odd ones divided by 16, and the factor 2^24 goes into the group's scale (not into the power of two of the other
+// operand's values: times 2^24 that passes fp32's range where they are 2^117 and more).
 //
 // fp32 calls take code - 8 instead, as value = (low + 8 * scale) + scale * (code - 8): the sums of a group's two terms, which rounding
 // (and the tensor cores' cutting off) is relative to, then hardly cancel.  1024 + code in fp16 is the same mask with the exponent's bits

@@ -101,7 +101,7 @@ __device__ __forceinline__ void convert_row(const Eight<T> & raw, unsigned char 
 	if (lane % (GROUP / 8) == 0) { sums[(xb * GROUPS + lane / (GROUP / 8)) * ROWS + row] = part; }
 	float factor, inverse;
 	fit_f16(largest, factor, inverse);
-	if (lane == 0) { inverses[xb * ROWS + row] = inverse * How::UNIT; }
+	if (lane == 0) { inverses[xb * ROWS + row] = inverse; }
 	// (what is not finite makes its own column of the products NaN, and the inverse does so anyway)
 	float high[8], rest[8];
 	const float odd_factor = factor * How::ODD;
@@ -332,6 +332,8 @@ four_product_kernel(const ProductParams p)
 					float2 sl0 = halves(pairs[mt * 16 * S::SCALE_PITCH + q]), sl1 = halves(pairs[(mt * 16 + 8) * S::SCALE_PITCH + q]);
 					sl0.y += How::SHIFT * sl0.x;
 					sl1.y += How::SHIFT * sl1.x;
+					sl0.x *= How::UNIT;
+					sl1.x *= How::UNIT;
 					#pragma unroll
 					for (int nt = 0; nt < NT; ++nt)
 					{

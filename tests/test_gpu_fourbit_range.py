@@ -1,0 +1,55 @@
+"""Four-bit operators at the ends of their types' ranges, and where scales and codes are far from even."""
+import math
+
+import numpy as np
+import pytest
+
+import four_reference as R
+from test_gpu_fourbit import Sequences, TYPES, check_product, double, ids, matrix, rng
+
+torch = pytest.importorskip("torch")
+
+from darknet_b200 import fourbit as F  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("n, k, group, rows", [(40, 300, 32, 1), (40, 300, 64, 5), (70, 1000, 128, 13), (8300, 16200, 128, 9)])
+def test_products_of_the_largest_rows(dtype, n, k, group, rows):
+    """Values of up to 2^127, neighbours of opposite signs, by weights of some 2^-13: what comes out is far inside the type's range."""
+    m = matrix(n, k, group, n)
+    m.scales.mul_(2.0 ** -13)
+    x = torch.rand(rows, k, generator=rng(k)).mul(2.0 ** 127).to(dtype).cuda()
+    x[:, 0] = 2.0 ** 127
+    x[:, 1::2] = -x[:, :k // 2 * 2:2]
+    y = F.forward_connected4(m, x)
+    assert torch.isfinite(y).all()
+    picked = torch.arange(0, n, max(1, n // 40)).cuda()
+    check_product(F.Matrix4(m.codes[picked].contiguous(), m.scales[picked].contiguous(), k, group), x, y[:, picked])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("share, dim, group", [(1, 64, 32), (5, 128, 128), (12, 96, 32)])
+def test_attention_of_the_largest_queries(dtype, share, dim, group):
+    """Queries of up to 2^126.  The keys of one position point along them and the others do not: that position is all there is.  Keys that are
+    all 0: the mean of the values."""
+    s = Sequences([70, 40], 1, dim, group, 16, seed=dim)
+    c = s.cache
+    q = (torch.rand(2, 1, share, dim, generator=rng(1)) + 0.5).mul(2.0 ** 125).to(dtype).cuda()
+    c.k_codes.zero_()
+    c.k_scales.zero_()
+    table, lengths = s.device()
+    every = [[(s.table[b][at // 16], at % 16) for at in range(s.lengths[b])] for b in range(2)]
+    _, _, v, v_scales = s.buffers()
+    held = [np.stack([R.values(v[p, 0, i], v_scales[p, 0, i], group, dim)[0] for p, i in places]) for places in every]
+    mean = double(F.attend4(c, q, table, lengths))
+    for b in range(2):
+        # 70 weights of 1: fp32 sums, and one rounding
+        assert (np.abs(mean[b, 0] - held[b].mean(0)) <= np.abs(held[b]).max() * 2.0 ** -8 * (1 if dtype == torch.bfloat16 else 2.0 ** -10)).all()
+    for b, at in ((0, 37), (1, 39)):
+        page, place = every[b][at]
+        c.k_scales[page, 0, place, :, 1] = 2.0 ** -20
+    one = double(F.attend4(c, q, table, lengths))
+    for b, at in ((0, 37), (1, 39)):
+        assert (np.abs(one[b, 0] - held[b][at]) <= np.abs(held[b][at]).max() * 2.0 ** -8 * (1 if dtype == torch.bfloat16 else 2.0 ** -10)).all()
