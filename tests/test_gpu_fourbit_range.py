@@ -53,3 +53,27 @@ def test_attention_of_the_largest_queries(dtype, share, dim, group):
     one = double(F.attend4(c, q, table, lengths))
     for b, at in ((0, 37), (1, 39)):
         assert (np.abs(one[b, 0] - held[b][at]) <= np.abs(held[b][at]).max() * 2.0 ** -8 * (1 if dtype == torch.bfloat16 else 2.0 ** -10)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("tokens, share, dim, group", [(1, 8, 64, 32), (1, 3, 128, 128), (5, 5, 128, 64), (1, 2, 256, 64)])
+def test_equal_values_average_to_themselves(dtype, tokens, share, dim, group):
+    """Whatever the weights are: every output is the type's value next to the values' own.  Errors: a weight times a scale as two fp16 parts
+    (2^-22), at most 40 positions' 2^-31 of the largest where fp16 runs out of bits, and fp32 sums of at most 32 links (2^-23 each) of
+    |low + 8 s| + s |code - 8|; a value that lies as near as that to the middle of two of the type's may go either way."""
+    s = Sequences([40, 9, 3], 2, dim, group, 16, seed=tokens + dim)
+    c = s.cache
+    for b in range(3):
+        pages = [p for p in s.table[b] if p >= 0]
+        c.v_codes[pages] = c.v_codes[pages[0], :, :1].clone()
+        c.v_scales[pages] = c.v_scales[pages[0], :, :1].clone()
+    q = torch.randn(3, tokens, 2 * share, dim, generator=rng(2)).to(dtype).cuda()
+    table, lengths = s.device()
+    got = F.attend4(c, q, table, lengths).cpu()
+    _, _, codes, scales = s.buffers()
+    for b in range(3):
+        v, size = (torch.from_numpy(x) for x in R.values(codes[s.table[b][0], :, 0], scales[s.table[b][0], :, 0], group, dim, 8))      # [head][dim]
+        tolerance = size * (2.0 ** -22 + 40 * 2.0 ** -31 + 32 * 2.0 ** -23)
+        low, high = ((v + way * tolerance).to(dtype).repeat_interleave(share, 0) for way in (-1, 1))
+        for row in got[b, max(0, tokens - s.lengths[b]):]:
+            assert ((row >= low) & (row <= high)).all()
