@@ -6,7 +6,7 @@
 // positions at a time, its columns eight by eight, and both products run on the tensor cores with the codes as they lie (four_common.cuh):
 //   scores  [16 positions x 8 columns] = codes of k . q         then  scale_k * that + low_k * sum(q), group by group
 //   out     [16 channels x 8 columns] += (codes of v - 8) . (p * scale_v), and sum(p * (low_v + 8 * scale_v)) beside it in fp32
-// (around the middle code, or long flat sums would be lost in what the tensor cores cut off: 131072 positions by one CTA came out 5% off).
+// (around the middle code, so that the two hardly cancel).
 // q and p * scale_v are fp16 next to powers of two of their own (q: of the column; scale_v: of the largest so far); p * scale_v is two parts,
 // fp32 calls' q too.  The running maximum moves only when a score passes it by more than 2^8, so most
 // steps neither exchange it nor rescale.
@@ -624,36 +624,70 @@ four_attend_kernel(const AttendParams p)
 			}
 		}
 
-		// ---- values
+		// ---- values.  The tensor cores cut a sum off where fp32 rounds it, which adds up over a long run (60000 positions of codes 2 to 4: 3e-6
+		// of what goes into the sums, and half a percent of the results): the products of 32 positions go into sums that start at 0, and those
+		// are added to the others by fp32 additions.
 		#pragma unroll
 		for (int gr = 0; gr < GROUPS; ++gr)
 		{
+			uint32_t pv[2][NT][PP][2];
 			#pragma unroll
 			for (int h = 0; h < 2; ++h)
 			{
-				uint32_t pv[NT][PP][2];
-				if (wild) { weigh<true, NT, PP>(pv, lows[gr], s[h], sv[h][0][gr], sv[h][1][gr], unit); }
-				else { weigh<false, NT, PP>(pv, lows[gr], s[h], sv[h][0][gr], sv[h][1][gr], unit); }
-				uint32_t w[4][GB];
+				if (wild) { weigh<true, NT, PP>(pv[h], lows[gr], s[h], sv[h][0][gr], sv[h][1][gr], unit); }
+				else { weigh<false, NT, PP>(pv[h], lows[gr], s[h], sv[h][0][gr], sv[h][1][gr], unit); }
+			}
+			constexpr int WORDS = GB == 4 ? 1 : GB;               // of a row at a time (131072 positions: 47.4 us, with all four, that spill, 49)
+			#pragma unroll
+			for (int j0 = 0; j0 < GB; j0 += WORDS)
+			{
+				uint32_t w[2][4][WORDS];
 				#pragma unroll
-				for (int i = 0; i < 4; ++i)
+				for (int h = 0; h < 2; ++h)
 				{
-					load_words<GB>(w[i], at + S::V_AT + (h * 16 + i / 2 * 8 + i % 2 + 2 * t) * S::V_PITCH + gr * 16 * GB + (g & 3) * 4 * GB);
+					#pragma unroll
+					for (int i = 0; i < 4; ++i)
+					{
+						load_words<WORDS>(w[h][i], at + S::V_AT + (h * 16 + i / 2 * 8 + i % 2 + 2 * t) * S::V_PITCH + gr * 16 * GB + (g & 3) * 4 * GB + j0 * 4);
+					}
 				}
 				#pragma unroll
-				for (int j = 0; j < GB; ++j)
+				for (int j = 0; j < WORDS; ++j)
 				{
-					const uint32_t x = __byte_perm(w[0][j], w[1][j], pick), y = __byte_perm(w[2][j], w[3][j], pick), x_up = upper(x), y_up = upper(y);
-					const uint32_t even[4] = {even_codes<true>(x), even_codes<true>(x_up), even_codes<true>(y), even_codes<true>(y_up)};
-					const uint32_t odd[4] = {odd_codes<true>(x), odd_codes<true>(x_up), odd_codes<true>(y), odd_codes<true>(y_up)};
+					float of_step[2][NT][4];                      // [even, odd channels]
+					#pragma unroll
+					for (int h = 0; h < 2; ++h)
+					{
+						const uint32_t x = __byte_perm(w[h][0][j], w[h][1][j], pick), y = __byte_perm(w[h][2][j], w[h][3][j], pick), x_up = upper(x), y_up = upper(y);
+						const uint32_t even[4] = {even_codes<true>(x), even_codes<true>(x_up), even_codes<true>(y), even_codes<true>(y_up)};
+						const uint32_t odd[4] = {odd_codes<true>(x), odd_codes<true>(x_up), odd_codes<true>(y), odd_codes<true>(y_up)};
+						#pragma unroll
+						for (int nt = 0; nt < NT; ++nt)
+						{
+							#pragma unroll
+							for (int part = 0; part < PP; ++part)
+							{
+								if (h + part == 0)
+								{
+									mma_16816_first(of_step[0][nt], even, pv[h][nt][part][0], pv[h][nt][part][1]);
+									mma_16816_first(of_step[1][nt], odd, pv[h][nt][part][0], pv[h][nt][part][1]);
+								}
+								else
+								{
+									mma_16816(of_step[0][nt], even, pv[h][nt][part][0], pv[h][nt][part][1]);
+									mma_16816(of_step[1][nt], odd, pv[h][nt][part][0], pv[h][nt][part][1]);
+								}
+							}
+						}
+					}
 					#pragma unroll
 					for (int nt = 0; nt < NT; ++nt)
 					{
 						#pragma unroll
-						for (int part = 0; part < PP; ++part)
+						for (int e = 0; e < 4; ++e)
 						{
-							mma_16816(o[gr][j][0][nt], even, pv[nt][part][0], pv[nt][part][1]);
-							mma_16816(o[gr][j][1][nt], odd, pv[nt][part][0], pv[nt][part][1]);
+							o[gr][j0 + j][0][nt][e] += of_step[0][nt][e];
+							o[gr][j0 + j][1][nt][e] += of_step[1][nt][e];
 						}
 					}
 				}

@@ -77,3 +77,33 @@ def test_equal_values_average_to_themselves(dtype, tokens, share, dim, group):
         low, high = ((v + way * tolerance).to(dtype).repeat_interleave(share, 0) for way in (-1, 1))
         for row in got[b, max(0, tokens - s.lengths[b]):]:
             assert ((row >= low) & (row <= high)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("dim, group, share", [(32, 32, 1), (128, 128, 1), (128, 64, 20), (256, 128, 2)])
+def test_long_sums_of_codes_far_from_the_middle(dtype, dim, group, share):
+    """60000 positions by one CTA, all of weight 1 (the queries are 0), codes 2 to 4 with low = -3 * scale, as a group has them whose other
+    channels are loud: sums around code 8 that come to five scales a position, of which the result is a thousandth.
+
+    Errors: weights and scales are exact.  An fp32 sum that grows evenly to S in n additions is off by at most 2^-23 / sqrt(12) * S * sqrt(n / 3)
+    (one standard deviation; every addition rounds to nearest), n = 60000 / 32 / 4 additions of a warp, four of which are averaged: six
+    deviations are 1.3e-6 S, below 2^-19 of |low + 8 s| + s |code - 8|.  The sums of low have four times the additions in each of 8 lanes of
+    a warp, which is less.  One rounding of the result."""
+    batch, kv_heads = 160, 4
+    s = Sequences([60000], kv_heads, dim, group, 256, seed=1)
+    c = s.cache
+    even, odd = (torch.randint(2, 5, c.v_codes.shape, generator=rng(i), dtype=torch.uint8) for i in (1, 2))
+    c.v_codes.copy_((even | odd << 4).cuda())
+    c.v_scales[..., 1] = -3 * c.v_scales[..., 0]
+    table, lengths = s.device()
+    q = torch.zeros(batch, 1, kv_heads * share, dim, dtype=dtype, device="cuda")
+    got = F.attend4(c, q, table.expand(batch, -1).contiguous(), lengths.expand(batch).contiguous())
+    assert (got == got[:1]).all()
+    got = double(got[0, 0]).reshape(kv_heads, share, dim)
+    codes, scales = (t[torch.tensor(s.table[0]).cuda()].transpose(0, 1).flatten(1, 2)[:, :60000].cpu().numpy() for t in (c.v_codes, c.v_scales))
+    for h in range(kv_heads):
+        v, size = R.values(codes[h], scales[h], group, dim, 8)
+        want, bound = v.mean(0), size.mean(0) * 2.0 ** -19
+        off = np.abs(got[h] - want)
+        tolerance = bound + np.abs(want) * R.HALF_STEP[dtype] * 1.001 + 2.0 ** -25 * (dtype == torch.float16)
+        assert (off <= tolerance).all(), (off / tolerance).max()
