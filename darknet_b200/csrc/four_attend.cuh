@@ -7,9 +7,9 @@
 //   scores  [16 positions x 8 columns] = codes of k . q         then  scale_k * that + low_k * sum(q), group by group
 //   out     [16 channels x 8 columns] += (codes of v - 8) . (p * scale_v), and sum(p * (low_v + 8 * scale_v)) beside it in fp32
 // (around the middle code, so that the two hardly cancel).
-// q and p * scale_v are fp16 next to powers of two of their own (q: of the column; scale_v: of the largest so far); p * scale_v is two parts,
-// fp32 calls' q too.  The running maximum moves only when a score passes it by more than 2^8, so most
-// steps neither exchange it nor rescale.
+// q and p * scale_v are fp16 next to powers of two of their own (q: of the column; p * scale_v: of the largest of the column and the group so
+// far); p * scale_v is two parts, fp32 calls' q too.  The running maximum moves only when a score passes it by more than 2^8 (as others do
+// it), so most steps neither exchange it nor rescale.
 //
 // A CTA has four warps that share a run of positions, two steps by two, each with a ring of its own; then their sums meet in shared memory.
 // Long sequences are split over CTAs: up to eight of them are a cluster and meet in its shared memory, more leave their sums in the
@@ -36,6 +36,7 @@ namespace cg = cooperative_groups;
 constexpr int FA_WARPS = 4, FA_THREADS = 32 * FA_WARPS;
 constexpr int FA_STAGES = 2;
 constexpr float FA_SLACK = 8.0f;                          // how far (log2) a score may pass the running maximum
+constexpr int FA_MOST_UNIT = 127 + 64, FA_MOST_P = 15;     // of p * scale_v: the largest unit's exponent, and log2 of the largest product in it
 
 struct AttendParams
 {
@@ -154,7 +155,7 @@ struct AttendShape
 	static constexpr int K_PITCH = (GROUPS | 1) * 16 * GB, V_PITCH = (NB | 1) * 16, Q_PITCH = (NB | 1) * 64;
 	static constexpr int V_AT = 32 * K_PITCH, PAIRS_AT = V_AT + 32 * V_PITCH, STAGE = PAIRS_AT + 2 * 32 * GROUPS * 4;
 	static constexpr int U_PITCH = NB * 32 + 4, WARP = FA_STAGES * STAGE > COLS * U_PITCH * 4 ? FA_STAGES * STAGE : COLS * U_PITCH * 4;
-	static constexpr size_t SMEM = (size_t)FA_WARPS * WARP + QP * COLS * Q_PITCH + COLS * (4 + GROUPS * 4 + 8 + FA_WARPS * 12 + 8);
+	static constexpr size_t SMEM = (size_t)FA_WARPS * WARP + QP * COLS * Q_PITCH + COLS * (4 + GROUPS * 4 + 8 + FA_WARPS * 8 + (GROUPS == 1 ? FA_WARPS * 4 + 8 : FA_WARPS * GROUPS * 4));
 };
 
 template <int W>
@@ -190,31 +191,76 @@ __device__ __forceinline__ void load_pairs(uint32_t (&w)[GROUPS], const uint32_t
 	}
 }
 
-// Weights of 16 positions with the scales of a group: operands of the product with the codes, and the sums of weight * low.  WILD: a
-// weight of 0 counts as nothing, whatever the scale (a branch that is hardly ever taken costs less than selecting every time).
+// Weights of 16 positions times the scales of a group, in the columns' units: operands of the product with the codes; `most`: the largest of
+// them.  WILD: a weight of 0 counts as nothing, whatever the scale (a branch that is hardly ever taken costs less than selecting every time).
 template <bool WILD, int NT, int PP>
-__device__ __forceinline__ void weigh(uint32_t (&pv)[NT][PP][2], float (&lows)[NT][2], const float (&w)[NT][4], uint32_t pair0, uint32_t pair1, float unit)
+__device__ __forceinline__ void weigh(uint32_t (&pv)[NT][PP][2], const float (&w)[NT][4], uint32_t pair0, uint32_t pair1, const float2 (&unit)[NT], __half2 & most)
 {
 	#pragma unroll
 	for (int r = 0; r < 2; ++r)
 	{
-		float2 sl = halves(r == 0 ? pair0 : pair1);
-		sl.y += 8.0f * sl.x;
-		sl.x *= unit;
+		const float scale = halves(r == 0 ? pair0 : pair1).x;
 		#pragma unroll
 		for (int nt = 0; nt < NT; ++nt)
 		{
 			const float wx = w[nt][2 * r], wy = w[nt][2 * r + 1];
-			const float x = WILD && wx == 0.0f ? 0.0f : wx * sl.x, y = WILD && wy == 0.0f ? 0.0f : wy * sl.x;
-			lows[nt][0] = WILD && wx == 0.0f ? lows[nt][0] : lows[nt][0] + wx * sl.y;
-			lows[nt][1] = WILD && wy == 0.0f ? lows[nt][1] : lows[nt][1] + wy * sl.y;
+			const float x = WILD && wx == 0.0f ? 0.0f : wx * unit[nt].x * scale, y = WILD && wy == 0.0f ? 0.0f : wy * unit[nt].y * scale;
 			const uint32_t high = pair_f16(x, y);
+			most = __hmax2(most, __habs2(as_half2(high)));
 			pv[nt][0][r] = transposed(high);
 			if (PP == 2)
 			{
 				const float2 back = halves(high);
 				pv[nt][PP - 1][r] = transposed(pair_f16(x - back.x, y - back.y));
 			}
+		}
+	}
+}
+
+// The largest |weight * scale| of 32 positions, of this lane's two columns, to 8 bits.  What is not finite makes sums that are not, in any unit:
+// it does not take the others' bits away.
+template <int GROUPS>
+__device__ __forceinline__ float2 most_of(const float (&w)[2][4], const uint32_t (&pairs)[2][2][GROUPS], int group)
+{
+	float most[2] = {0.0f, 0.0f};
+	#pragma unroll
+	for (int i = 0; i < 8; ++i)
+	{
+		const float v = fabsf(w[i / 4][i % 4] * halves(pairs[i / 4][i / 2 % 2][group]).x);
+		most[i & 1] = v < INFINITY ? fmaxf(most[i & 1], v) : most[i & 1];
+	}
+	__nv_bfloat162 both = __floats2bfloat162_rn(most[0], most[1]);
+	#pragma unroll
+	for (int m = 4; m < 32; m <<= 1) { both = __hmax2(both, __shfl_xor_sync(0xffffffffu, both, m)); }
+	return __bfloat1622float2(both);
+}
+
+// Powers of two are handled by their exponents' bits (127: 1).
+__device__ __forceinline__ int exponent_of(float v) { return (int)(__float_as_uint(v) >> 23); }
+__device__ __forceinline__ float power_of(int exponent) { return exponent > 0 ? __uint_as_float((uint32_t)exponent << 23) : 0.0f; }
+
+// The exponent of the unit that brings `most` to [2^6, 2^7), where that of `unit` would bring it to FA_MOST_P or more.
+__device__ __forceinline__ int unit_for(float most, int unit)
+{
+	const int e = exponent_of(most);
+	return e + unit >= 2 * 127 + FA_MOST_P ? 2 * 127 + 6 - e : unit;
+}
+
+// The sums of weight * (value of code 8) of 16 positions.
+template <bool WILD, int NT>
+__device__ __forceinline__ void weigh_lows(float (&lows)[NT][2], const float (&w)[NT][4], uint32_t pair0, uint32_t pair1)
+{
+	#pragma unroll
+	for (int r = 0; r < 2; ++r)
+	{
+		const float2 sl = halves(r == 0 ? pair0 : pair1);
+		const float middle = sl.y + 8.0f * sl.x;
+		#pragma unroll
+		for (int nt = 0; nt < NT; ++nt)
+		{
+			const float wx = w[nt][2 * r], wy = w[nt][2 * r + 1];
+			lows[nt][0] = WILD && wx == 0.0f ? lows[nt][0] : lows[nt][0] + wx * middle;
+			lows[nt][1] = WILD && wy == 0.0f ? lows[nt][1] : lows[nt][1] + wy * middle;
 		}
 	}
 }
@@ -240,6 +286,7 @@ four_attend_kernel(const AttendParams p)
 	float * s_m = (float *)(s_to + COLS);                                             // [warp][column]
 	float * s_l = s_m + FA_WARPS * COLS, * s_by = s_l + FA_WARPS * COLS;
 	float * s_top = s_by + FA_WARPS * COLS, * s_all = s_top + COLS;                   // [column]
+	float * s_unit = s_by + warp * GROUPS * COLS;             // [group][column], of each warp; in the room of the last three, which come when all are through
 
 	pdl_wait();
 
@@ -383,8 +430,10 @@ four_attend_kernel(const AttendParams p)
 	float base[NT][2] = {}, limit[NT][2], total[NT][2] = {};
 	#pragma unroll
 	for (int nt = 0; nt < NT; ++nt) { limit[nt][0] = limit[nt][1] = -INFINITY; }
-	uint32_t unit_top = 0;                                    // scales of values up to these fp16 bits fit
-	float unit = 1.0f;                                        // what p * scale_v is multiplied by: a power of two
+	// What p * scale_v of a group and column is multiplied by: brings the largest of those that count to 2^6 and more, so that what fp16 then
+	// cuts off of any is 2^-31 of it.  No weight or scale has a say in a unit but those of the column and the group.
+	for (int i = lane; i < GROUPS * COLS; i += 32) { s_unit[i] = power_of(FA_MOST_UNIT); }
+	__syncwarp();
 	const uint32_t pick = g < 4 ? 0x5410u : 0x7632u;          // the half of a word that holds this lane's channels
 
 	int stage = 0;
@@ -522,9 +571,8 @@ four_attend_kernel(const AttendParams p)
 			wild = __any_sync(0xffffffffu, wild);
 		}
 
-		// ---- the maximum, and the unit of the values' scales, where they have to move
+		// ---- the maximum, where it has to move
 		bool move = false;
-		__half2 widest = __habs2(as_half2(sv[0][0][0]));
 		#pragma unroll
 		for (int h = 0; h < 2; ++h)
 		{
@@ -534,41 +582,13 @@ four_attend_kernel(const AttendParams p)
 				#pragma unroll
 				for (int e = 0; e < 4; ++e) { move |= !(s[h][nt][e] <= limit[nt][e & 1]); }           // (a NaN moves it, too)
 			}
-			#pragma unroll
-			for (int gr = 0; gr < GROUPS; ++gr)
-			{
-				#pragma unroll
-				for (int r = 0; r < 2; ++r) { widest = __hmax2(widest, __habs2(as_half2(sv[h][r][gr]))); }
-			}
 		}
-		move |= (as_word(widest) & 0xffffu) > unit_top;
 		if (__any_sync(0xffffffffu, move))
 		{
-			// a scale that is not finite makes sums that are not, in any unit: it does not take the others' bits away
-			uint32_t largest = 0;
-			#pragma unroll
-			for (int gr = 0; gr < GROUPS; ++gr)
-			{
-				#pragma unroll
-				for (int i = 0; i < 4; ++i)
-				{
-					const uint32_t bits = sv[i / 2][i % 2][gr] & 0x7fffu;
-					largest = max(largest, bits < 0x7c00u ? bits : 0);
-				}
-			}
-			largest = __reduce_max_sync(0xffffffffu, largest);
-			float rescale = 1.0f;
-			if (largest > unit_top)
-			{
-				const uint32_t e = __float_as_uint(__half2float(__ushort_as_half((unsigned short)largest))) >> 23;
-				const float now = __uint_as_float((260 - e) << 23);       // 2^(6 - (e - 127)): the largest scale comes to [2^6, 2^7)
-				rescale = unit_top == 0 ? 1.0f : now / unit;
-				unit = now;
-				unit_top = largest < 0x400u ? largest : largest | 0x3ffu; // all that share its exponent; subnormals: up to this one
-			}
 			#pragma unroll
 			for (int nt = 0; nt < NT; ++nt)
 			{
+				int back[2];                                      // what there is counts for 2^-back of what it did
 				#pragma unroll
 				for (int e = 0; e < 2; ++e)
 				{
@@ -585,27 +605,39 @@ four_attend_kernel(const AttendParams p)
 					m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
 					m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
 					// others may have moved theirs: a column's sums depend on its own scores alone
-					float keep = 1.0f;
+					back[e] = 0;
 					if (m > limit[nt][e])
 					{
-						keep = limit[nt][e] == -INFINITY ? 0.0f : exp2_fast(base[nt][e] - m);
+						m = ceilf(m);
+						back[e] = limit[nt][e] == -INFINITY ? 256 : (int)fminf(m - base[nt][e], 256.0f);
 						base[nt][e] = m;
 						limit[nt][e] = m + FA_SLACK;
 					}
-					total[nt][e] *= keep;
+				}
+				// A unit may grow as much, and the sum in it stays as it is; as far as these positions' weights let it.
+				float w[2][4];
+				#pragma unroll
+				for (int i = 0; i < 8; ++i) { w[i / 4][i % 4] = exp2_fast(s[i / 4][nt][i % 4] - base[nt][i & 1]); }
+				const float keep[2] = {power_of(127 - back[0]), power_of(127 - back[1])};
+				total[nt][0] *= keep[0];
+				total[nt][1] *= keep[1];
+				#pragma unroll
+				for (int gr = 0; gr < GROUPS; ++gr)
+				{
+					const float2 most = most_of(w, sv, gr);
+					float2 & unit = *(float2 *)(s_unit + gr * COLS + nt * 8 + t * 2);
+					const int was[2] = {exponent_of(unit.x), exponent_of(unit.y)};
+					const int now[2] = {unit_for(most.x, min(was[0] + back[0], FA_MOST_UNIT)), unit_for(most.y, min(was[1] + back[1], FA_MOST_UNIT))};
+					const float by[2] = {power_of(127 + now[0] - was[0] - back[0]), power_of(127 + now[1] - was[1] - back[1])};
+					__syncwarp();
+					unit = make_float2(power_of(now[0]), power_of(now[1]));       // (the same from the eight lanes of a column)
 					#pragma unroll
-					for (int gr = 0; gr < GROUPS; ++gr)
-					{
-						lows[gr][nt][e] *= keep;
-						#pragma unroll
-						for (int i = 0; i < GB * 2; ++i)
-						{
-							o[gr][i / 2][i % 2][nt][e] *= keep * rescale;
-							o[gr][i / 2][i % 2][nt][2 + e] *= keep * rescale;
-						}
-					}
+					for (int i = 0; i < GB * 8; ++i) { o[gr][i / 8][i / 4 % 2][nt][i % 4] *= by[i & 1]; }
+					lows[gr][nt][0] *= keep[0];
+					lows[gr][nt][1] *= keep[1];
 				}
 			}
+			__syncwarp();
 		}
 
 		// ---- weights: 0 for what is not seen
@@ -631,11 +663,45 @@ four_attend_kernel(const AttendParams p)
 		for (int gr = 0; gr < GROUPS; ++gr)
 		{
 			uint32_t pv[2][NT][PP][2];
+			{
+				float2 unit[NT];
+				#pragma unroll
+				for (int nt = 0; nt < NT; ++nt) { unit[nt] = *(const float2 *)(s_unit + gr * COLS + nt * 8 + t * 2); }
+				__half2 most = as_half2(0);
+				#pragma unroll
+				for (int h = 0; h < 2; ++h)
+				{
+					if (wild) { weigh<true, NT, PP>(pv[h], s[h], sv[h][0][gr], sv[h][1][gr], unit, most); }
+					else { weigh<false, NT, PP>(pv[h], s[h], sv[h][0][gr], sv[h][1][gr], unit, most); }
+				}
+				const bool over = __half2float(__hmax(__low2half(most), __high2half(most))) >= (float)(1 << FA_MOST_P);
+				if (__any_sync(0xffffffffu, over))
+				{
+					#pragma unroll
+					for (int nt = 0; nt < NT; ++nt)
+					{
+						float w[2][4];
+						#pragma unroll
+						for (int i = 0; i < 8; ++i) { w[i / 4][i % 4] = s[i / 4][nt][i % 4]; }
+						const float2 most = most_of(w, sv, gr);
+						const int was[2] = {exponent_of(unit[nt].x), exponent_of(unit[nt].y)}, now[2] = {unit_for(most.x, was[0]), unit_for(most.y, was[1])};
+						const float by[2] = {power_of(127 + now[0] - was[0]), power_of(127 + now[1] - was[1])};
+						unit[nt] = make_float2(power_of(now[0]), power_of(now[1]));
+						__syncwarp();
+						*(float2 *)(s_unit + gr * COLS + nt * 8 + t * 2) = unit[nt];
+						#pragma unroll
+						for (int i = 0; i < GB * 8; ++i) { o[gr][i / 8][i / 4 % 2][nt][i % 4] *= by[i & 1]; }
+					}
+					__syncwarp();
+					#pragma unroll
+					for (int h = 0; h < 2; ++h) { weigh<true, NT, PP>(pv[h], s[h], sv[h][0][gr], sv[h][1][gr], unit, most); }
+				}
+			}
 			#pragma unroll
 			for (int h = 0; h < 2; ++h)
 			{
-				if (wild) { weigh<true, NT, PP>(pv[h], lows[gr], s[h], sv[h][0][gr], sv[h][1][gr], unit); }
-				else { weigh<false, NT, PP>(pv[h], lows[gr], s[h], sv[h][0][gr], sv[h][1][gr], unit); }
+				if (wild) { weigh_lows<true, NT>(lows[gr], s[h], sv[h][0][gr], sv[h][1][gr]); }
+				else { weigh_lows<false, NT>(lows[gr], s[h], sv[h][0][gr], sv[h][1][gr]); }
 			}
 			constexpr int WORDS = GB == 4 ? 1 : GB;               // of a row at a time (131072 positions: 47.4 us, with all four, that spill, 49)
 			#pragma unroll
@@ -725,7 +791,7 @@ four_attend_kernel(const AttendParams p)
 				float low = lows[gr][nt][e];
 				#pragma unroll
 				for (int m = 4; m < 32; m <<= 1) { low += __shfl_xor_sync(0xffffffffu, low, m); }
-					const float by = 1.0f / unit;
+				const float by = power_of(2 * 127 - exponent_of(s_unit[gr * COLS + c]));
 				#pragma unroll
 				for (int j = 0; j < GB; ++j)
 				{

@@ -107,3 +107,55 @@ def test_long_sums_of_codes_far_from_the_middle(dtype, dim, group, share):
         off = np.abs(got[h] - want)
         tolerance = bound + np.abs(want) * R.HALF_STEP[dtype] * 1.001 + 2.0 ** -25 * (dtype == torch.float16)
         assert (off <= tolerance).all(), (off / tolerance).max()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("tokens, share, dim, group", [(1, 8, 64, 64), (1, 4, 128, 128), (2, 7, 128, 32), (5, 5, 128, 64), (1, 2, 256, 32)])
+def test_scales_that_do_not_count_take_no_bits(dtype, tokens, share, dim, group):
+    """Values whose scales differ by up to 2^36, from position to position and from group to group.  Even heads of queries see the large
+    ones with weights of 2^-100 and less, odd ones are all theirs.  Errors as for any other values, next to what the column itself sums."""
+    s = Sequences([90, 33, 300], 2, dim, group, 16, seed=dim)
+    c = s.cache
+    size = 2.0 ** torch.randint(-24, 13, c.v_scales.shape[:-1], generator=rng(1)).float()
+    loud = torch.rand(c.v_scales.shape[:3], generator=rng(2)) < 0.3
+    size = torch.where(loud[..., None], size, size.clamp(max=2.0 ** -12))
+    c.v_scales[..., 0] = (size * (1 + torch.rand(size.shape, generator=rng(3)))).half().cuda()
+    c.v_scales[..., 1] = -7 * c.v_scales[..., 0]
+    c.k_scales[..., 0] *= 0.01
+    c.k_scales[..., 1] = torch.where(loud[..., None], 1.0, 0.0).half().cuda()
+    q = torch.randn(3, tokens, 2 * share, dim, generator=rng(4))
+    q[:, :, 0::2] = -q[:, :, 0::2].abs() * 2000 / dim
+    q[:, :, 1::2] = q[:, :, 1::2].abs() * 2000 / dim
+    q = q.to(dtype).cuda()
+    table, lengths = s.device()
+    got = double(F.attend4(c, q, table, lengths, scale=0.1))
+    want, _, bound, score = R.attend(double(q), *s.buffers(), s.table, s.lengths, None, group, 0.1, 0, 8 if dtype == torch.float32 else 0)
+    assert score.max() < 600
+    # as check_attend has it: scores, weights (two parts: 2^-22), sums of at most 300 / 16 + 64 links, one rounding
+    weight = 2 * score * (2.0 ** -22 + 24 * 2.0 ** -23) + 2 * 2.0 ** -22 + 2.0 ** -20 + 83 * 2.0 ** -23
+    tolerance = bound * weight[..., None] * 1.01 + np.abs(want) * R.HALF_STEP[dtype] * 1.001 + 2.0 ** -25 * (dtype == torch.float16)
+    assert (np.abs(got - want) <= tolerance).all(), (np.abs(got - want) / tolerance).max()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("dim, group, share", [(32, 32, 3), (128, 64, 4), (256, 128, 1)])
+@pytest.mark.parametrize("far", [-3e4, 3e4, -1e30, 1e30])
+def test_scores_far_from_zero(dtype, dim, group, share, far):
+    """Scores that are all the same, far below zero or above: every position counts alike.  Errors: 200 weights of 1, fp32 sums of at most 64
+    links, one rounding."""
+    if dtype == torch.float16 and abs(far) > 1e9:
+        pytest.skip("beyond what fp16 queries reach")
+    s = Sequences([200, 50], 1, dim, group, 16, seed=3)
+    c = s.cache
+    c.k_codes.zero_()
+    c.k_scales[..., 0] = 0
+    c.k_scales[..., 1] = 1.0
+    q = torch.full((2, 1, share, dim), far / 64 / dim, dtype=dtype, device="cuda")
+    table, lengths = s.device()
+    got = double(F.attend4(c, q, table, lengths, scale=64.0))
+    _, _, codes, scales = s.buffers()
+    for b in range(2):
+        at = [(s.table[b][i // 16], i % 16) for i in range(s.lengths[b])]
+        v, size = (np.stack(x) for x in zip(*(R.values(codes[p, 0, i], scales[p, 0, i], group, dim, 8) for p, i in at)))
+        want, bound = v.mean(0), size.mean(0) * (2.0 ** -22 + 64 * 2.0 ** -23)
+        assert (np.abs(got[b, 0] - want) <= bound + np.abs(want) * R.HALF_STEP[dtype] * 1.001 + 2.0 ** -25 * (dtype == torch.float16)).all()
