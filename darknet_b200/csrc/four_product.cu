@@ -88,29 +88,28 @@ __device__ __forceinline__ void convert_row(const Eight<T> & raw, unsigned char 
 	float * inverses = (float *)numbers, * sums = inverses + blocks * ROWS;
 	float v[8];
 	eight_f32(raw, v);
-	float most = 0.0f, part = 0.0f;
+	float most[4];                                                // (pairs of pairs: these chains are what a short call waits for)
 	#pragma unroll
-	for (int e = 0; e < 8; ++e)
-	{
-		most = max_nan(most, fabsf(v[e]));
-		part += v[e];
-	}
-	const uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
-	#pragma unroll
-	for (int m = 1; m < GROUP / 8; m <<= 1) { part += __shfl_xor_sync(0xffffffffu, part, m); }
-	if (lane % (GROUP / 8) == 0) { sums[(xb * GROUPS + lane / (GROUP / 8)) * ROWS + row] = part; }
+	for (int e = 0; e < 4; ++e) { most[e] = max_nan(fabsf(v[e]), fabsf(v[e + 4])); }
+	most[0] = max_nan(max_nan(most[0], most[1]), max_nan(most[2], most[3]));
+	const uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(most[0]) & 0x7fffffffu);
 	float factor, inverse;
 	fit_f16(largest, factor, inverse);
 	if (lane == 0) { inverses[xb * ROWS + row] = inverse; }
 	// (what is not finite makes its own column of the products NaN, and the inverse does so anyway)
 	float high[8], rest[8];
-	const float odd_factor = factor * How::ODD;
 	#pragma unroll
 	for (int e = 0; e < 8; ++e)
 	{
-		high[e] = v[e] * (e & 1 ? odd_factor : factor);
+		v[e] *= factor;
+		high[e] = v[e] * (e & 1 ? How::ODD : 1.0f);
 		if (PARTS == 2) { split_f16(high[e], high[e], rest[e]); }
 	}
+	// the sum at that power of two (that of the largest values passes fp32's range)
+	float part = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+	#pragma unroll
+	for (int m = 1; m < GROUP / 8; m <<= 1) { part += __shfl_xor_sync(0xffffffffu, part, m); }
+	if (lane % (GROUP / 8) == 0) { sums[(xb * GROUPS + lane / (GROUP / 8)) * ROWS + row] = part; }
 	unsigned char * at = buffer + (xb * PARTS * x_rows + row) * FP_X_BYTES + (lane / (4 * W) * (4 * W) + lane % W * 4 + lane / W % 4) * 16;
 	*reinterpret_cast<uint4 *>(at) = make_uint4(pair_f16(high[0], high[4]), pair_f16(high[2], high[6]), pair_f16(high[1], high[5]), pair_f16(high[3], high[7]));
 	if (PARTS == 2)
@@ -338,14 +337,10 @@ four_product_kernel(const ProductParams p)
 					for (int nt = 0; nt < NT; ++nt)
 					{
 						const float2 xsum = *(const float2 *)(sums + (xb * GROUPS + q) * ROWS + nt * 8 + t * 2);
-						of_block[mt][nt][0] += sl0.x * acc[mt][nt][0];
-						of_block[mt][nt][1] += sl0.x * acc[mt][nt][1];
-						of_block[mt][nt][2] += sl1.x * acc[mt][nt][2];
-						of_block[mt][nt][3] += sl1.x * acc[mt][nt][3];
-						sum[mt][nt][0] += sl0.y * xsum.x;
-						sum[mt][nt][1] += sl0.y * xsum.y;
-						sum[mt][nt][2] += sl1.y * xsum.x;
-						sum[mt][nt][3] += sl1.y * xsum.y;
+						of_block[mt][nt][0] = fmaf(sl0.x, acc[mt][nt][0], fmaf(sl0.y, xsum.x, of_block[mt][nt][0]));
+						of_block[mt][nt][1] = fmaf(sl0.x, acc[mt][nt][1], fmaf(sl0.y, xsum.y, of_block[mt][nt][1]));
+						of_block[mt][nt][2] = fmaf(sl1.x, acc[mt][nt][2], fmaf(sl1.y, xsum.x, of_block[mt][nt][2]));
+						of_block[mt][nt][3] = fmaf(sl1.x, acc[mt][nt][3], fmaf(sl1.y, xsum.y, of_block[mt][nt][3]));
 					}
 				}
 			}

@@ -30,6 +30,19 @@ def test_products_of_the_largest_rows(dtype, n, k, group, rows):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("n, k, group, rows", [(40, 300, 32, 1), (40, 300, 64, 5), (70, 1000, 128, 13), (8300, 16200, 128, 9)])
+def test_products_of_the_largest_rows_of_one_sign(dtype, n, k, group, rows):
+    """The sum of a group's values is beyond fp32; times weights of both signs, of some 2^-15, nothing is."""
+    m = matrix(n, k, group, n)
+    m.scales.mul_(2.0 ** -15)
+    x = (0.5 + torch.rand(rows, k, generator=rng(k)) / 2).mul(2.0 ** 127).to(dtype).cuda()
+    y = F.forward_connected4(m, x)
+    assert torch.isfinite(y).all()
+    picked = torch.arange(0, n, max(1, n // 40)).cuda()
+    check_product(F.Matrix4(m.codes[picked].contiguous(), m.scales[picked].contiguous(), k, group), x, y[:, picked])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
 @pytest.mark.parametrize("share, dim, group", [(1, 64, 32), (5, 128, 128), (12, 96, 32)])
 def test_attention_of_the_largest_queries(dtype, share, dim, group):
     """Queries of up to 2^126.  The keys of one position point along them and the others do not: that position is all there is.  Keys that are
