@@ -42,6 +42,22 @@ def test_products_of_the_largest_rows_of_one_sign(dtype, n, k, group, rows):
     check_product(F.Matrix4(m.codes[picked].contiguous(), m.scales[picked].contiguous(), k, group), x, y[:, picked])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=ids)
+@pytest.mark.parametrize("group, rows", [(32, 1), (64, 3), (128, 1), (128, 11)])
+def test_products_around_the_middle_code(dtype, group, rows):
+    """Codes 9 and 7 of neighbours whose values are equal and positive: sums around the middle code never get far from 0, the result, and what
+    the tensor cores cut off of them is at most 2^-23 of the 32 that 16 values below 2 come to: after each of 4096 / 16 instructions (twice
+    that in two parts).  Sums of codes 0..15 come to 300 a group of 128, and all that is cut off has one sign."""
+    n, k = 40, 4096
+    codes = torch.full((n, k // 2), 9 | 7 << 4, dtype=torch.uint8)
+    scales = torch.tensor([1.0, -8.0]).half().expand(n, k // group, 2).contiguous()
+    m = F.Matrix4(codes.cuda(), scales.cuda(), k, group)
+    x = (1 + torch.rand(rows, k // 2, generator=rng(group)) * 0.99) * 2.0 ** -torch.randint(0, 11, (rows, k // 2), generator=rng(1)).float()
+    x = x.to(dtype).repeat_interleave(2, 1).cuda()
+    y = double(F.forward_connected4(m, x))
+    assert (np.abs(y) <= (2 if dtype == torch.float32 else 1) * k / 16 * 2.0 ** -23 * 32).all(), np.abs(y).max()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
 @pytest.mark.parametrize("share, dim, group", [(1, 64, 32), (5, 128, 128), (12, 96, 32)])
 def test_attention_of_the_largest_queries(dtype, share, dim, group):
