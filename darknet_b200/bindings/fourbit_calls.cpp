@@ -286,4 +286,16 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fourbit", "Calls of darknet_b200.
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__fourbit() { return PyModule_Create(&module); }
+// (build.py looks for these words in the file)
+extern "C" __attribute__((used)) const char fourbit_built_for[] = "built for torch " BUILT_FOR_TORCH ";";
+
+PyMODINIT_FUNC PyInit__fourbit()
+{
+	PyObject * m = PyModule_Create(&module);
+	if (m != nullptr && PyModule_AddStringConstant(m, "built_for", BUILT_FOR_TORCH) < 0)
+	{
+		Py_DECREF(m);
+		return nullptr;
+	}
+	return m;
+}

@@ -35,6 +35,8 @@ class _Calls:
         except ImportError as e:
             raise FileNotFoundError(f"_fourbit.so is missing or does not load ({e}): it has not been built (python -m darknet_b200.build). "
                                     "There is no CPU or PyTorch fallback for this path.") from e
+        if _fourbit.built_for != torch.__version__:
+            raise FileNotFoundError(f"_fourbit.so has been built for torch {_fourbit.built_for}, this is {torch.__version__}: build it again (python -m darknet_b200.build)")
         for f in ("product", "append", "read", "attend"):
             setattr(self, f, getattr(_fourbit, f))
         return object.__getattribute__(self, name)
