@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <climits>
 #include <cmath>
 #include <optional>
 
@@ -110,6 +111,7 @@ PyObject * product(PyObject *, PyObject * const * args, Py_ssize_t n_args)
 				|| !take(args[4], given) || codes == nullptr || scales == nullptr || x == nullptr || !PyLong_Check(args[3])) { Py_RETURN_NONE; }
 		if (codes->dim() != 2) { Py_RETURN_NONE; }
 		const int64_t n = codes->size(0), k = whole(PyTuple_GET_ITEM(args[0], 2));
+		if (n > INT_MAX || k > INT_MAX) { Py_RETURN_NONE; }
 		const c10::Device d = codes->device();
 		const int type = type_of(*x);
 		if (!on(*codes, d) || !on(*scales, d) || !on(*x, d) || type < 0 || x->dim() != 2 || x->size(1) != k || (k != 1 && x->stride(1) != 1)) { Py_RETURN_NONE; }
@@ -154,10 +156,10 @@ bool take_cache(PyObject * o, xnor_b200_kv4_cache & c, std::optional<c10::Device
 		if (!on(*v, *d)) { return false; }
 	}
 	const at::IntArrayRef s = t[0]->sizes();
-	if (s.size() != 4) { return false; }
+	if (s.size() != 4 || s[0] > INT_MAX || s[1] > INT_MAX || s[2] > INT_MAX || s[3] > INT_MAX / 2) { return false; }
 	c = {(uint8_t *)t[0]->data_ptr(), t[1]->data_ptr(), (uint8_t *)t[2]->data_ptr(), t[3]->data_ptr(), (int)s[0], (int)s[1], (int)s[2], (int)(2 * s[3]),
 			(int)whole(PyTuple_GET_ITEM(o, 4))};
-	return s[0] <= INT_MAX && s[1] <= INT_MAX && s[2] <= INT_MAX;
+	return true;
 }
 
 bool take_rows(PyObject * table_o, PyObject * lengths_o, PyObject * counts_o, const c10::Device & d, int64_t batch, int64_t tokens, xnor_b200_kv4_rows & r)

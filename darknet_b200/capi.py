@@ -116,6 +116,7 @@ class ConvGeom(C.Structure):
 
 
 F32, F16, BF16 = 0, 1, 2
+W4_MAX_K, W4_MAX_N = 1 << 24, 1 << 28       # XNOR_B200_W4_MAX_K, XNOR_B200_W4_MAX_N
 KV4_MAX_DIM = 256               # XNOR_B200_KV4_MAX_DIM
 
 

@@ -60,6 +60,11 @@ def _on(device: torch.device, *tensors) -> None:
         raise ValueError(f"tensors on {device}: this path runs on a CUDA device only")
 
 
+def _fits(n: int, k: int) -> None:
+    if n > capi.W4_MAX_N or k > capi.W4_MAX_K:
+        raise ValueError(f"a matrix has at most {capi.W4_MAX_N} rows of at most {capi.W4_MAX_K} values: got [{n}][{k}]")
+
+
 class _Fixed:
     """What a handle was made of and checked for stays what it is."""
 
@@ -80,6 +85,7 @@ class Matrix4(_Fixed):
             raise ValueError(f"scales must be contiguous fp16 [{codes.shape[0]}][{(k + group - 1) // group}][2]")
         if scales.device != codes.device:
             raise ValueError(f"codes on {codes.device}, scales on {scales.device}")
+        _fits(codes.shape[0], k)
         self.__dict__.update(codes=codes, scales=scales, n=codes.shape[0], k=k, group=group, device=codes.device, _native=(codes, scales, k, group))
 
 
@@ -90,6 +96,7 @@ def quantize_weights4(weights: torch.Tensor, group: int) -> Matrix4:
     if group not in _GROUPS:
         raise ValueError(f"group must be one of {_GROUPS}, not {group}")
     n, k = weights.shape
+    _fits(n, k)
     dtype = _dtype(weights, "weights")
     _on(weights.device)
     with torch.cuda.device(weights.device):
@@ -137,6 +144,8 @@ class Cache4(_Fixed):
             raise ValueError("codes must be [pages][kv_heads][page][dim/2]")
         pages, kv_heads, page, half = k_codes.shape
         dim = 2 * half
+        if pages >= 2 ** 31 or kv_heads >= 2 ** 31 or page >= 2 ** 31:
+            raise ValueError(f"pages, heads and tokens of a page are below 2^31: got {list(k_codes.shape)}")
         if page % 16 or dim % 32 or dim % group or dim > capi.KV4_MAX_DIM:
             raise ValueError(f"page must be a multiple of 16, dim one of 32 and of the group, at most {capi.KV4_MAX_DIM}: got page {page}, dim {dim}, group {group}")
         for codes, scales in ((k_codes, k_scales), (v_codes, v_scales)):

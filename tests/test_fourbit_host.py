@@ -168,3 +168,31 @@ def test_matrices_of_other_shapes_are_refused(what):
 def test_caches_of_other_shapes_are_refused(shape):
     with pytest.raises(ValueError):
         F.new_cache4(*shape, device="cpu")
+
+
+@pytest.mark.parametrize("n, k", [(2 ** 32 + 5, 32), (2 ** 28 + 1, 8), (1, 2 ** 24 + 1), (2, 2 ** 32 + 64)])
+def test_matrices_beyond_an_int_are_refused(n, k):
+    """(Sizes that the C ABI's ints would have cut down to other, valid ones.)"""
+    on = dict(device="meta")
+    codes, scales = torch.empty(n, (k + 31) // 32 * 16, dtype=torch.uint8, **on), torch.empty(n, (k + 31) // 32, 2, dtype=torch.float16, **on)
+    with pytest.raises(ValueError, match="at most"):
+        F.Matrix4(codes, scales, k, 32)
+    with pytest.raises(ValueError, match="at most"):
+        F.quantize_weights4(torch.empty(n, k, **on), 32)
+    F.Matrix4(torch.empty(2 ** 28, 16, dtype=torch.uint8, **on), torch.empty(2 ** 28, 1, 2, dtype=torch.float16, **on), 32, 32)
+    F.Matrix4(torch.empty(2, 2 ** 23, dtype=torch.uint8, **on), torch.empty(2, 2 ** 19, 2, dtype=torch.float16, **on), 2 ** 24, 32)
+
+
+def test_caches_beyond_an_int_are_refused():
+    with pytest.raises(ValueError, match="below 2"):
+        F.new_cache4(2 ** 32 + 1, 1, 16, 32, 32, device="meta")
+    F.new_cache4(2 ** 31 - 1, 1, 16, 32, 32, device="meta")
+
+
+def test_the_limits_are_the_headers():
+    import os
+    import re
+    header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "xnor_b200.h")).read()
+    for name in ("W4_MAX_K", "W4_MAX_N", "KV4_MAX_DIM"):
+        value = re.search(rf"#define XNOR_B200_{name}\s+(.*)", header)[1]
+        assert eval(value) == getattr(capi, name)
