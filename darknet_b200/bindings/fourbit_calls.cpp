@@ -3,20 +3,22 @@
 // A decoding step is a dozen kernels of 4 to 8 us, so the host that issues them is what it waits for.  Asked through ctypes, a call took 8 us
 // (a product) to 11 us (attention), 3 of them the launch; most of the others went into looking up shapes, types, strides and addresses one by
 // one.  Here they are read from the tensors themselves.  Every function returns None where an argument is not what it has to be (fourbit.py
-// then looks for what is wrong and says so), the library's code as a number where the library refused, and its result otherwise.
+// then looks for what is wrong and says so), the library's code as a number where the library refused, and its result otherwise; outputs that
+// share memory with inputs are refused here, where the addresses are.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
-#include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <optional>
+#include <vector>
 
 #include "xnor_b200.h"
 
@@ -100,6 +102,141 @@ long long whole(PyObject * o)
 	return v;
 }
 
+// ---- memory in common.  What a call writes to is looked at where it was given: a comparison of two ranges, and only where those meet (views of
+// one buffer, side by side) the elements themselves.
+struct Dim { int64_t size, stride; };
+
+// A tensor's dimensions of more than one entry, the widest stride first; false where more of them would be than in any call.
+bool layout(const Tensor & t, Dim (&d)[4], int & n)
+{
+	n = 0;
+	for (int64_t i = 0; i < t.dim(); ++i)
+	{
+		if (t.size(i) == 1) { continue; }
+		if (n == 4) { return false; }
+		d[n++] = {t.size(i), t.stride(i)};
+	}
+	std::sort(d, d + n, [](const Dim & a, const Dim & b) { return a.stride > b.stride; });
+	return true;
+}
+
+// Entries from the first to behind the last.
+int64_t extent(const Dim * d, int n)
+{
+	int64_t e = 1;
+	for (int i = 0; i < n; ++i) { e += (d[i].size - 1) * d[i].stride; }
+	return e;
+}
+
+// Every dimension's steps pass over all that the narrower ones cover: no entry is there twice.
+bool nested(const Dim * d, int n)
+{
+	for (int i = 0; i < n; ++i)
+	{
+		if (d[i].stride < extent(d + i + 1, n - i - 1)) { return false; }
+	}
+	return true;
+}
+
+// Two tensors of these nested dimensions, the second `apart` entries behind the first, have an entry in common: two steps of a dimension at
+// most come near enough for the narrower ones.
+bool within(const Dim * d, int n, int64_t apart)
+{
+	if (n == 0) { return apart == 0; }
+	const int64_t inner = extent(d + 1, n - 1), first = apart >= 0 ? apart / d->stride : -((-apart + d->stride - 1) / d->stride);
+	for (int64_t steps = first; steps <= first + 1; ++steps)
+	{
+		const int64_t rest = apart - steps * d->stride;
+		if (steps > -d->size && steps < d->size && rest > -inner && rest < inner && within(d + 1, n - 1, rest)) { return true; }
+	}
+	return false;
+}
+
+// Where a tensor's rows start, in order, and their bytes.  One row where all of it is contiguous.
+std::vector<uintptr_t> rows_of(const Tensor & t, size_t & bytes)
+{
+	const uintptr_t first = (uintptr_t)t.data_ptr();
+	const int64_t size = t.element_size(), dims = t.dim();
+	std::vector<uintptr_t> rows = {first};
+	if (t.is_contiguous())
+	{
+		bytes = (size_t)(t.numel() * size);
+		return rows;
+	}
+	const bool whole_rows = t.stride(dims - 1) == 1 || t.size(dims - 1) == 1;
+	bytes = (size_t)(whole_rows ? t.size(dims - 1) * size : size);
+	for (int64_t i = 0; i < dims - (whole_rows ? 1 : 0); ++i)
+	{
+		const size_t before = rows.size();
+		for (int64_t j = 1; j < t.size(i); ++j)
+		{
+			for (size_t r = 0; r < before; ++r) { rows.push_back(rows[r] + j * t.stride(i) * size); }
+		}
+	}
+	std::sort(rows.begin(), rows.end());
+	return rows;
+}
+
+bool meet(const Tensor & a, const Tensor & b)
+{
+	if (a.numel() == 0 || b.numel() == 0) { return false; }
+	Dim da[4], db[4];
+	int na, nb;
+	const bool known = layout(a, da, na) && layout(b, db, nb);
+	const uintptr_t a0 = (uintptr_t)a.data_ptr(), b0 = (uintptr_t)b.data_ptr();
+	const int64_t size = a.element_size();
+	if (known)
+	{
+		if (a0 + extent(da, na) * size <= b0 || b0 + extent(db, nb) * b.element_size() <= a0) { return false; }
+		const int64_t bytes = (int64_t)(b0 - a0);
+		if (na == nb && b.element_size() == size && bytes % size == 0 && nested(da, na)
+				&& std::equal(da, da + na, db, [](const Dim & x, const Dim & y) { return x.size == y.size && x.stride == y.stride; }))
+		{
+			return within(da, na, bytes / size);
+		}
+	}
+	size_t a_bytes, b_bytes;
+	const std::vector<uintptr_t> ra = rows_of(a, a_bytes), rb = rows_of(b, b_bytes);
+	for (size_t i = 0, j = 0; i < ra.size() && j < rb.size(); )
+	{
+		if (ra[i] + a_bytes <= rb[j]) { ++i; }
+		else if (rb[j] + b_bytes <= ra[i]) { ++j; }
+		else { return true; }
+	}
+	return false;
+}
+
+bool meets_itself(const Tensor & t)
+{
+	Dim d[4];
+	int n;
+	if (t.numel() == 0 || (layout(t, d, n) && nested(d, n))) { return false; }
+	size_t bytes;
+	const std::vector<uintptr_t> rows = rows_of(t, bytes);
+	for (size_t i = 1; i < rows.size(); ++i)
+	{
+		if (rows[i - 1] + bytes > rows[i]) { return true; }
+	}
+	return false;
+}
+
+// The same entries in the same order.
+bool same(const Tensor & a, const Tensor & b)
+{
+	if (a.data_ptr() != b.data_ptr() || a.sizes() != b.sizes()) { return false; }
+	for (int64_t i = 0; i < a.dim(); ++i)
+	{
+		if (a.size(i) > 1 && a.stride(i) != b.stride(i)) { return false; }
+	}
+	return true;
+}
+
+[[noreturn]] void refuse(const char * what)
+{
+	PyErr_SetString(PyExc_ValueError, what);
+	throw Failed();
+}
+
 // ---- products: ((codes, scales, k, group), x, biases, activation, out)
 PyObject * product(PyObject *, PyObject * const * args, Py_ssize_t n_args)
 {
@@ -122,6 +259,14 @@ PyObject * product(PyObject *, PyObject * const * args, Py_ssize_t n_args)
 		const int64_t rows = x->size(0);
 		if (given != nullptr && (!on(*given, d) || given->scalar_type() != x->scalar_type() || given->dim() != 2 || given->size(0) != rows || given->size(1) != n
 				|| (n != 1 && given->stride(1) != 1))) { Py_RETURN_NONE; }
+		if (given != nullptr)
+		{
+			for (const Tensor * input : {x, biases, codes, scales})
+			{
+				if (input != nullptr && meet(*given, *input)) { refuse("out has memory in common with what the product reads"); }
+			}
+			if (meets_itself(*given)) { refuse("out has entries that are the same memory"); }
+		}
 		const c10::cuda::CUDAGuard guard(d);
 		const Tensor out = given != nullptr ? *given : empty({rows, n}, x->scalar_type(), d);
 		if (rows == 0) { return THPVariable_Wrap(out); }
@@ -257,8 +402,14 @@ PyObject * attend(PyObject *, PyObject * const * args, Py_ssize_t n_args)
 		{
 			Py_RETURN_NONE;
 		}
-		if (given != nullptr && (given->sizes() != q->sizes() || !take_tensor(*given, *d, ot) || ot.dtype != qt.dtype
-				|| at::has_internal_overlap(*given) == at::MemOverlap::Yes)) { Py_RETURN_NONE; }
+		if (given != nullptr)
+		{
+			if (given->sizes() != q->sizes() || !take_tensor(*given, *d, ot) || ot.dtype != qt.dtype) { Py_RETURN_NONE; }
+			if (meets_itself(*given)) { refuse("out has entries that are the same memory"); }
+			// (every CTA has read its queries before any writes the same ones' results)
+			if (!same(*given, *q) && meet(*given, *q)) { refuse("out has memory in common with q, and is not q itself"); }
+		}
+		if (lse != nullptr && (meet(*lse, *q) || (given != nullptr && meet(*lse, *given)))) { refuse("lse has memory in common with q or out"); }
 		const c10::cuda::CUDAGuard guard(*d);
 		const Tensor out = given != nullptr ? *given : empty(q->sizes(), q->scalar_type(), *d);
 		if (q->numel() == 0) { return THPVariable_Wrap(out); }
@@ -276,11 +427,23 @@ PyObject * attend(PyObject *, PyObject * const * args, Py_ssize_t n_args)
 	});
 }
 
+// (a, b): whether two tensors have memory in common; (a): whether entries of one are the same memory.
+PyObject * shares(PyObject *, PyObject * const * args, Py_ssize_t n_args)
+{
+	return guarded([&]() -> PyObject *
+	{
+		const Tensor * a, * b = nullptr;
+		if (n_args < 1 || n_args > 2 || !take(args[0], a) || a == nullptr || (n_args == 2 && (!take(args[1], b) || b == nullptr))) { Py_RETURN_NONE; }
+		return PyBool_FromLong(b != nullptr ? meet(*a, *b) : meets_itself(*a));
+	});
+}
+
 PyMethodDef methods[] = {
 	{"product", (PyCFunction)(void *)product, METH_FASTCALL, "xnor_b200_w4_forward"},
 	{"append", (PyCFunction)(void *)append, METH_FASTCALL, "xnor_b200_kv4_append"},
 	{"read", (PyCFunction)(void *)read, METH_FASTCALL, "xnor_b200_kv4_read"},
 	{"attend", (PyCFunction)(void *)attend, METH_FASTCALL, "xnor_b200_kv4_attend"},
+	{"shares", (PyCFunction)(void *)shares, METH_FASTCALL, "whether two tensors, or entries of one, are the same memory"},
 	{nullptr, nullptr, 0, nullptr},
 };
 

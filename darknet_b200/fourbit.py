@@ -123,7 +123,7 @@ def _refuse_product(m: Matrix4, x, biases, activation, out) -> None:
 def forward_connected4(m: Matrix4, x: torch.Tensor, biases: Optional[torch.Tensor] = None, activation: int = capi.LINEAR,
                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """act(x @ W.T + biases) for x [rows][k] (rows contiguous, any distance apart), W the packed matrix: xnor_b200_w4_forward.
-    biases: fp32 [n].  out: [rows][n] of x's type, rows contiguous; made where it is not given.  One pass over the weights serves up to
+    biases: fp32 [n].  out: [rows][n] of x's type, rows contiguous, no memory in common with any input; made where it is not given.  One pass over the weights serves up to
     16 rows."""
     y = _calls.product(m._native, x, biases, activation, out)
     if y is None:
@@ -212,7 +212,8 @@ def attend4(c: Cache4, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tens
             scale: Optional[float] = None, window: int = 0, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the newest tokens' queries [batch][tokens][heads][dim] over what their sequences hold, those tokens among it (append4
     comes first): xnor_b200_kv4_attend.  scale: 1/sqrt(dim) where not given.  window: positions that a token sees, itself among them
-    (0: all).  Rows that see nothing are 0.  out: as q; made where it is not given.  lse: fp32 [batch][tokens][heads], contiguous, receives
+    (0: all).  Rows that see nothing are 0.  out: as q, and may be q itself, but have no other memory in common with it; made where it is not
+    given.  lse: fp32 [batch][tokens][heads], contiguous, receives
     the logarithm of each row's sum of exponentials."""
     y = _calls.attend(c._native, q, table, lengths, counts, scale, window, out, lse)
     if y is None:
@@ -221,8 +222,8 @@ def attend4(c: Cache4, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tens
         if q.dim() != 4 or q.shape[3] != c.dim or q.shape[2] == 0 or q.shape[2] % c.kv_heads or q.stride(3) != 1:
             raise ValueError(f"q must be [batch][tokens][heads][{c.dim}], heads a multiple of {c.kv_heads}, the last dimension contiguous")
         _refuse_rows(c, q.shape[0], table, lengths, counts)
-        if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1 or torch._debug_has_internal_overlap(out) == 1):
-            raise ValueError(f"out must be {q.dtype} {list(q.shape)}, the last dimension contiguous, no memory used twice")
+        if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1):
+            raise ValueError(f"out must be {q.dtype} {list(q.shape)}, the last dimension contiguous")
         if lse is not None and (lse.shape != q.shape[:3] or lse.dtype != torch.float32 or not lse.is_contiguous()):
             raise ValueError(f"lse must be contiguous fp32 {list(q.shape[:3])}")
         raise ValueError("window must be a number, at least 0")

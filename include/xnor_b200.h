@@ -661,7 +661,7 @@ XNOR_B200_API int xnor_b200_kv4_read(const xnor_b200_kv4_cache * cache, const xn
 /* Attention of the rows over their sequences: row i of sequence b, at position lengths[b] - counts[b] + i, sees the positions up to its
  * own (with window > 0 the last `window` of them) that are kept in pages that the cache has; per head of `heads` (a multiple of
  * kv_heads; heads / kv_heads neighbours share a head of keys), output = sum_j softmax_j(scale * q . k_j) v_j.  q and output:
- * [batch][tokens][heads][dim] of one type, no memory in common.  A row that sees nothing, and rows of counts[b] and above, are 0.
+ * [batch][tokens][heads][dim] of one type; output may be q itself, and has no other memory in common with it.  A row that sees nothing, and rows of counts[b] and above, are 0.
  * lse: fp32 [batch][tokens][heads] or NULL, receives log(sum_j exp(scale * q . k_j)), -infinity where nothing is seen.  Scores,
  * softmax and sums are fp32, rounded once.  What lies behind a sequence's length in its last page is never counted.
  * scratch: xnor_b200_kv4_attend_scratch_bytes() bytes on the current device (0: may be NULL), 16-byte aligned, of this call alone until

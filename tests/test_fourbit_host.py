@@ -196,3 +196,34 @@ def test_the_limits_are_the_headers():
     for name in ("W4_MAX_K", "W4_MAX_N", "KV4_MAX_DIM"):
         value = re.search(rf"#define XNOR_B200_{name}\s+(.*)", header)[1]
         assert eval(value) == getattr(capi, name)
+
+
+def test_memory_in_common_is_found(L):
+    """Views of one buffer against what their entries' numbers say."""
+    import random
+    from darknet_b200 import _fourbit
+    r = random.Random(5)
+    buffer = torch.arange(600, dtype=torch.int16)
+    found = {True: 0, False: 0}
+    for i in range(4000):
+        def view(like=None):
+            if like is not None and r.random() < 0.5:
+                size, stride = like.size(), like.stride()
+            else:
+                size = [r.choice((1, 1, 2, 3, 4)) for _ in range(r.choice((1, 2, 3)))] + [r.choice((1, 2, 5))]
+                stride = [r.choice((0, 1, 3, 5, 6, 10, 20, 40)) for _ in size[:-1]] + [r.choice((1, 1, 1, 2))]
+            room = 600 - sum((n - 1) * s for n, s in zip(size, stride))
+            return buffer.as_strided(size, stride, r.randrange(min(60, room)))
+        a = view()
+        b = view(a)
+        entries = a.flatten().tolist()
+        assert _fourbit.shares(a) == (len(set(entries)) < len(entries)), (a.size(), a.stride())
+        want = bool(set(entries) & set(b.flatten().tolist()))
+        assert _fourbit.shares(a, b) == want, (a.size(), a.stride(), b.size(), b.stride(), a.storage_offset(), b.storage_offset())
+        found[want] += 1
+    assert min(found.values()) > 500
+    wide = buffer.view(torch.int32)                          # entries of another size
+    assert _fourbit.shares(wide[3:5], buffer[9:20]) and not _fourbit.shares(wide[3:5], buffer[10:20])
+    assert not _fourbit.shares(buffer[:0], buffer) and _fourbit.shares(torch.zeros(2, 2)) is False
+    qkv = torch.zeros(64, 512, 24, 128, device="cpu", dtype=torch.float16)
+    assert not _fourbit.shares(qkv[:, :, :8], qkv[:, :, 8:16]) and _fourbit.shares(qkv[:, :, :9], qkv[:, :, 8:17])

@@ -188,3 +188,44 @@ def test_scores_far_from_zero(dtype, dim, group, share, far):
         v, size = (np.stack(x) for x in zip(*(R.values(codes[p, 0, i], scales[p, 0, i], group, dim, 8) for p, i in at)))
         want, bound = v.mean(0), size.mean(0) * (2.0 ** -22 + 64 * 2.0 ** -23)
         assert (np.abs(got[b, 0] - want) <= bound + np.abs(want) * R.HALF_STEP[dtype] * 1.001 + 2.0 ** -25 * (dtype == torch.float16)).all()
+
+
+def test_outputs_that_share_memory():
+    m = matrix(64, 64, 32, 1)
+    whole = torch.randn(6, 160, generator=rng(1)).cuda()
+    x = whole[:, :64]
+    want = F.forward_connected4(m, x)
+    assert torch.equal(F.forward_connected4(m, x, out=whole[:, 64:128]), want)               # side by side
+    for out in (x, whole[:, 32:96], whole.view(-1)[100:484].view(6, 64), whole.as_strided((6, 64), (64, 1), 0)):
+        with pytest.raises(ValueError, match="memory"):
+            F.forward_connected4(m, x, out=out)
+    bias = torch.zeros(640, device="cuda")
+    with pytest.raises(ValueError, match="memory"):
+        F.forward_connected4(m, x, bias[100:164], out=bias[:384].view(6, 64))
+    with pytest.raises(ValueError, match="memory"):
+        F.forward_connected4(m, x, out=bias.as_strided((6, 64), (63, 1), 0))
+
+    for lengths in ([40, 7], [900, 30]):                     # one CTA, and a cluster of them, a sequence
+        s = Sequences(lengths, 2, 64, 32, room=30)
+        table, n = s.device()
+        qs = torch.randn(2, 3, 12, 64, generator=rng(2)).half().cuda()
+        q = qs[:, :, :4]
+        want = F.attend4(s.cache, q, table, n)
+        assert torch.equal(F.attend4(s.cache, q, table, n, out=qs[:, :, 4:8]), want)
+        for out in (qs[:, :, 1:5], qs.as_strided(q.shape, (0, 768, 64, 1), 2000), qs.as_strided(q.shape, q.stride(), 32)):
+            with pytest.raises(ValueError, match="memory"):
+                F.attend4(s.cache, q, table, n, out=out)
+        copy = q.clone()
+        assert torch.equal(F.attend4(s.cache, copy, table, n, out=copy), want)               # in the place of the queries
+        room = torch.zeros(4096, device="cuda")
+        qf = room[:1536].view(2, 3, 4, 64)
+        with pytest.raises(ValueError, match="memory"):
+            F.attend4(s.cache, qf, table, n, lse=room[1500:1524].view(2, 3, 4))
+        with pytest.raises(ValueError, match="memory"):
+            F.attend4(s.cache, qf, table, n, out=room[2000:3536].view(2, 3, 4, 64), lse=room[3535:3559].view(2, 3, 4))
+        F.attend4(s.cache, qf, table, n, out=room[2000:3536].view(2, 3, 4, 64), lse=room[3536:3560].view(2, 3, 4))
+    s = Sequences([6000], 1, 64, 32, 64)                     # more splits than a cluster has
+    table, n = s.device()
+    q = torch.randn(1, 5, 8, 64, generator=rng(3)).half().cuda()
+    want = F.attend4(s.cache, q, table, n)
+    assert torch.equal(F.attend4(s.cache, q, table, n, out=q), want)
