@@ -214,7 +214,7 @@ def attend4(c: Cache4, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tens
     comes first): xnor_b200_kv4_attend.  scale: 1/sqrt(dim) where not given.  window: positions that a token sees, itself among them
     (0: all).  Rows that see nothing are 0.  out: as q, and may be q itself, but have no other memory in common with it; made where it is not
     given.  lse: fp32 [batch][tokens][heads], contiguous, receives
-    the logarithm of each row's sum of exponentials."""
+    the logarithm of each row's sum of exponentials.  tokens * heads: up to half a million a call, up to dim 128 three times as many."""
     y = _calls.attend(c._native, q, table, lengths, counts, scale, window, out, lse)
     if y is None:
         _on(c.device, q, out, lse)

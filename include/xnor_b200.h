@@ -608,8 +608,9 @@ XNOR_B200_API int xnor_b200_w4_quantize(const xnor_b200_w4_desc * desc, const vo
 		uint8_t * codes, void * scales, void * stream);
 
 /* forward_connected_layer_gpu (src-lib/connected_layer.cpp) with such weights: output[r][i] = act(sum_j x[r][j] * value[i][j] + biases[i])
- * for `rows` rows of x, ldx elements apart, to rows ldo elements apart, both of type `dtype`; biases fp32 [n] or NULL.  Sums are fp32,
- * rounded once.  A row of x that holds an infinity or a NaN gives NaN.  Made for few rows (one pass over the weights serves 16).
+ * for `rows` rows of x, ldx elements apart, to rows ldo elements apart, both of type `dtype`; biases fp32 [n] or NULL.  Sums are
+ * fp32 (of fp32 rows' values to 22 bits, next to the largest of 256 neighbours), rounded once.  A row of x that holds an infinity or a NaN
+ * gives NaN.  Made for few rows (one pass over the weights serves 16).
  * output overlaps no input.  scratch: xnor_b200_w4_scratch_bytes() bytes (0 for all but large products of many rows: may be NULL), 16-byte
  * aligned, of this call alone until it has run; needs no initialisation. */
 XNOR_B200_API size_t xnor_b200_w4_scratch_bytes(const xnor_b200_w4_desc * desc, int dtype, int rows);
@@ -617,9 +618,9 @@ XNOR_B200_API int xnor_b200_w4_forward(const xnor_b200_w4_desc * desc, const voi
 		const uint8_t * codes, const void * scales, const float * biases, void * output, long long ldo, void * scratch, size_t scratch_bytes,
 		void * stream);
 
-/* Keys and values of tokens in pages of `page` tokens (a multiple of 16): codes [pages][kv_heads][page][dim/2] bytes, scales
- * [pages][kv_heads][page][dim/group][2] fp16, all four 16-byte aligned.  dim: a multiple of 32, at most XNOR_B200_KV4_MAX_DIM, and
- * of group. */
+/* Keys and values of tokens in pages of `page` tokens (a multiple of 16, at most 2^20; attention: pages * kv_heads * page below 2^35): codes
+ * [pages][kv_heads][page][dim/2] bytes, scales [pages][kv_heads][page][dim/group][2] fp16, all four 16-byte aligned.  dim: a multiple of 32,
+ * at most XNOR_B200_KV4_MAX_DIM, and of group. */
 #define XNOR_B200_KV4_MAX_DIM 256
 typedef struct xnor_b200_kv4_cache
 {
@@ -661,9 +662,13 @@ XNOR_B200_API int xnor_b200_kv4_read(const xnor_b200_kv4_cache * cache, const xn
 /* Attention of the rows over their sequences: row i of sequence b, at position lengths[b] - counts[b] + i, sees the positions up to its
  * own (with window > 0 the last `window` of them) that are kept in pages that the cache has; per head of `heads` (a multiple of
  * kv_heads; heads / kv_heads neighbours share a head of keys), output = sum_j softmax_j(scale * q . k_j) v_j.  q and output:
- * [batch][tokens][heads][dim] of one type; output may be q itself, and has no other memory in common with it.  A row that sees nothing, and rows of counts[b] and above, are 0.
- * lse: fp32 [batch][tokens][heads] or NULL, receives log(sum_j exp(scale * q . k_j)), -infinity where nothing is seen.  Scores,
- * softmax and sums are fp32, rounded once.  What lies behind a sequence's length in its last page is never counted.
+ * [batch][tokens][heads][dim] of one type; output may be q itself, and has no other memory in common with it.  A row that sees nothing, and rows of
+ * counts[b] and above, are 0.  lse: fp32 [batch][tokens][heads] or NULL, receives log(sum_j exp(scale * q . k_j)), -infinity where nothing is
+ * seen.  Scores, softmax and sums are fp32, of weights and fp32 queries to 22 bits; results are rounded once.  What lies behind a sequence's
+ * length in its last page is never counted.
+ * A call's grid has room for 65535 tiles of columns, a column being a token's head of queries: ceil(tokens * heads / kv_heads / 8) * kv_heads,
+ * in eights up to dim 256, in up to 24s up to dim 128 (32 heads: some 16 000 tokens of a sequence a call, and some 49 000).  Beyond, and for
+ * more than 65535 sequences or heads of keys, XNOR_B200_ERR_TOO_LARGE: a longer prompt takes several calls.
  * scratch: xnor_b200_kv4_attend_scratch_bytes() bytes on the current device (0: may be NULL), 16-byte aligned, of this call alone until
  * it has run; needs no initialisation. */
 XNOR_B200_API size_t xnor_b200_kv4_attend_scratch_bytes(const xnor_b200_kv4_cache * cache, const xnor_b200_kv4_rows * rows, int heads, int window);

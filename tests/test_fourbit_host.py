@@ -227,3 +227,12 @@ def test_memory_in_common_is_found(L):
     assert not _fourbit.shares(buffer[:0], buffer) and _fourbit.shares(torch.zeros(2, 2)) is False
     qkv = torch.zeros(64, 512, 24, 128, device="cpu", dtype=torch.float16)
     assert not _fourbit.shares(qkv[:, :, :8], qkv[:, :, 8:16]) and _fourbit.shares(qkv[:, :, :9], qkv[:, :, 8:17])
+
+
+def test_attention_over_prompts_has_the_limit_that_the_header_names(L):
+    """65535 tiles of columns in a call's grid: of 8 columns, up to dim 128 of 24.  (Refusals only: nothing is launched.)"""
+    def attend(tokens, heads, kv_heads, dim):
+        c, r, t = cache(dim=dim, kv_heads=kv_heads), rows(tokens=tokens), tensor()
+        return L.xnor_b200_kv4_attend(c, r, t, heads, 1.0, 0, t, None, None, 0, None)
+    assert attend(65535 // 8 * 2 + 2, 32, 8, 256) == 6 and attend(65535 // 8 * 6 + 6, 32, 8, 128) == 6
+    assert attend(1, 32, 65536, 64) in (1, 6) and attend((1 << 31) - 1, 64, 1, 64) == 6

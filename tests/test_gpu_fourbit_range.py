@@ -229,3 +229,44 @@ def test_outputs_that_share_memory():
     q = torch.randn(1, 5, 8, 64, generator=rng(3)).half().cuda()
     want = F.attend4(s.cache, q, table, n)
     assert torch.equal(F.attend4(s.cache, q, table, n, out=q), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("lengths, kv_heads, tokens, page", [([90, 50, 70, 33], 16, 1, 16), ([900, 700, 40, 600], 2, 3, 16), ([5000, 3000, 4100, 10], 1, 1, 64)])
+def test_a_sequences_results_do_not_depend_on_the_others(dtype, lengths, kv_heads, tokens, page):
+    """The first sequence among others of other lengths, pages, queries and counts, of scales that are not finite, and in another place of the
+    batch: one CTA a sequence, clusters, and splits that meet in scratch memory."""
+    s = Sequences(lengths, kv_heads, 64, 32, page, seed=4, spare=40)
+    c = s.cache
+    q = torch.randn(4, tokens, 6 * kv_heads, 64, generator=rng(1)).to(dtype).cuda()
+    table, n = s.device()
+    counts = torch.full((4,), tokens, dtype=torch.int32, device="cuda")
+    want = F.attend4(c, q, table, n, counts)[0].clone()
+    other = torch.randn(4, tokens, 6 * kv_heads, 64, generator=rng(2)).to(dtype).cuda()
+    other[0] = q[0]
+    n2, counts2, table2 = n.clone(), counts.clone(), table.clone()
+    n2[1:] = torch.tensor([1, 700 % lengths[2], 0], dtype=torch.int32)
+    counts2[2] = 0
+    table2[3] = -1
+    other[1] = math.nan
+    for scales in (c.k_scales, c.v_scales):
+        scales[table[2][table[2] >= 0].long()] = math.inf
+    got = F.attend4(c, other, table2, n2, counts2)
+    assert torch.equal(got[0], want) and not got[3].any()
+    order = torch.tensor([2, 3, 0, 1]).cuda()
+    got = F.attend4(c, other[order], table2[order], n2[order], counts2[order])
+    assert torch.equal(got[2], want)
+
+
+def test_rows_inside_a_table_that_is_too_short_are_read_back():
+    s = Sequences([64, 40], 2, 64, 32, 16, seed=5)
+    s.lengths = [70, 66]                                     # (of 64 and 48 places: rows 0 and 1 of the first have one)
+    table, lengths = s.device()
+    k, v = (torch.randn(2, 8, 2, 64, generator=rng(i)).cuda() for i in (3, 4))
+    F.append4(s.cache, k, v, table, lengths)
+    for given, got in zip((k, v), F.read4(s.cache, table, lengths, 8)):
+        codes, scales = R.quantize(double(given[0, :2]), 32)
+        want = R.values(R.pack(codes), scales, 32, 64)[0]
+        # one fma, rounded to fp32
+        assert (np.abs(double(got[0, :2]) - want) <= np.abs(want) * 2.0 ** -23).all()
+        assert not got[0, 2:].any() and not got[1].any()
