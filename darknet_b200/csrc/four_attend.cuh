@@ -588,7 +588,8 @@ four_attend_kernel(const AttendParams p)
 			#pragma unroll
 			for (int nt = 0; nt < NT; ++nt)
 			{
-				int back[2];                                      // what there is counts for 2^-back of what it did
+				float keep[2];                                    // what there is counts for that much of what it did: 2^-back, and not quite half of it
+				int back[2];
 				#pragma unroll
 				for (int e = 0; e < 2; ++e)
 				{
@@ -605,20 +606,21 @@ four_attend_kernel(const AttendParams p)
 					m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
 					m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
 					// others may have moved theirs: a column's sums depend on its own scores alone
+					keep[e] = 1.0f;
 					back[e] = 0;
 					if (m > limit[nt][e])
 					{
-						m = ceilf(m);
-						back[e] = limit[nt][e] == -INFINITY ? 256 : (int)fminf(m - base[nt][e], 256.0f);
+						const bool fresh = limit[nt][e] == -INFINITY;
+						keep[e] = fresh ? 0.0f : exp2_fast(base[nt][e] - m);
+						back[e] = fresh ? 256 : (int)fminf(m - base[nt][e], 256.0f);
 						base[nt][e] = m;
 						limit[nt][e] = m + FA_SLACK;
 					}
 				}
-				// A unit may grow as much, and the sum in it stays as it is; as far as these positions' weights let it.
+				// A unit may grow as much, and the sum in it hardly changes; as far as these positions' weights let it.
 				float w[2][4];
 				#pragma unroll
 				for (int i = 0; i < 8; ++i) { w[i / 4][i % 4] = exp2_fast(s[i / 4][nt][i % 4] - base[nt][i & 1]); }
-				const float keep[2] = {power_of(127 - back[0]), power_of(127 - back[1])};
 				total[nt][0] *= keep[0];
 				total[nt][1] *= keep[1];
 				#pragma unroll
@@ -628,7 +630,7 @@ four_attend_kernel(const AttendParams p)
 					float2 & unit = *(float2 *)(s_unit + gr * COLS + nt * 8 + t * 2);
 					const int was[2] = {exponent_of(unit.x), exponent_of(unit.y)};
 					const int now[2] = {unit_for(most.x, min(was[0] + back[0], FA_MOST_UNIT)), unit_for(most.y, min(was[1] + back[1], FA_MOST_UNIT))};
-					const float by[2] = {power_of(127 + now[0] - was[0] - back[0]), power_of(127 + now[1] - was[1] - back[1])};
+					const float by[2] = {keep[0] * power_of(127 + now[0] - was[0]), keep[1] * power_of(127 + now[1] - was[1])};
 					__syncwarp();
 					unit = make_float2(power_of(now[0]), power_of(now[1]));       // (the same from the eight lanes of a column)
 					#pragma unroll

@@ -270,3 +270,22 @@ def test_rows_inside_a_table_that_is_too_short_are_read_back():
         # one fma, rounded to fp32
         assert (np.abs(double(got[0, :2]) - want) <= np.abs(want) * 2.0 ** -23).all()
         assert not got[0, 2:].any() and not got[1].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("dim, group, share", [(64, 32, 4), (128, 128, 1), (96, 32, 9), (256, 64, 2)])
+def test_a_token_that_sees_one_position_gets_its_values(dtype, dim, group, share):
+    """The first token of a sequence, and any behind a window of one: the values as they are, rounded once.  (Scales and lows of few bits, so
+    that every step of the sums is exact in fp32; a last bit off would send values half way between two of a type's the wrong way.)"""
+    s = Sequences([1, 40, 17, 300], 2, dim, group, 16, seed=7)
+    c = s.cache
+    c.v_scales[..., 0] = torch.randint(1, 2000, c.v_scales.shape[:-1], generator=rng(1)).mul(2.0 ** -13).half().cuda()
+    c.v_scales[..., 1] = torch.randint(-2000, 2000, c.v_scales.shape[:-1], generator=rng(2)).mul(2.0 ** -9).half().cuda()
+    q = torch.randn(4, 1, 2 * share, dim, generator=rng(3)).to(dtype).cuda()
+    table, lengths = s.device()
+    got = F.attend4(c, q, table, lengths, window=1).cpu()
+    _, _, codes, scales = s.buffers()
+    for b, n in enumerate(s.lengths):
+        page, place = s.table[b][(n - 1) // 16], (n - 1) % 16
+        v = torch.from_numpy(R.values(codes[page, :, place], scales[page, :, place], group, dim)[0])
+        assert torch.equal(got[b, 0], v.to(dtype).repeat_interleave(share, 0))
