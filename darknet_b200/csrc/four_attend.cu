@@ -28,9 +28,11 @@ static AttendPlan plan_attend(const xnor_b200_kv4_cache & c, const xnor_b200_kv4
 	long long most = (long long)r.max_pages * c.page;                          // positions that a tile may see
 	if (window > 0 && most > (long long)window + r.tokens) { most = (long long)window + r.tokens; }
 	const long long steps = (most + 15) / 16, sms = sm_count();
-	// A CTA costs about 2 us of an SM's time before and after its steps, and hides latency for the others: up to two on an SM as long as
-	// each of their warps has a pair of steps, more where the steps are many (8 heads of 128 channels by 64, one sequence, us at 2 / 3 / 4
-	// CTAs on an SM: 16384 positions 13.5 / - / 16.6, 65536 25.6 / - / 27.9, 131072 42.7 / 42.1 / 43.5, 262144 74.7 / - / 70.9).
+	// A CTA costs about 2 us of an SM's time before and after its steps, and hides latency for the others; its sums have to be joined: up to two
+	// on an SM as long as each of their warps has a pair of steps, more where the steps are many.  One sequence, us at 2 / 3 / 4 CTAs on an
+	// SM: 8 heads of 128 channels by 64, 16384 positions 18.8 / 18.9 / 16.4, 65536 44 / 34.7 / 29.3, 131072 78 / 59 / 48.4, 262144 145 / 104 / 82;
+	// 8 heads of 64 by 32, 16384 15.5 / 15.5 / 15.0, 65536 33 / 30.5 / 26, 131072 56 / 49 / 40.5; 2 heads of 64 by 16 (four times the splits a
+	// head to join), 32768 14.5 / 14.5 / 16.1, 65536 16.7 / 16.7 / 20.9, 131072 20.9 / 22.5 / 23.8, 262144 29.7 / 30.0 / 29.2.
 	const int on_sm = attend_on_sm(c.dim / 32, a.nt);
 	long long splits = 1;
 	for (int k = 1; k <= on_sm; ++k)

@@ -8,18 +8,20 @@
 //   out     [16 channels x 8 columns] += (codes of v - 8) . (p * scale_v), and sum(p * (low_v + 8 * scale_v)) beside it in fp32
 // (around the middle code, so that the two hardly cancel).
 // q and p * scale_v are fp16 next to powers of two of their own (q: of the column; p * scale_v: of the largest of the column and the group so
-// far); p * scale_v is two parts, fp32 calls' q too.  The running maximum moves only when a score passes it by more than 2^8 (as others do
-// it), so most steps neither exchange it nor rescale.
+// far); p * scale_v is two parts, fp32 calls' q too.  The running maximum moves only when a score passes it by more than 2^8 (a published
+// refinement of the running softmax), so most steps neither exchange it nor rescale.
 //
 // A CTA has four warps that share a run of positions, two steps by two, each with a ring of its own; then their sums meet in shared memory.
 // Long sequences are split over CTAs: up to eight of them are a cluster and meet in its shared memory, more leave their sums in the
 // scratch buffer and a second kernel joins them.  Everything is summed in a fixed order.
 //
-// What bounds it: issue slots.  32 positions of 128 channels in one group take some 590 instructions of a warp for the 4.4 KB they come
-// in, 176 of them the masks and shifts of the codes (on a pipe of half the rate); one sequence of 131072 tokens, 8 heads of keys and 64 of
-// queries, is read at 4.9 TB/s once it runs, 3.5 TB/s from launch to end (40 us; the copy rate is 6.5 TB/s).  Before and after its steps
-// a CTA costs 1000 instructions a warp: calls of few positions are that and a chain of four loads (lengths, table, codes, sums): 6 us.
-// Tried and slower: five CTAs on an SM (96 registers: 50 against 45 us), three stages (52).
+// What bounds it: issue slots, where a tile of columns is enough.  32 positions of 128 channels in one group take some 705 instructions of a
+// warp for the 4.4 KB they come in, 176 of them the masks and shifts of the codes (on a pipe of half the rate), 32 the additions of their sums;
+// one sequence of 131072 tokens, 8 heads of keys and 64 of queries, is read at 4.3 TB/s once it runs, 2.9 TB/s from launch to end (48 us; the
+// copy rate is 6.5 TB/s).  Before and after its steps a CTA costs 900 instructions a warp: calls of few positions are that and a chain of four
+// loads (lengths, table, codes, sums): 7.6 us.  Three tiles of columns take all registers there are, eight warps on an SM: those wait for
+// one another's results (a third of the issue slots in use).  Tried and slower: five CTAs on an SM (96 registers: 50 against 45 us, of an
+// earlier build), three stages (52).
 #pragma once
 
 #include <cooperative_groups.h>
@@ -139,7 +141,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v)
 }
 
 // fp16 parts of queries and of weights times scales.  Weights of 11 bits show, in bf16 calls too: of 64 sequences' results one in ten was not
-// the bf16 value next to the exact one, with two parts one in 650 is not (a twelfth of the time: 39.5 us for 35.9).
+// the bf16 value next to the exact one, with two parts one in 1600 is not (a tenth of the time: 39.5 us for 35.9).
 template <class T> struct Parts { static constexpr int Q = 1, P = 2; };
 template <> struct Parts<float> { static constexpr int Q = 2, P = 2; };
 
@@ -765,7 +767,8 @@ four_attend_kernel(const AttendParams p)
 	}
 
 	// The next kernel (the one that joins, too) may be launched once every CTA is through its steps.  Before, its CTAs would fill the SMs that
-	// are done first, and go to work on those alone (64 sequences of up to 2048 tokens, one call behind the other: 40 us, 36 from here).
+	// are done first, and go to work on those alone (64 sequences of up to 2048 tokens, one call behind the other, an earlier build: 40 us, 36
+	// from here).
 	pdl_trigger();
 
 	// ---- the warps' sums meet

@@ -11,10 +11,11 @@
 // operand's values: times 2^24 that passes fp32's range where they are 2^117 and more).
 //
 // fp32 and fp16 calls take code - 8 instead, as value = (low + 8 * scale) + scale * (code - 8): the sums of a group's two terms, which rounding
-// (and the tensor cores' cutting off) is relative to, then hardly cancel.  1024 + code in fp16 is the same mask with the exponent's bits
-// set, one addition takes 1032 off; 1024 + 16 * code, times 1/16, less 72.  Four more operations for eight codes (of a product of few rows
-// 2 to 10 % of the time: 16384 x 16384 by one row 34.7 us, by 16 51.7 and 47.6), and a product of 1024 fp32 values is 2e-7 off where it was
-// 1.3e-6; of fp16 results 0.02 % are not the nearest to the exact ones where 1.9 % were not (4096 x 4096; the sums in plain fp32: 0.15 %).
+// (and the tensor cores' cutting off) is relative to, then hardly cancel.  1024 + code in fp16 is the same mask with the exponent's bits set
+// (the common way from small integers to floats), one addition takes 1032 off; 1024 + 16 * code, times 1/16, less 72.  Four more operations
+// for eight codes (2 to 10 % of a product's time: 16384 x 16384 by one row 38.2 and 34.7 us, by 16 51.7 and 47.6), and a product of 1024 fp32
+// values is 2e-7 off where it was 1.3e-6; of fp16 results 0.02 % are not the nearest to the exact ones where 1.9 % were not (4096 x 4096; the
+// sums in plain fp32: 0.15 %).
 // bf16 results are too coarse to show it (16384 x 16384: 0.17 %, in plain fp32 0.13 %).
 #pragma once
 
@@ -212,8 +213,9 @@ template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile
 __device__ __forceinline__ uint32_t four_smem(const void * p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // Power of two that brings values of this largest magnitude (its bits) to [2^13, 2^14), and its inverse: fp16 then holds all 11 bits of
-// anything down to 2^-27 of the largest, and its error is at most 2^-38 of the largest below that.  An infinity or a NaN: the factor is 0
-// and the inverse NaN, so that every sum over the values is NaN.
+// anything down to 2^-27 of the largest, and its error is at most 2^-38 of the largest below that.  Odd neighbours of bf16 calls, divided by
+// 16: 2^-23 and 2^-34; bf16's own 8 bits are all there down to 2^-26 of the largest (even neighbours: 2^-30).  An infinity or a NaN: the
+// factor is 0 and the inverse NaN, so that every sum over the values is NaN.
 __device__ __forceinline__ void fit_f16(uint32_t largest, float & factor, float & inverse)
 {
 	const uint32_t e = max(largest >> 23, 14u);

@@ -3,16 +3,18 @@
 // forward_connected_layer of Darknet (src-lib/connected_layer.cpp) with packed weights, one to some sixteen rows.  A group's sum is
 // scale * sum(x * code) + low * sum(x): the codes go into the tensor cores as they lie (four_common.cuh), and scale and low come in once a
 // group.  x is converted once a block of 256 neighbours, to fp16 next to a power of two of the block's own (fp32: to two fp16 parts,
-// multiplied one after the other), which loses nothing of a 16-bit x.
+// multiplied one after the other), which loses nothing of a 16-bit x down
+// to some 2^-26 of the block's largest value, and next to nothing of that value below (fit_f16).
 //
 // A CTA has eight warps of 16 or 32 filters and a slice of the neighbours; each warp copies its own codes into a ring of its own, so that
 // only the conversion of x, a turn ahead, is waited for.  The slices of the same filters are a cluster: their sums meet in shared memory, in
 // a fixed order, so results do not vary.
 //
-// What bounds it: one row of 16384 x 16384 runs at 4.3 TB/s (33 us; the copy rate is 6.5 TB/s) with issue slots half full, 16 rows of bf16
-// at 3.1 (46 us): the tensor pipe 38% busy, clusters of four on 132 of 148 SMs, the barrier of a block.  Tried and slower by 16 rows: seven
+// What bounds it: one row of 16384 x 16384 runs at 4.1 TB/s in bf16 (34.8 us; the copy rate is 6.5 TB/s), 3.7 in fp16 (38.1), 16 rows of bf16
+// at 3.0 (47.6 us).  No unit is full (integer pipe 46 and 34 %, tensor pipe 23 and 38 %, issue slots 56 and 44 %, DRAM 42 and 35 %): 256 CTAs
+// on 132 of 148 SMs with one or two steps of codes on their way, that come to a barrier every block.  Tried and slower by 16 rows: seven
 // warps, whose 74 clusters do not fit at a time (66 us), barriers every other block with twice the room for x (52).  Up to 4096 x 4096
-// (8 MB from the L2, 5 us) it is a chain of latencies: launch, x, codes, the cluster's sums.
+// (8 MB from the L2, 6 us) it is a chain of latencies: launch, x, codes, the cluster's sums.
 #include <cooperative_groups.h>
 
 #include <climits>
@@ -392,8 +394,10 @@ four_product_kernel(const ProductParams p)
 	cluster.sync();                                                                   // nobody leaves while its sums are read
 }
 
-// Large products of many rows: every CTA would convert all of x again, a fifth of its work (16384 x 16384 by 16 rows of bf16: 55 us, 46 with
-// a kernel for that; fp32 rows, whose parts are twice as much to copy, gain nothing: 8192 x 8192 by 12 rows 38 against 26).
+// Large products of many rows: every CTA would convert all of x again, a fifth of its work.  By 16 rows of bf16 in groups of 128, us with a
+// kernel for that / without: 2^24 weights 11.8 / 9.4, 2^26 18.3 / 19.4, 12288 x 8192 33.6 / 40.5, 2^27 27.5 / 32, 2^28 47.5 / 57 (groups of 32:
+// 2^26 24.2 / 23.7, 12288 x 8192 48.9 / 47.8, 2^27 41 / 43, 2^28 74 / 80).  fp32 rows, whose parts are twice as much to copy, gain nothing:
+// 8192 x 8192 by 12 rows 38 against 26.
 static bool wants_ready(int n, int k, int dtype, int rows)
 {
 	return rows > 8 && dtype != XNOR_B200_F32 && (long long)n * k >= (1LL << 27);
@@ -445,8 +449,8 @@ static int launch_product_shape(ProductParams & p, int dtype, void * scratch, cu
 			if (wants_ready(p.n, p.k, dtype, p.rows)) { return launch_product<T, NT, 2, 8, GROUP, true>(p, scratch, stream); }
 		}
 		// 256 filters of a CTA share its x and its loads of x, 128 fill the SMs where there are few, and are all that the registers of fp32
-		// rows and the sums of small groups leave room for (us with 256 / 128: one row 16384 x 16384 33 / 41, 8192 x 8192 12.2 / 13.4, 4096 x
-		// 4096 6.9 / 5.4; groups of 32, 4096 x 16384 by 8 rows 17.4 / 16.9; fp32, 8192 x 8192 by 12 rows 28 / 26)
+		// rows and the sums of small groups leave room for (us with 256 / 128, one row of bf16: 16384 x 16384 34.8 / 40.4, 8192 x 8192
+		// 13.0 / 14.2, 4096 x 4096 7.4 / 6.2; groups of 32, 4096 x 16384 by 8 rows 17.4 / 16.9; fp32, 8192 x 8192 by 12 rows 28 / 26)
 		const int blocks = (p.k + FP_K - 1) / FP_K;
 		if constexpr (GROUP > 32)
 		{

@@ -10,8 +10,9 @@
 // what a thread has to do rather than by memory, so: the minimum and the maximum of 16-bit values are taken in pairs; the scale is one
 // product and a check; the quotient is a product with 1/scale, whose nearest integer is the bits of its sum with 1.5 * 2^23, and the
 // remainder tells whether it is close to a half and which way it has to go; what fp16 cannot hold and NaN show in the minimum and the
-// maximum.  4 x 2048 tokens (three quarters of them new) of 8 heads of 128 fp16 channels, keys and values: 15 us, 2.2 TB/s; 29 with
-// divisions and 8 neighbours a thread.  The other way 10 us, 3.3 TB/s.
+// maximum.  4 x 2048 tokens (three quarters of them new) of 8 heads of 128 fp16 channels, keys and values: 13.6 us, 2.5 TB/s; 29 with
+// divisions and 8 neighbours a thread.  The other way 9.4 us, 3.6 TB/s.  A matrix of 16384 x 16384 fp32 values: 199 us, 6.2 TB/s; 4096 x 4096
+// of fp16, from the L2, 18.6 us.
 #include "four_common.cuh"
 
 namespace xnor
