@@ -62,6 +62,18 @@ Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const c10::Device & d)
 
 struct Failed {};                 // a Python error is set
 
+[[noreturn]] void refuse(const char * what)
+{
+	PyErr_SetString(PyExc_ValueError, what);
+	throw Failed();
+}
+
+// A handle's buffers may have been resized or given other memory since it was made: the kernels go by the sizes.
+void as_made(bool still)
+{
+	if (!still) { refuse("a buffer of the handle is not the one it was made with: it has been resized or set to other memory"); }
+}
+
 void out_of_memory(const char * what)
 {
 	PyObject * torch = PyImport_ImportModule("torch");
@@ -231,12 +243,6 @@ bool same(const Tensor & a, const Tensor & b)
 	return true;
 }
 
-[[noreturn]] void refuse(const char * what)
-{
-	PyErr_SetString(PyExc_ValueError, what);
-	throw Failed();
-}
-
 // ---- products: ((codes, scales, k, group), x, biases, activation, out)
 PyObject * product(PyObject *, PyObject * const * args, Py_ssize_t n_args)
 {
@@ -249,6 +255,10 @@ PyObject * product(PyObject *, PyObject * const * args, Py_ssize_t n_args)
 		if (codes->dim() != 2) { Py_RETURN_NONE; }
 		const int64_t n = codes->size(0), k = whole(PyTuple_GET_ITEM(args[0], 2));
 		if (n > INT_MAX || k > INT_MAX) { Py_RETURN_NONE; }
+		const int64_t group = whole(PyTuple_GET_ITEM(args[0], 3));
+		as_made(k > 0 && group > 0 && codes->scalar_type() == at::kByte && codes->size(1) == (k + 31) / 32 * 16 && codes->is_contiguous()
+				&& scales->scalar_type() == at::kHalf && scales->dim() == 3 && scales->size(0) == n && scales->size(1) == (k + group - 1) / group && scales->size(2) == 2
+				&& scales->is_contiguous());
 		const c10::Device d = codes->device();
 		const int type = type_of(*x);
 		if (!on(*codes, d) || !on(*scales, d) || !on(*x, d) || type < 0 || x->dim() != 2 || x->size(1) != k || (k != 1 && x->stride(1) != 1)) { Py_RETURN_NONE; }
@@ -272,7 +282,7 @@ PyObject * product(PyObject *, PyObject * const * args, Py_ssize_t n_args)
 		if (rows == 0) { return THPVariable_Wrap(out); }
 		const long long activation = whole(args[3]);
 		if (rows > INT_MAX || activation < 0 || activation > 1) { Py_RETURN_NONE; }
-		const xnor_b200_w4_desc desc = {(int)n, (int)k, (int)whole(PyTuple_GET_ITEM(args[0], 3)), (int)activation};
+		const xnor_b200_w4_desc desc = {(int)n, (int)k, (int)group, (int)activation};
 		const size_t bytes = xnor_b200_w4_scratch_bytes(&desc, type, (int)rows);
 		const Tensor scratch = bytes != 0 ? empty({(int64_t)bytes}, at::kByte, d) : Tensor();
 		void * const stream = (void *)c10::cuda::getCurrentCUDAStream(d.index()).stream();
@@ -295,15 +305,22 @@ bool take_cache(PyObject * o, xnor_b200_kv4_cache & c, std::optional<c10::Device
 	{
 		if (!take(PyTuple_GET_ITEM(o, i), t[i]) || t[i] == nullptr) { return false; }
 	}
+	const at::IntArrayRef s = t[0]->sizes();
+	if (s.size() != 4 || s[0] > INT_MAX || s[1] > INT_MAX || s[2] > INT_MAX || s[3] > INT_MAX / 2) { return false; }
+	const int64_t group = whole(PyTuple_GET_ITEM(o, 4));
+	for (int i = 0; i < 4; i += 2)
+	{
+		const Tensor & codes = *t[i], & scales = *t[i + 1];
+		as_made(group > 0 && codes.scalar_type() == at::kByte && codes.sizes() == s && codes.is_contiguous() && scales.scalar_type() == at::kHalf && scales.dim() == 5
+				&& scales.sizes().slice(0, 3) == s.slice(0, 3) && scales.size(3) == 2 * s[3] / group && scales.size(4) == 2 && scales.is_contiguous());
+	}
 	d = t[0]->device();
 	for (const Tensor * v : t)
 	{
 		if (!on(*v, *d)) { return false; }
 	}
-	const at::IntArrayRef s = t[0]->sizes();
-	if (s.size() != 4 || s[0] > INT_MAX || s[1] > INT_MAX || s[2] > INT_MAX || s[3] > INT_MAX / 2) { return false; }
 	c = {(uint8_t *)t[0]->data_ptr(), t[1]->data_ptr(), (uint8_t *)t[2]->data_ptr(), t[3]->data_ptr(), (int)s[0], (int)s[1], (int)s[2], (int)(2 * s[3]),
-			(int)whole(PyTuple_GET_ITEM(o, 4))};
+			(int)group};
 	return true;
 }
 

@@ -236,3 +236,23 @@ def test_attention_over_prompts_has_the_limit_that_the_header_names(L):
         return L.xnor_b200_kv4_attend(c, r, t, heads, 1.0, 0, t, None, None, 0, None)
     assert attend(65535 // 8 * 2 + 2, 32, 8, 256) == 6 and attend(65535 // 8 * 6 + 6, 32, 8, 128) == 6
     assert attend(1, 32, 65536, 64) in (1, 6) and attend((1 << 31) - 1, 64, 1, 64) == 6
+
+
+def test_handles_whose_buffers_have_changed_are_refused(L):
+    """The attributes are fixed, the tensors are the caller's: one that has been resized would be read and written beyond its end."""
+    i32 = dict(dtype=torch.int32)
+    x = torch.zeros(1, 64)
+    for change in (lambda m: m.codes.resize_(9, 32), lambda m: m.scales.resize_(4, 1, 2), lambda m: m.scales.set_(torch.zeros(1, dtype=torch.float16)),
+                   lambda m: m.codes.t_()):
+        m = F.Matrix4(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, 2, dtype=torch.float16), 64, 32)
+        change(m)
+        with pytest.raises(ValueError, match="made with"):
+            F.forward_connected4(m, x)
+    kv, table, lengths = torch.zeros(1, 1, 2, 64), torch.zeros(1, 2, **i32), torch.zeros(1, **i32)
+    for change in (lambda c: c.k_codes.resize_(4, 2, 16, 32), lambda c: c.v_codes.resize_(1, 2, 16, 32), lambda c: c.k_scales.resize_(3, 2, 16, 1, 2),
+                   lambda c: c.v_scales.set_(torch.zeros(5, dtype=torch.float16)), lambda c: c.v_codes.transpose_(0, 1)):
+        c = F.new_cache4(3, 2, 16, 64, 32, device="cpu")
+        change(c)
+        for call in (lambda: F.append4(c, kv, kv, table, lengths), lambda: F.read4(c, table, lengths, 1), lambda: F.attend4(c, kv, table, lengths)):
+            with pytest.raises(ValueError, match="made with"):
+                call()
