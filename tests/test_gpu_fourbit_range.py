@@ -289,3 +289,41 @@ def test_a_token_that_sees_one_position_gets_its_values(dtype, dim, group, share
         page, place = s.table[b][(n - 1) // 16], (n - 1) % 16
         v = torch.from_numpy(R.values(codes[page, :, place], scales[page, :, place], group, dim)[0])
         assert torch.equal(got[b, 0], v.to(dtype).repeat_interleave(share, 0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=ids)
+def test_large_products_in_graphs_and_on_two_streams(dtype):
+    """Those whose rows are converted by a kernel in front: captured, behind a kernel that writes the rows and one that writes the scales,
+    replayed on two streams at a time."""
+    n, k, rows = 16384, 8192, 9
+    m = [matrix(n, k, 64, i) for i in range(2)]
+    base = [x.scales.clone() for x in m]
+    xs = [torch.zeros(rows, k, dtype=dtype, device="cuda") for _ in m]
+    halves = [torch.zeros(1, dtype=torch.float16, device="cuda") for _ in m]
+
+    def work(i):
+        m[i].scales.copy_(base[i] * halves[i])
+        return F.forward_connected4(m[i], xs[i] * 2)
+
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in m]
+    for i in range(2):
+        work(i)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(work(i))
+    for turn in range(6):
+        for i in range(2):
+            xs[i].copy_(torch.randn(rows, k, generator=rng(10 * turn + i)))
+            halves[i].fill_(0.5 if turn % 2 else 1.0)
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        got = [y.clone() for y in outs]
+        for i in range(2):
+            assert torch.equal(got[i], work(i))
+    picked = torch.arange(0, n, 411).cuda()
+    part = F.Matrix4(m[0].codes[picked].contiguous(), m[0].scales[picked].contiguous(), k, 64)
+    check_product(part, xs[0] * 2, work(0)[:, picked])
