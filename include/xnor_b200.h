@@ -664,8 +664,9 @@ XNOR_B200_API int xnor_b200_kv4_read(const xnor_b200_kv4_cache * cache, const xn
  * kv_heads; heads / kv_heads neighbours share a head of keys), output = sum_j softmax_j(scale * q . k_j) v_j.  q and output:
  * [batch][tokens][heads][dim] of one type; output may be q itself, and has no other memory in common with it.  A row that sees nothing, and rows of
  * counts[b] and above, are 0.  lse: fp32 [batch][tokens][heads] or NULL, receives log(sum_j exp(scale * q . k_j)), -infinity where nothing is
- * seen.  Scores, softmax and sums are fp32, of weights and fp32 queries to 22 bits; results are rounded once.  What lies behind a sequence's
- * length in its last page is never counted.
+ * seen.  Scores, softmax and sums are fp32, fp32 queries taken to 22 bits, and a weight times its value's scale, too (or to 2^-31 of the
+ * largest of those that the output sums, where that is more); results are rounded once.  What lies behind a sequence's length in its last
+ * page is never counted.
  * A call's grid has room for 65535 tiles of columns, a column being a token's head of queries: ceil(tokens * heads / kv_heads / 8) * kv_heads,
  * in eights up to dim 256, in up to 24s up to dim 128 (32 heads: some 16 000 tokens of a sequence a call, and some 49 000).  Beyond, and for
  * more than 65535 sequences or heads of keys, XNOR_B200_ERR_TOO_LARGE: a longer prompt takes several calls.
