@@ -590,7 +590,7 @@ four_attend_kernel(const AttendParams p)
 			#pragma unroll
 			for (int nt = 0; nt < NT; ++nt)
 			{
-				float keep[2];                                    // what there is counts for that much of what it did: 2^-back, and not quite half of it
+				float keep[2];                                    // what there is counts for that much of what it did: 2^-back down to half of that
 				int back[2];
 				#pragma unroll
 				for (int e = 0; e < 2; ++e)
